@@ -373,6 +373,139 @@ TKV_API int tkv_exchange_merge(const tkv_exchange_t* ex, int num_seqs, int num_q
                                void* stream);
 
 /* ---------------------------------------------------------------- */
+/* Rotary positions with several axes                                 */
+/* ---------------------------------------------------------------- */
+/* The step before the cache: query and key channels are turned in pairs by
+ * angle = position * theta^(-2 i / rotary_dim), i = 0 .. rotary_dim/2 - 1.
+ * Every token has one position per axis (time, height, width for images and
+ * video; all equal for text; one axis is the ordinary rotary embedding), and
+ * every pair i belongs to one axis.  The reference rotates with one axis only
+ * (third_party/custom_kernels/megakernel.cu, its rotary step). */
+#define TKV_ROPE_MAX_PAIRS 128
+#define TKV_ROPE_MAX_AXES 8
+#define TKV_ROPE_HALVES 0   /* pair i is channels (i, i + rotary_dim / 2)     */
+#define TKV_ROPE_ADJACENT 1 /* pair i is channels (2 i, 2 i + 1)              */
+#define TKV_ROPE_BLOCKS 0      /* axis a owns the next sections[a] pairs      */
+#define TKV_ROPE_ROUND_ROBIN 1 /* pairs go to the axes in turn, while an axis */
+                               /* has pairs of its section left               */
+typedef struct tkv_rope_plan {
+  int32_t rotary_dim, n_axes, pairing, reserved;
+  double turns[TKV_ROPE_MAX_PAIRS];  /* revolutions per position: theta^(-2i/r) / (2 pi) */
+  uint8_t axis[TKV_ROPE_MAX_PAIRS];  /* axis of pair i, < n_axes                         */
+} tkv_rope_plan_t;
+/* Fills *plan (host memory).  rotary_dim: a multiple of 16 up to 256; sections
+ * [n_axes] >= 0, their sum rotary_dim / 2; theta > 0 and finite; order and
+ * pairing as above.  A caller with scaled frequencies changes plan->turns. */
+TKV_API int tkv_rope_plan_init(tkv_rope_plan_t* plan, int rotary_dim, double theta,
+                               const int32_t* sections, int n_axes, int order, int pairing);
+/* Turns q [n_tokens][num_q_heads][head_dim] and k [n_tokens][num_k_heads]
+ * [head_dim] (fp16 or bf16; k may be NULL with num_k_heads 0) into q_out and
+ * k_out; channels from rotary_dim on are copied.  q_out == q (k_out == k) with
+ * the same strides turns in place; other overlaps are not allowed.  strides[8]:
+ * token and head strides in elements of q, k, q_out, k_out, in that order, all
+ * multiples of 8; data pointers 16-byte aligned.  positions: int32
+ * [n_axes][n_tokens], axes axis_stride elements apart.  inverse != 0 turns by
+ * the negative angles, which undoes the rotation and is its gradient.  Angles
+ * are reduced in 64 bits, so far positions keep their precision.  One launch. */
+TKV_API int tkv_rope_axes(const tkv_rope_plan_t* plan, const void* q, const void* k, void* q_out,
+                          void* k_out, int dtype, int num_q_heads, int num_k_heads, int head_dim,
+                          int n_tokens, const int64_t* strides, const int32_t* positions,
+                          int64_t axis_stride, int inverse, void* stream);
+
+/* ---------------------------------------------------------------- */
+/* Paged int8 cache                                                   */
+/* ---------------------------------------------------------------- */
+/* An 8-bit cache with the KIVI cache's block tables and 16-token pages and no
+ * residual ring: every token is quantised as it is written.  The D values x of
+ * one (token, kv head) share one 32-bit scale s = max|x| / 127 (rounded to
+ * f32) and become codes round(x / s), halves to even, stored as code + 128; a
+ * code stands for code * s.  A row of zeros, or one whose s is below the
+ * smallest normal float, has s = 0; a row with a NaN or an infinity has s =
+ * NaN and reads back as NaN.  The bytes do not depend on how tokens were split
+ * into append calls.
+ *
+ * Page pool (per layer): [num_pages][n_kv_heads][page_bytes], page_bytes =
+ * 32 D + 128 (4224 for D = 128, 2176 for D = 64).  One (page, head) block:
+ *   K codes [D/16 chunks][16 slots][16 channels]: token t of chunk c (channels
+ *           16 c ..) sits in slot t ^ (2 (c % 4)).  (16-byte units that the
+ *           attention kernels read and store without bank conflicts.)
+ *   V codes [D/32][8][4][4][4]: channel 32 u + 4 g + j of token 4 t + i at
+ *           [u][g][t][j][i].  (Four tokens of a channel are one 32-bit word:
+ *           the A-operand registers of mma.m16n8k16 for V^T tiles.)
+ *   scales  [16 tokens][2] f32: the key's, the value's.
+ * Block tables are [num_seqs][max_blocks_per_seq] int32, token p of sequence s
+ * in page block_tables[s][p / 16] (cuda_allocator.cpp:273).  A page is written
+ * as long as its sequence grows into it, so sequences that share a partly
+ * filled page must copy it before either appends. */
+typedef struct tkv_int8_cache {
+  void* pool;         /* [num_pages][n_kv_heads][page_bytes], 16-byte aligned */
+  int32_t num_pages;  /* pages in the pool (bounds for block-table entries)   */
+  int32_t n_kv_heads;
+  int32_t head_dim;   /* 64 or 128 */
+  int32_t reserved;
+} tkv_int8_cache_t;
+
+/* Bytes of one (page, kv head) block; 0 for an unsupported head_dim. */
+TKV_API int64_t tkv_int8_page_bytes(int head_dim);
+
+/* Quantises and writes, for each sequence s, the tokens k_new/v_new
+ * [cu_new[s] .. cu_new[s+1]) after its seq_lens_old[s] existing ones (the
+ * reshape_and_cache slot, cache_kernels.cu:202-232).  k_new, v_new: fp16 or
+ * bf16 [total_new_tokens][n_kv_heads][D] with token and head strides
+ * strides[4] = {k token, k head, v token, v head} in elements (multiples of 8,
+ * 16-byte aligned pointers).  max_new_tokens bounds cu_new[s+1] - cu_new[s].
+ * The block table must cover the new length; two sequences that write the same
+ * page in one call leave it undefined.  Sequences whose offsets or lengths are
+ * out of range are skipped and flagged TKV_ERR_BAD_LENGTH; tokens whose page is
+ * outside the pool are skipped and flagged TKV_ERR_BAD_PAGE.  One launch. */
+TKV_API int tkv_int8_append(const tkv_int8_cache_t* cache, const void* k_new, const void* v_new,
+                            int in_dtype, const int64_t* strides, const int32_t* cu_new,
+                            const int32_t* seq_lens_old, const int32_t* block_tables,
+                            int max_blocks_per_seq, int num_seqs, int total_new_tokens,
+                            int max_new_tokens, int* err_flag, void* stream);
+
+/* Reads tokens back: row cu[s] + i of k_out / v_out [total_tokens][n_kv_heads]
+ * [D] (fp16, bf16 or f32, contiguous, 16-byte aligned; one of them may be NULL)
+ * gets token starts[s] + i of sequence s, i < cu[s+1] - cu[s] <= max_tokens.
+ * Rows outside [cu[0], cu[num_seqs]) and rows of sequences out of range
+ * (flagged TKV_ERR_BAD_LENGTH) are left as they are; tokens whose page is
+ * outside the pool read as zeros and are flagged TKV_ERR_BAD_PAGE.  One launch. */
+TKV_API int tkv_int8_read(const tkv_int8_cache_t* cache, void* k_out, void* v_out, int out_dtype,
+                          const int32_t* block_tables, int max_blocks_per_seq,
+                          const int32_t* starts, const int32_t* cu, int num_seqs, int total_tokens,
+                          int max_tokens, int* err_flag, void* stream);
+
+/* Attention of each sequence's last tokens over its pages (the
+ * paged_attention_v1/v2 slot and the prefill, cuda_engine.cpp:51-62,842-860):
+ * the n_s = cu_q[s+1] - cu_q[s] rows q[cu_q[s] ..) of sequence s are its last
+ * n_s tokens (already appended), at positions p = seq_lens[s] - n_s + i.  Each
+ * attends to the tokens (p - window, p] (window 0: [0, p]):
+ *   out = softmax(scale * q . k) v, kv head = q head / (num_q_heads / n_kv_heads).
+ * n_s = 1 is a decode step; 0 is allowed.  q: fp16 or bf16 [total_q_tokens]
+ * [num_q_heads][D] with token and head strides q_stride[2] in elements
+ * (multiples of 8, 16-byte aligned); out: contiguous, fp16 or bf16, 16-byte
+ * aligned.  Rows outside [cu_q[0], cu_q[num_seqs]) are left as they are.
+ * max_q_tokens bounds n_s and max_context_len bounds seq_lens (they size the
+ * grid and the splits); sequences out of these bounds, with n_s > seq_lens[s]
+ * or longer than their block table are left as they are and flagged
+ * TKV_ERR_BAD_LENGTH.  A block-table entry outside the pool is flagged
+ * TKV_ERR_BAD_PAGE and read as page 0 (that sequence's output is not
+ * meaningful).
+ * workspace: tkv_int8_attend_workspace_bytes(...) bytes for the same sizes,
+ * 16-byte aligned, zeroed once when it is allocated (every call leaves its
+ * counters zero); calls that share one must not overlap on the GPU. */
+TKV_API size_t tkv_int8_attend_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads,
+                                               int head_dim, int max_q_tokens,
+                                               int max_context_len);
+TKV_API int tkv_int8_attend(const tkv_int8_cache_t* cache, const void* q, int q_dtype,
+                            const int64_t* q_stride, void* out, int out_dtype,
+                            const int32_t* cu_q, const int32_t* block_tables,
+                            int max_blocks_per_seq, const int32_t* seq_lens, int num_seqs,
+                            int num_q_heads, int total_q_tokens, int max_q_tokens,
+                            int max_context_len, int window, float scale, void* workspace,
+                            size_t workspace_bytes, int* err_flag, void* stream);
+
+/* ---------------------------------------------------------------- */
 /* Page allocator (host)                                              */
 /* ---------------------------------------------------------------- */
 /* Replaces the bookkeeping of CudaAllocator

@@ -30,6 +30,11 @@ TKV_NOALLOC_SCRATCH_BYTES = 16 << 20
 TKV_MAX_PEERS = 8
 TKV_IPC_HANDLE_BYTES = 64
 
+TKV_ROPE_MAX_PAIRS = 128
+TKV_ROPE_MAX_AXES = 8
+TKV_ROPE_HALVES, TKV_ROPE_ADJACENT = 0, 1
+TKV_ROPE_BLOCKS, TKV_ROPE_ROUND_ROBIN = 0, 1
+
 
 class TkvFormat(C.Structure):
     _fields_ = [
@@ -46,6 +51,17 @@ class TkvCache(C.Structure):
         ("pool", C.c_void_p), ("ring", C.c_void_p), ("num_pages", C.c_int32),
         ("max_seqs", C.c_int32), ("fmt", TkvFormat),
     ]
+
+
+class TkvInt8Cache(C.Structure):
+    _fields_ = [("pool", C.c_void_p), ("num_pages", C.c_int32), ("n_kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("reserved", C.c_int32)]
+
+
+class TkvRopePlan(C.Structure):
+    _fields_ = [("rotary_dim", C.c_int32), ("n_axes", C.c_int32), ("pairing", C.c_int32),
+                ("reserved", C.c_int32), ("turns", C.c_double * TKV_ROPE_MAX_PAIRS),
+                ("axis", C.c_uint8 * TKV_ROPE_MAX_PAIRS)]
 
 
 class TkvExchange(C.Structure):
@@ -72,6 +88,7 @@ class TkvAllocatorStats(C.Structure):
 _vp, _i32, _i64, _sz, _f32 = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float
 _ip = C.POINTER(C.c_int)
 _u64 = C.c_uint64
+_i64p = C.POINTER(C.c_int64)
 
 # name -> (restype, argtypes); every symbol the header declares.
 SIGNATURES = {
@@ -115,6 +132,19 @@ SIGNATURES = {
                                   _vp]),
     "tkv_paged_prefill": (_i32, [C.POINTER(TkvCache), _vp, _i32, _vp, _i32, _vp, _vp, _i32, _vp,
                                  _vp, _i32, _i32, _i32, _i32, _f32, _vp, _vp]),
+    "tkv_rope_plan_init": (_i32, [C.POINTER(TkvRopePlan), _i32, C.c_double, C.POINTER(C.c_int32),
+                                  _i32, _i32, _i32]),
+    "tkv_rope_axes": (_i32, [C.POINTER(TkvRopePlan), _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32,
+                             _i32, _i64p, _vp, _i64, _i32, _vp]),
+    "tkv_int8_page_bytes": (_i64, [_i32]),
+    "tkv_int8_append": (_i32, [C.POINTER(TkvInt8Cache), _vp, _vp, _i32, _i64p, _vp, _vp, _vp,
+                               _i32, _i32, _i32, _i32, _vp, _vp]),
+    "tkv_int8_read": (_i32, [C.POINTER(TkvInt8Cache), _vp, _vp, _i32, _vp, _i32, _vp, _vp, _i32,
+                             _i32, _i32, _vp, _vp]),
+    "tkv_int8_attend_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "tkv_int8_attend": (_i32, [C.POINTER(TkvInt8Cache), _vp, _i32, _i64p, _vp, _i32, _vp, _vp,
+                               _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _f32, _vp, _sz,
+                               _vp, _vp]),
     "tkv_allocator_create": (_i32, [C.POINTER(TkvFormat), _i32, _i32, _i32, C.POINTER(_vp)]),
     "tkv_allocator_destroy": (None, [_vp]),
     "tkv_allocator_pages_for": (_i32, [_vp, _i32]),

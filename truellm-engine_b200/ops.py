@@ -5,11 +5,14 @@ Mirrors, with the same argument meaning:
       src/inference/backends/cuda/compression/kivi_cache.cuh:32-84
   reshape_and_cache  -> paged_append    (cuda_engine.cpp:48-50, cache_kernels.cu:202-232)
   paged_attention_v1/v2 -> paged_decode (cuda_engine.cpp:51-62)
+and, beside the KIVI cache, the paged int8 cache (int8_append, int8_read,
+int8_attend) and rotary positions with several axes (rope_axes).
 Every call goes to the sm_100a library; tensors must be CUDA tensors.
 """
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from dataclasses import dataclass
 from typing import Optional
@@ -483,3 +486,327 @@ def swap_ring_rows(cache: KiviPagedCache, images: torch.Tensor, mapping: torch.T
     L.check("tkv_swap_ring_rows", L.lib().tkv_swap_ring_rows(
         C.byref(c), _ptr(images), int(images.shape[0]), _ptr(mapping), n, int(direction),
         _ptr(err), C.c_void_p(_stream(stream))))
+
+
+# ---------------------------------------------------------------------------
+# rotary positions with several axes, and the paged int8 cache
+# ---------------------------------------------------------------------------
+class _On:
+    """Makes a tensor's device and the call's stream current, so that what a
+    call allocates or copies belongs to the stream its kernel runs on."""
+
+    def __init__(self, device: torch.device, stream):
+        if stream is not None and not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(int(stream), device=device)
+        if stream is not None and stream.device != device:
+            raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
+        self._ctx = []
+        if torch.cuda.current_device() != device.index:
+            self._ctx.append(torch.cuda.device(device))
+        if stream is not None:
+            self._ctx.append(torch.cuda.stream(stream))
+        self._device = device
+
+    def __enter__(self) -> int:
+        for c in self._ctx:
+            c.__enter__()
+        return torch.cuda.current_stream(self._device).cuda_stream
+
+    def __exit__(self, *exc):
+        for c in reversed(self._ctx):
+            c.__exit__(*exc)
+
+
+def _same_device(device: torch.device, *ts) -> None:
+    for t in ts:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors are on {t.device} and {device}: one CUDA device is needed")
+
+
+def _index(name: str, t: torch.Tensor, *shape) -> int:
+    """Address of a contiguous int32 tensor of this shape (None: any size)."""
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != len(shape) or any(
+            n is not None and n != m for n, m in zip(shape, t.shape)):
+        want = ", ".join("*" if n is None else str(n) for n in shape)
+        raise ValueError(f"{name} must be a contiguous int32 [{want}] tensor")
+    return t.data_ptr()
+
+
+def _err_ptr(err: Optional[torch.Tensor]):
+    if err is None:
+        return None
+    if err.dtype != torch.int32 or err.numel() < 1:
+        raise ValueError("err must be an int32 tensor of one word")
+    return err.data_ptr()
+
+
+def _heads(name: str, t: torch.Tensor) -> torch.Tensor:
+    """[T, H, D] fp16/bf16 whose 16-byte vectors the kernels can address: any
+    token and head strides that are multiples of 8 elements, else a copy."""
+    if t.dim() != 3 or t.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{name} must be an fp16 or bf16 [tokens, heads, channels] tensor")
+    st, sh, sd = t.stride()
+    if sd != 1 or st % 8 or sh % 8 or t.data_ptr() % 16:
+        return t.contiguous()
+    return t
+
+
+def _no_grad_path(name: str, *ts) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
+
+
+@functools.lru_cache(maxsize=64)
+def _rope_plan(rotary_dim: int, sections: tuple, theta: float, order: str,
+               pairing: str) -> L.TkvRopePlan:
+    orders = {"blocks": L.TKV_ROPE_BLOCKS, "round_robin": L.TKV_ROPE_ROUND_ROBIN}
+    pairings = {"halves": L.TKV_ROPE_HALVES, "adjacent": L.TKV_ROPE_ADJACENT}
+    if order not in orders or pairing not in pairings:
+        raise ValueError("order is 'blocks' or 'round_robin', pairing 'halves' or 'adjacent'")
+    if not 1 <= len(sections) <= L.TKV_ROPE_MAX_AXES:
+        raise ValueError(f"1 to {L.TKV_ROPE_MAX_AXES} axes are supported")
+    p = L.TkvRopePlan()
+    L.check("tkv_rope_plan_init", L.lib().tkv_rope_plan_init(
+        C.byref(p), rotary_dim, theta, (C.c_int32 * len(sections))(*sections), len(sections),
+        orders[order], pairings[pairing]))
+    return p
+
+
+def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, sections,
+              theta: float = 10000.0, order: str = "blocks", pairing: str = "halves",
+              inverse: bool = False, q_out: Optional[torch.Tensor] = None,
+              k_out: Optional[torch.Tensor] = None, stream=None):
+    """Rotary positions with several axes on queries and keys.
+
+    q: [T, Hq, D], k: [T, Hk, D] (or None), both fp16 or both bf16; positions:
+    int32 [axes, T]; sections: frequency pairs of each axis, their sum half of
+    the rotary channels (channels from 2 * sum(sections) on are copied).  Pair i
+    turns by positions[axis of i] * theta ** (-2 i / rotary_dim); order
+    "blocks" gives axis a the next sections[a] pairs, "round_robin" deals the
+    pairs to the axes in turn; pairing "halves" couples channels (i, i +
+    rotary_dim / 2), "adjacent" (2 i, 2 i + 1).  inverse turns back (and is the
+    gradient; calls on tensors that require one are differentiable).  q_out /
+    k_out may be q / k (in place).  Returns (q_out, k_out)."""
+    ts = (q,) if k is None else (q, k)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        if q_out is not None or k_out is not None:
+            raise ValueError("q_out / k_out cannot be given where a gradient is needed")
+        got = _RopeAxes.apply(q, k, positions, tuple(sections), theta, order, pairing,
+                              inverse, stream)
+        return got if k is not None else (got[0], None)
+    _need_cuda(q, k, positions)
+    _same_device(q.device, k, positions, q_out, k_out)
+    sections = tuple(int(n) for n in sections)
+    rotary = 2 * sum(sections)
+    plan = _rope_plan(rotary, sections, float(theta), order, pairing)
+    with _On(q.device, stream) as s:
+        qx = _heads("q", q)
+        T, Hq, D = qx.shape
+        kx = None if k is None else _heads("k", k)
+        if kx is not None and (kx.shape[0] != T or kx.shape[2] != D or kx.dtype != qx.dtype):
+            raise ValueError("k must have q's tokens, channels and type")
+        if (positions.dtype != torch.int32 or positions.dim() != 2 or
+                tuple(positions.shape) != (len(sections), T) or
+                (T > 1 and positions.stride(1) != 1)):
+            raise ValueError(f"positions must be an int32 [{len(sections)}, {T}] tensor")
+        if q_out is None:
+            q_out = torch.empty((T, Hq, D), dtype=qx.dtype, device=qx.device)
+        if kx is not None and k_out is None:
+            k_out = torch.empty_like(kx, memory_format=torch.contiguous_format)
+        for name, o, x in (("q_out", q_out, qx), ("k_out", k_out, kx)):
+            if o is None or x is None:
+                if o is not None:
+                    raise ValueError("k_out without k")
+                continue
+            if o.shape != x.shape or o.dtype != x.dtype or _heads(name, o) is not o:
+                raise ValueError(f"{name} must have its input's shape and type, contiguous "
+                                 "channels and strides that are multiples of 8")
+        Hk = 0 if kx is None else kx.shape[1]
+        kst, kos = ((0, 0), (0, 0)) if kx is None else (kx.stride(), k_out.stride())
+        qst, qos = qx.stride(), q_out.stride()
+        strides = (C.c_int64 * 8)(qst[0], qst[1], kst[0], kst[1], qos[0], qos[1], kos[0], kos[1])
+        L.check("tkv_rope_axes", L.lib().tkv_rope_axes(
+            C.byref(plan), qx.data_ptr(), None if kx is None else kx.data_ptr(),
+            q_out.data_ptr(), None if kx is None else k_out.data_ptr(), _DT[qx.dtype], Hq, Hk, D,
+            T, strides, positions.data_ptr(), positions.stride(0), int(bool(inverse)), s))
+    return q_out, k_out
+
+
+class _RopeAxes(torch.autograd.Function):
+    """A rotation's gradient is the rotation back."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, sections, theta, order, pairing, inverse, stream):
+        ctx.save_for_backward(positions)
+        ctx.how = (sections, theta, order, pairing)
+        ctx.inverse, ctx.stream, ctx.has_k = inverse, stream, k is not None
+        with torch.no_grad():
+            qo, ko = rope_axes(q, k, positions, sections, theta, order, pairing, inverse,
+                               stream=stream)
+        return (qo, ko) if k is not None else (qo,)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        (positions,) = ctx.saved_tensors
+        with torch.no_grad():
+            gq, gk = rope_axes(grads[0], grads[1] if ctx.has_k else None, positions,
+                               *ctx.how, not ctx.inverse, stream=ctx.stream)
+        return gq, gk, None, None, None, None, None, None, None
+
+
+class Int8PagedCache:
+    """Device buffer of one layer's paged int8 cache: pool [num_pages,
+    n_kv_heads, page_bytes] uint8, allocated zeroed, or the caller's (pool=)."""
+
+    def __init__(self, n_kv_heads: int, head_dim: int, num_pages: Optional[int] = None,
+                 device="cuda", pool: Optional[torch.Tensor] = None):
+        self.n_kv_heads, self.head_dim = int(n_kv_heads), int(head_dim)
+        self.page_bytes = int(L.lib().tkv_int8_page_bytes(self.head_dim))
+        if not self.page_bytes:
+            raise ValueError(f"head_dim {head_dim}: 64 and 128 are supported")
+        if (num_pages is None) == (pool is None):
+            raise ValueError("give either num_pages or a pool")
+        if pool is None:
+            pool = torch.zeros((num_pages, self.n_kv_heads, self.page_bytes), dtype=torch.uint8,
+                               device=device)
+        elif (pool.dtype != torch.uint8 or not pool.is_cuda or not pool.is_contiguous() or
+              tuple(pool.shape[1:]) != (self.n_kv_heads, self.page_bytes) or pool.dim() != 3):
+            raise ValueError(f"pool must be a contiguous CUDA uint8 [pages, {self.n_kv_heads}, "
+                             f"{self.page_bytes}] tensor")
+        self.pool = pool
+        self.num_pages = int(pool.shape[0])
+        self._c = L.TkvInt8Cache(pool.data_ptr(), self.num_pages, self.n_kv_heads, self.head_dim, 0)
+
+    def c_struct(self) -> L.TkvInt8Cache:
+        return self._c
+
+
+def int8_append(cache: Int8PagedCache, k_new: torch.Tensor, v_new: torch.Tensor,
+                cu_new: torch.Tensor, seq_lens_old: torch.Tensor, block_tables: torch.Tensor,
+                max_new_tokens: Optional[int] = None, err: Optional[torch.Tensor] = None,
+                stream=None) -> None:
+    """Quantises K/V as they are written into the int8 pages.
+
+    k_new, v_new: [T, n_kv_heads, D], both fp16 or both bf16, any token and head
+    strides that are multiples of 8 (slices of a fused projection are read where
+    they lie); cu_new [B+1], seq_lens_old [B], block_tables [B, max_blocks]
+    int32; max_new_tokens bounds a sequence's new tokens (default T)."""
+    _need_cuda(k_new, v_new, cu_new, seq_lens_old, block_tables)
+    _no_grad_path("int8_append", k_new, v_new)
+    dev = cache.pool.device
+    _same_device(dev, k_new, v_new, cu_new, seq_lens_old, block_tables, err)
+    B = int(seq_lens_old.shape[0]) if seq_lens_old.dim() == 1 else -1
+    with _On(dev, stream) as s:
+        k, v = _heads("k_new", k_new), _heads("v_new", v_new)
+        if k.shape != v.shape or k.dtype != v.dtype or k.shape[1:] != (cache.n_kv_heads,
+                                                                      cache.head_dim):
+            raise ValueError(f"k_new and v_new must both be [tokens, {cache.n_kv_heads}, "
+                             f"{cache.head_dim}] of one type")
+        T = int(k.shape[0])
+        ks, vs = k.stride(), v.stride()
+        L.check("tkv_int8_append", L.lib().tkv_int8_append(
+            C.byref(cache._c), k.data_ptr(), v.data_ptr(), _DT[k.dtype],
+            (C.c_int64 * 4)(ks[0], ks[1], vs[0], vs[1]), _index("cu_new", cu_new, B + 1),
+            _index("seq_lens_old", seq_lens_old, B), _index("block_tables", block_tables, B, None),
+            block_tables.shape[1], B, T, T if max_new_tokens is None else int(max_new_tokens),
+            _err_ptr(err), s))
+
+
+def int8_read(cache: Int8PagedCache, block_tables: torch.Tensor, starts: torch.Tensor,
+              cu: torch.Tensor, total_tokens: int, max_tokens: Optional[int] = None,
+              dtype: torch.dtype = torch.float16, k_out: Optional[torch.Tensor] = None,
+              v_out: Optional[torch.Tensor] = None, err: Optional[torch.Tensor] = None,
+              stream=None):
+    """Reads tokens back from the int8 pages: row cu[s] + i of the returned K
+    and V ([total_tokens, n_kv_heads, D] fp16, bf16 or fp32) is token starts[s]
+    + i of sequence s.  Rows outside the sequences are not written."""
+    _need_cuda(block_tables, starts, cu, k_out, v_out)
+    dev = cache.pool.device
+    _same_device(dev, block_tables, starts, cu, k_out, v_out, err)
+    B = int(starts.shape[0]) if starts.dim() == 1 else -1
+    shape = (int(total_tokens), cache.n_kv_heads, cache.head_dim)
+    with _On(dev, stream) as s:
+        given = [t for t in (k_out, v_out) if t is not None]
+        if given:
+            dtype = given[0].dtype
+        for t in given:
+            if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
+                raise ValueError(f"k_out / v_out must be contiguous {list(shape)} tensors of one type")
+        if dtype not in _DT:
+            raise ValueError("dtype must be fp16, bf16 or fp32")
+        if k_out is None:
+            k_out = torch.empty(shape, dtype=dtype, device=dev)
+        if v_out is None:
+            v_out = torch.empty(shape, dtype=dtype, device=dev)
+        L.check("tkv_int8_read", L.lib().tkv_int8_read(
+            C.byref(cache._c), k_out.data_ptr(), v_out.data_ptr(), _DT[dtype],
+            _index("block_tables", block_tables, B, None), block_tables.shape[1],
+            _index("starts", starts, B), _index("cu", cu, B + 1), B, shape[0],
+            shape[0] if max_tokens is None else int(max_tokens), _err_ptr(err), s))
+    return k_out, v_out
+
+
+def int8_workspace_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                         max_q_tokens: int, max_context_len: int) -> int:
+    return int(L.lib().tkv_int8_attend_workspace_bytes(num_seqs, num_q_heads, num_kv_heads,
+                                                       head_dim, max_q_tokens, max_context_len))
+
+
+def int8_workspace(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
+                   max_q_tokens: int, max_context_len: int, device="cuda") -> torch.Tensor:
+    """Zeroed workspace of int8_attend calls of up to these sizes (calls that
+    may overlap on the GPU need one each)."""
+    n = int8_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, max_q_tokens,
+                             max_context_len)
+    if n <= 0:
+        raise ValueError("sizes out of range")
+    return torch.zeros(n, dtype=torch.uint8, device=device)
+
+
+def int8_attend(cache: Int8PagedCache, q: torch.Tensor, cu_q: torch.Tensor,
+                block_tables: torch.Tensor, seq_lens: torch.Tensor,
+                max_q_tokens: Optional[int] = None, max_context_len: Optional[int] = None,
+                scale: Optional[float] = None, window: int = 0,
+                out: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None,
+                workspace: Optional[torch.Tensor] = None, err: Optional[torch.Tensor] = None,
+                stream=None) -> torch.Tensor:
+    """Attention of each sequence's last tokens over the int8 pages: rows
+    cu_q[s] .. cu_q[s+1] of q [T, Hq, D] (fp16 or bf16, any token and head
+    strides that are multiples of 8) are the last tokens of sequence s, already
+    appended; each attends to itself and the tokens before it, or to the last
+    `window` of them.  One row a sequence is a decode step.  Returns out [T, Hq,
+    D] (fp16 or bf16); its rows outside the sequences are not written."""
+    _need_cuda(q, cu_q, block_tables, seq_lens, out, workspace)
+    _no_grad_path("int8_attend", q)
+    dev = cache.pool.device
+    _same_device(dev, q, cu_q, block_tables, seq_lens, out, workspace, err)
+    B = int(seq_lens.shape[0]) if seq_lens.dim() == 1 else -1
+    with _On(dev, stream) as s:
+        x = _heads("q", q)
+        T, Hq, D = x.shape
+        if D != cache.head_dim:
+            raise ValueError(f"q has {D} channels, the cache {cache.head_dim}")
+        if Hq % cache.n_kv_heads:
+            raise ValueError(f"{Hq} q heads do not share {cache.n_kv_heads} kv heads evenly")
+        bt = _index("block_tables", block_tables, B, None)
+        mb = int(block_tables.shape[1])
+        mq = T if max_q_tokens is None else int(max_q_tokens)
+        ml = mb * L.TKV_PAGE_SIZE if max_context_len is None else int(max_context_len)
+        if out is None:
+            out = torch.empty((T, Hq, D), dtype=out_dtype or x.dtype, device=dev)
+        elif tuple(out.shape) != (T, Hq, D) or not out.is_contiguous():
+            raise ValueError(f"out must be a contiguous {[T, Hq, D]} tensor")
+        if out.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError("out must be fp16 or bf16")
+        if workspace is None:
+            workspace = int8_workspace(B, Hq, cache.n_kv_heads, D, mq, ml, dev)
+        elif not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        st = x.stride()
+        L.check("tkv_int8_attend", L.lib().tkv_int8_attend(
+            C.byref(cache._c), x.data_ptr(), _DT[x.dtype], (C.c_int64 * 2)(st[0], st[1]),
+            out.data_ptr(), _DT[out.dtype], _index("cu_q", cu_q, B + 1), bt, mb,
+            _index("seq_lens", seq_lens, B), B, Hq, T, mq, ml, int(window),
+            1.0 / math.sqrt(D) if scale is None else float(scale), workspace.data_ptr(),
+            workspace.numel() * workspace.element_size(), _err_ptr(err), s))
+    return out
