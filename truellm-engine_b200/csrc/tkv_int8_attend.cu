@@ -7,7 +7,9 @@
 // output.
 #include <limits.h>
 
-#include "tkv_int8.cuh"
+#include <algorithm>
+
+#include "tkv_int8_attend.cuh"
 
 namespace tkv {
 namespace {
@@ -26,12 +28,8 @@ __global__ void __launch_bounds__(32 * kWarps) int8_attend_kernel(Int8AttendArgs
   const int warp = threadIdx.x >> 5;
   const int s = blockIdx.y;
   const int len = __ldg(a.seq_lens + s), q0 = __ldg(a.cu_q + s), n = __ldg(a.cu_q + s + 1) - q0;
-  const bool ok = int8_seq_ok(0, len, 0, len, a.max_len, a.max_blocks) && n <= len &&
-                  int8_seq_ok(0, n, q0, a.total_q, a.max_q, INT_MAX / kPage);
-  if (!ok) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) set_err(a.err, TKV_ERR_BAD_LENGTH);
-    return;
-  }
+  if (!int8_attend_ok(a, len, q0, n)) return;  // flagged by the decode kernel
+  if (static_cast<long long>(n) * a.grp <= kInt8DecodeRows) return;  // the decode kernel's
   const long long r = static_cast<long long>(blockIdx.x) * kWarps + warp;
   if (r >= static_cast<long long>(n) * a.num_q_heads) return;
   const int i = static_cast<int>(r / a.num_q_heads), hq = static_cast<int>(r % a.num_q_heads);
@@ -108,9 +106,57 @@ __global__ void __launch_bounds__(32 * kWarps) int8_attend_kernel(Int8AttendArgs
 
 }  // namespace
 
-size_t int8_attend_workspace(int, int, int, int, int, int) { return 256; }
+namespace {
 
-int launch_int8_attend(const Int8AttendArgs& a, int head_dim, void*, size_t, cudaStream_t stream) {
+constexpr int kSlots = 148 * 3;  // resident CTAs of the decode kernel
+constexpr int kMinRun = 8;       // pages: one step of each of a CTA's warps
+constexpr int kMaxRun = 64;
+constexpr int kMaxRuns = 512;
+
+size_t round256(size_t x) { return (x + 255) / 256 * 256; }
+
+// How decode contexts of up to these sizes are cut: runs of equal length that
+// give every resident CTA one, but not shorter than a step of each warp nor
+// longer than kMaxRun pages.
+void decode_splits(Int8Splits& sp, int num_seqs, int num_kv_heads, int grp, int max_q, int max_len) {
+  const long long pages = (static_cast<long long>(max_len) + kPage - 1) / kPage;
+  const long long total = pages * num_seqs * num_kv_heads;
+  long long run = (total + kSlots - 1) / kSlots;
+  run = std::min<long long>(kMaxRun, std::max<long long>(kMinRun, (run + kMinRun - 1) / kMinRun * kMinRun));
+  run = std::max(run, (pages + kMaxRuns - 1) / kMaxRuns);
+  sp.pages = static_cast<int>(run);
+  sp.n = static_cast<int>(std::max<long long>(1, (pages + run - 1) / run));
+  sp.rows = static_cast<int>(std::min<long long>(kInt8DecodeRows, static_cast<long long>(max_q) * grp));
+}
+
+// bytes of the decode kernel's share of the workspace
+size_t decode_bytes(const Int8Splits& sp, int num_seqs, int num_kv_heads, int head_dim) {
+  const size_t pairs = static_cast<size_t>(num_seqs) * num_kv_heads;
+  const size_t rb = sp.rows <= 8 ? 8 : 16;
+  return round256(pairs * 4) + (sp.n > 1 ? round256(pairs * sp.n * rb * 8) + pairs * sp.n * rb * head_dim * 4 : 0);
+}
+
+}  // namespace
+
+size_t int8_attend_workspace(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
+                             int max_q, int max_len) {
+  Int8Splits sp;
+  decode_splits(sp, num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_q, max_len);
+  return 256 + decode_bytes(sp, num_seqs, num_kv_heads, head_dim);
+}
+
+int launch_int8_attend(const Int8AttendArgs& a, int head_dim, void* workspace, size_t,
+                       cudaStream_t stream) {
+  Int8Splits sp;
+  decode_splits(sp, a.num_seqs, a.n_kv_heads, a.grp, a.max_q, a.max_len);
+  const size_t pairs = static_cast<size_t>(a.num_seqs) * a.n_kv_heads;
+  uint8_t* ws = static_cast<uint8_t*>(workspace) + 256;
+  sp.count = reinterpret_cast<unsigned int*>(ws);
+  ws += round256(pairs * 4);
+  sp.part_ml = reinterpret_cast<float*>(ws);
+  sp.part_o = reinterpret_cast<float*>(ws + round256(pairs * sp.n * (sp.rows <= 8 ? 8 : 16) * 8));
+  const int st = launch_int8_decode(a, sp, head_dim, stream);
+  if (st != TKV_OK || static_cast<long long>(a.max_q) * a.grp <= kInt8DecodeRows) return st;
   const long long rows = static_cast<long long>(a.max_q) * a.num_q_heads;
   const dim3 grid(static_cast<unsigned int>((rows + kWarps - 1) / kWarps), a.num_seqs);
 #define TKV_RUN(D, Q, O) int8_attend_kernel<D, Q, O><<<grid, 32 * kWarps, 0, stream>>>(a)

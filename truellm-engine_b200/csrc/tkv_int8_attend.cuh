@@ -1,0 +1,62 @@
+// tkv_int8_attend.cuh -- what the decode and the chunk kernel of the int8 cache
+// share: checks, the ranges of the f16 operands, and how a context is split.
+#pragma once
+
+#include "tkv_int8.cuh"
+
+namespace tkv {
+
+constexpr float kInt8Lazy = 8.f;        // log2 units a score may exceed its row's reference by
+constexpr float kInt8ScaleTop = 4.f;    // largest value scale over 2^E
+constexpr float kInt8WeightUp = 32.f;   // f16 weights are held times this
+constexpr int kInt8DecodeRows = 16;     // most rows of the decode kernel
+
+// Runs of a context.  Decode: `n` runs at most per (sequence, kv head), each of
+// `pages` pages or less (ns = min(n, ceil(pages of the sequence / pages)) are
+// used); `rows` is the largest row count the launch may meet.
+struct Int8Splits {
+  int n, pages, rows;
+  unsigned int* count;  // [pairs], zero between launches
+  float* part_ml;       // [pair][run][row block][2]  (m in log2 units, l)
+  float* part_o;        // [pair][run][row block][D]  normalised
+};
+
+// the lengths of one sequence (see tkv_int8_attend)
+__device__ __forceinline__ bool int8_attend_ok(const Int8AttendArgs& a, int len, int q0, int n) {
+  return len >= 0 && len <= a.max_len &&
+         static_cast<long long>(len) <= static_cast<long long>(a.max_blocks) * kPage && n >= 0 &&
+         n <= len && n <= a.max_q && q0 >= 0 && q0 <= a.total_q - n;
+}
+
+// Powers of two that bring a row whose largest magnitude is m into fp16's
+// range: down = 2^-e, up = 2^e with m 2^-e in [1, 4); 1 for zeros, infinities.
+__device__ __forceinline__ void int8_row_power(float m, float& up, float& down) {
+  const uint32_t e = __float_as_uint(m) >> 23;
+  up = down = 1.f;
+  if (e > 0 && e < 255) {
+    const uint32_t ec = min(e, 253u);  // 2^-127 is no normal float
+    up = __uint_as_float(ec << 23);
+    down = __uint_as_float((254u - ec) << 23);
+  }
+}
+
+// 2^-E with s 2^-E in [1/2, 1), s > 0 a finite scale (at most 2^121)
+__device__ __forceinline__ float int8_scale_inverse(float s) {
+  const int e = static_cast<int>(__float_as_uint(s) >> 23);  // 2^(e - 127) <= s
+  return __uint_as_float(static_cast<uint32_t>(min(253, max(1, 253 - e))) << 23);
+}
+
+// four consecutive channels of an output row, rounded once
+__device__ __forceinline__ void int8_store4(const Int8AttendArgs& a, int64_t at, float4 v) {
+  uint2 w;
+  if (a.out_bf16)
+    w = make_uint2(pack2<true>(v.x, v.y), pack2<true>(v.z, v.w));
+  else
+    w = make_uint2(pack2<false>(v.x, v.y), pack2<false>(v.z, v.w));
+  *reinterpret_cast<uint2*>(a.out + at) = w;
+}
+
+int launch_int8_decode(const Int8AttendArgs& a, const Int8Splits& sp, int head_dim,
+                       cudaStream_t stream);
+
+}  // namespace tkv
