@@ -366,6 +366,19 @@ def test_rows_of_no_sequence_stay(ops, cuda):
     assert (out[23:] == 3).all()
 
 
+@pytest.mark.parametrize("new", [1, 3, 40])
+def test_pages_that_the_window_has_passed_may_be_gone(ops, cuda, new):
+    b = Batch(ops, cuda, [700, 333], [new, new], 1, 128, BF16, seed=14)
+    b.fill()
+    q = b.query(8)
+    want = b.attend(q, 50)
+    for s in (0, 1):
+        b.bt[s, :(b.old[s] - 50 + 1) // PAGE] = -1
+    b.bt_t = t32(b.bt, cuda)
+    err = err_word(cuda)
+    assert torch.equal(b.attend(q, 50, err), want) and err.item() == 0
+
+
 def test_strided_queries_and_output_types(ops, cuda):
     b = Batch(ops, cuda, [50, 3], [1, 30], 2, 128, BF16, seed=8)
     b.fill()

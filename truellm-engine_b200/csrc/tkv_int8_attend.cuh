@@ -21,6 +21,15 @@ struct Int8Splits {
   float* part_o;        // [pair][run][row block][D]  normalised
 };
 
+// Chunk kernel: 256-row tiles of a (sequence, kv head), each over n runs of
+// equal length of its context.
+constexpr int kInt8ChunkRows = 256;
+struct Int8ChunkSplits {
+  int n, row_tiles;
+  float* part_ml;  // [pair][row tile][run][256][2]
+  float* part_o;   // [pair][row tile][run][256][D]  normalised
+};
+
 // the lengths of one sequence (see tkv_int8_attend)
 __device__ __forceinline__ bool int8_attend_ok(const Int8AttendArgs& a, int len, int q0, int n) {
   return len >= 0 && len <= a.max_len &&
@@ -58,5 +67,8 @@ __device__ __forceinline__ void int8_store4(const Int8AttendArgs& a, int64_t at,
 
 int launch_int8_decode(const Int8AttendArgs& a, const Int8Splits& sp, int head_dim,
                        cudaStream_t stream);
+
+int launch_int8_chunk(const Int8AttendArgs& a, const Int8ChunkSplits& sp, int head_dim,
+                      cudaStream_t stream);
 
 }  // namespace tkv

@@ -1,0 +1,632 @@
+// tkv_int8_chunk.cu -- attention over the paged int8 cache for chunks of query
+// rows, on the 5th-generation tensor cores (tcgen05).
+//
+// A CTA takes 256 query rows (query token x q head of the kv head's group) of a
+// (sequence, kv head) and a run of 128-token tiles of its pages.  Roles:
+//   producers (4 warps)  tiles of codes, loaded one tile ahead into registers,
+//                        become exact f16 integers in the K-major operands K
+//                        [128 tokens][D] and V^T [D][128 tokens] (double
+//                        buffered); one of the warps also brings the scales
+//   MMA (1 warp, 1 lane) S = Q K^T per softmax warpgroup into tensor memory
+//                        (M = N = 128), O += P V with P read from tensor memory
+//   softmax (2 x 4 warps) one thread per query row: score x key scale, online
+//                        softmax, weight x value scale rounded once to f16 and
+//                        written to tensor memory over the scores (in two
+//                        halves of 64 tokens, so O += P V starts at the first)
+// The two warpgroups alternate: while one computes its weights the tensor cores
+// run the other's products.  Scales multiply finished 32-bit numbers only, so
+// the codes enter both products exactly; a masked token's weight is exactly 0.
+// References of the softmax and of the value scales as in tkv_int8_decode.cu.
+//
+// Tensor memory of warpgroup w (256 columns): S at 0 (its weights P, f16 pairs,
+// over columns 0 .. 63), O at 128.  Column 8 (4 u + j) + g of O is channel 32 u
+// + 4 g + j: the order in which a V unit's words are stored without conflicts.
+#include <limits.h>
+
+#include <algorithm>
+#include <atomic>
+
+#include "tkv_int8_attend.cuh"
+#include "tkv_umma.cuh"
+
+namespace tkv {
+namespace {
+
+constexpr int kRows = 128;       // rows of a softmax warpgroup (the MMA's M)
+constexpr int kTN = 128;         // tokens per tile
+constexpr int kTP = kTN / kPage; // pages per tile
+constexpr int kSoftmax = 256, kProducers = 128;
+constexpr int kCtaThreads = kSoftmax + kProducers + 32;
+
+// n 32-bit words to this thread's lane, n consecutive columns
+__device__ __forceinline__ void st16u(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16};\n" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+// n consecutive 32-bit columns of this thread's lane; load and wait are one
+// statement, so nothing can use a value before it has arrived
+__device__ __forceinline__ void ld64_wait(uint32_t taddr, float (&v)[64]) {
+  asm volatile(
+      "{\n\ttcgen05.ld.sync.aligned.32x32b.x64.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, "
+      "%34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, "
+      "%50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63 "
+      "}, [%64];\n\ttcgen05.wait::ld.sync.aligned;\n\t}\n"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+        "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
+        "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]),
+        "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]),
+        "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]),
+        "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]),
+        "=f"(v[38]), "=f"(v[39]), "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]),
+        "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]), "=f"(v[48]), "=f"(v[49]),
+        "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]),
+        "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]),
+        "=f"(v[62]), "=f"(v[63])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void ld32_wait(uint32_t taddr, float (&v)[32]) {
+  asm volatile(
+      "{\n\ttcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31 "
+      "}, [%32];\n\ttcgen05.wait::ld.sync.aligned;\n\t}\n"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+        "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
+        "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]),
+        "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]),
+        "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void ld16_wait(uint32_t taddr, float (&v)[16]) {
+  asm volatile(
+      "{\n\ttcgen05.ld.sync.aligned.32x32b.x16.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15 "
+      "}, [%16];\n\ttcgen05.wait::ld.sync.aligned;\n\t}\n"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+        "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
+        "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+__device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;\n"
+      : "=l"(d)
+      : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
+  return *reinterpret_cast<const float2*>(&d);
+}
+
+template <int D>
+struct Sm {
+  static constexpr int Q_BYTES = kRows * D * 2, K_BYTES = kTN * D * 2, V_BYTES = D * kTN * 2;
+  static constexpr int Q_OFF = 0;                      // one operand per warpgroup
+  static constexpr int K_OFF = Q_OFF + 2 * Q_BYTES;    // two buffers
+  static constexpr int V_OFF = K_OFF + 2 * K_BYTES;    // two buffers
+  static constexpr int KS_OFF = V_OFF + 2 * V_BYTES;   // [3][128] f32 key scales
+  static constexpr int VS_OFF = KS_OFF + 3 * kTN * 4;  // [3][128] value scales 2^-E 2^5
+  static constexpr int VI_OFF = VS_OFF + 3 * kTN * 4;  // [3] 2^-E of the tile
+  static constexpr int BAR_OFF = VI_OFF + 32;
+  static constexpr int BYTES = BAR_OFF + 256;
+  static_assert(BYTES <= 227 * 1024, "one CTA's shared memory");
+  static_assert(BYTES <= (1 << 18), "descriptor address fields never carry");
+  static constexpr uint32_t TWG = 256, TO = 128, TCOLS = 512;
+};
+
+template <int D>
+__global__ void __launch_bounds__(kCtaThreads, 1)
+    int8_chunk_kernel(const Int8AttendArgs a, const Int8ChunkSplits sp) {
+  using F = Int8Fmt<D>;
+  using SM = Sm<D>;
+  constexpr int UNITS = kPage * D / 16;           // 16-byte units of a page's K (or V) codes
+  constexpr int UPT = kTP * UNITS / kProducers;   // units per producer thread and tile
+  constexpr int PSTEP = kProducers / UNITS;       // pages covered by one unit of every thread
+  extern __shared__ __align__(1024) uint8_t smem[];
+  // Barriers (tile j counted from the CTA's first; b = j % 2):
+  //   kready[b], vready[b]  operands stored (128 producer arrivals)
+  //   kfree[b]              S of tile j done in every warpgroup (commit)
+  //   vfree[b]              O += P V of tile j done (a commit per warpgroup)
+  //   sready[j % 3]         scales stored (32 arrivals)
+  //   sdone[w]              S of tile j done (commit)
+  //   pready[w][h]          half h of P of tile j written (128 arrivals)
+  //   odone[w][h]           O += P V of that half done (commit)
+  uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + SM::BAR_OFF);
+  uint64_t* const kready = bars;
+  uint64_t* const vready = bars + 2;
+  uint64_t* const kfree = bars + 4;
+  uint64_t* const vfree = bars + 6;
+  uint64_t* const sready = bars + 8;
+  uint64_t* const sdone = bars + 11;
+  uint64_t* const pready = bars + 13;  // [2 w + h]
+  uint64_t* const odone = bars + 17;   // [2 w + h]
+  uint32_t* const tslot = reinterpret_cast<uint32_t*>(bars + 21);
+  float* const ks_s = reinterpret_cast<float*>(smem + SM::KS_OFF);
+  float* const vs_s = reinterpret_cast<float*>(smem + SM::VS_OFF);
+  float* const vi_s = reinterpret_cast<float*>(smem + SM::VI_OFF);
+
+  const int ctid = threadIdx.x, warp = ctid >> 5, lane = ctid & 31;
+  const int split = blockIdx.x % sp.n;
+  const int rest = blockIdx.x / sp.n;
+  const int rt = sp.row_tiles - 1 - rest % sp.row_tiles;  // longest contexts first
+  const int bh = rest / sp.row_tiles, s = bh / a.n_kv_heads, h = bh - s * a.n_kv_heads;
+  const int L = __ldg(a.seq_lens + s), q0 = __ldg(a.cu_q + s), n = __ldg(a.cu_q + s + 1) - q0;
+  if (!int8_attend_ok(a, L, q0, n)) return;  // flagged by the decode kernel
+  const long long rows_l = static_cast<long long>(n) * a.grp;
+  const long long r0 = static_cast<long long>(rt) * kSoftmax;
+  if (rows_l <= kInt8DecodeRows || r0 >= rows_l) return;
+  const int rows = static_cast<int>(min(rows_l - r0, static_cast<long long>(kSoftmax)));
+  const int wgs = rows > kRows ? 2 : 1;
+  // tiles that some row of this CTA sees, cut into sp.n runs
+  const int p_first = L - n + static_cast<int>(r0 / a.grp);
+  const int kv_end = L - n + static_cast<int>((r0 + rows - 1) / a.grp) + 1;
+  const int kv_lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
+  const int tile0 = kv_lo / kTN, tiles = (kv_end + kTN - 1) / kTN - tile0;
+  const int j_lo = tile0 + static_cast<int>(static_cast<long long>(tiles) * split / sp.n);
+  const int nj = tile0 + static_cast<int>(static_cast<long long>(tiles) * (split + 1) / sp.n) - j_lo;
+
+  if (warp == 0) umma::alloc(tslot, SM::TCOLS);
+  if (ctid == 0) {
+    for (int i = 0; i < 4; ++i) mbar_init(&bars[i], kProducers);      // kready, vready
+    for (int i = 4; i < 6; ++i) mbar_init(&bars[i], 1);               // kfree
+    for (int i = 6; i < 8; ++i) mbar_init(&bars[i], wgs);             // vfree
+    for (int i = 8; i < 11; ++i) mbar_init(&bars[i], 32);             // sready
+    for (int i = 11; i < 13; ++i) mbar_init(&bars[i], 1);             // sdone
+    for (int i = 13; i < 17; ++i) mbar_init(&bars[i], kRows);         // pready
+    for (int i = 17; i < 21; ++i) mbar_init(&bars[i], 1);             // odone
+    fence_mbar_init();
+  }
+
+  // ---- the Q operands: softmax thread ctid stages its row ----
+  const bool softmax = ctid < kSoftmax;
+  const int wg = ctid >> 7, wt = ctid & 127;
+  const bool valid = softmax && ctid < rows;
+  const int qi = valid ? static_cast<int>((r0 + ctid) / a.grp) : 0;
+  const int hq = h * a.grp + (valid ? static_cast<int>((r0 + ctid) % a.grp) : 0);
+  float ra = a.alpha;  // 2^e * scale * log2(e) of this row
+  if (softmax) {
+    const uint4* src = reinterpret_cast<const uint4*>(a.q + (q0 + qi) * a.q_t + hq * a.q_h);
+    float up = 1.f, down = 1.f;
+    if (a.q_bf16 && valid) {
+      float m = 0.f;
+#pragma unroll 4
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 x = __ldg(src + c);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack2<true>(w[e]);
+          m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      }
+      int8_row_power(m, up, down);
+    }
+    ra *= up;
+#pragma unroll 4
+    for (int c = 0; c < D / 8; ++c) {
+      uint4 x = valid ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
+      if (a.q_bf16) {
+        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = unpack2<true>(w[e]);
+          w[e] = pack_h2(f.x * down, f.y * down);
+        }
+        x = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+      *reinterpret_cast<uint4*>(smem + SM::Q_OFF + wg * SM::Q_BYTES + umma::umma_off(wt, 8 * c, D)) = x;
+    }
+    umma::fence_smem_to_async();
+  }
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  const uint32_t tmem = *tslot;
+  constexpr uint32_t idS = umma::idesc_f16(kRows, kTN, false);
+  constexpr uint32_t idO = umma::idesc_f16(kRows, D, false);
+
+  if (ctid >= kSoftmax && ctid < kSoftmax + kProducers) {
+    // ============================ producers ============================
+    const int tid = ctid - kSoftmax;
+    const bool scales = tid < 32;  // this warp brings the scales: lane l tokens 4 l ..
+    const int32_t* bt = a.block_tables + static_cast<int64_t>(s) * a.max_blocks;
+    const int n_pages = (kv_end + kPage - 1) / kPage;
+    const uint8_t* const pool_h = a.pool + static_cast<int64_t>(h) * F::BYTES;
+    const int64_t page_stride = static_cast<int64_t>(a.n_kv_heads) * F::BYTES;
+    const int first_page = kv_lo / kPage;  // the table may have dropped what the window passed
+    auto page_at = [&](int p) {  // page p of the sequence, checked; 0 outside the seen pages
+      int id = p >= first_page && p < n_pages ? __ldg(bt + p) : 0;
+      if (id < 0 || id >= a.num_pages) {
+        set_err(a.err, TKV_ERR_BAD_PAGE);
+        id = 0;  // read in bounds; the sequence's output is not meaningful
+      }
+      return id;
+    };
+    // K unit of this thread in page PSTEP i + tid / UNITS: slot x % 16 of chunk
+    // x / 16 (x = tid % UNITS): 8 lanes read 128 bytes and fill one core matrix.
+    const int x = tid % UNITS, pg0 = tid / UNITS;
+    const int kc = x >> 4, ktok = (x & 15) ^ (2 * (kc & 3));
+    const uint32_t k_dst = umma::umma_off(ktok, 16 * kc, D);
+    // V unit: of its unit u the lane takes (g, t) so that 16 lanes' 8-byte stores
+    // fill 128 bytes
+    const int vu = x >> 5, vg = (lane >> 1) & 7, vt = (lane & 1) + 2 * (lane >> 4);
+    const uint32_t v_src = F::V_OFF + int8_v_unit(vu, vg, vt);
+    const uint32_t v_dst = 4 * vu * (16 * kTN) + (vt >> 1) * 128 + vg * 16 + (vt & 1) * 8;
+    int pid[UPT], spid = 0;
+    uint4 kr[UPT], vr[UPT], sr0 = make_uint4(0, 0, 0, 0), sr1 = sr0;
+    auto fetch_ids = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) pid[i] = page_at(j * kTP + PSTEP * i + pg0);
+      if (scales) spid = page_at(j * kTP + (lane >> 2));
+    };
+    auto load_k = [&]() {
+#pragma unroll
+      for (int i = 0; i < UPT; ++i)
+        kr[i] = __ldg(reinterpret_cast<const uint4*>(pool_h + pid[i] * page_stride) + x);
+      if (scales) {
+        const uint4* p = reinterpret_cast<const uint4*>(pool_h + spid * page_stride + F::SCALE_OFF) +
+                         2 * (lane & 3);
+        sr0 = __ldg(p);
+        sr1 = __ldg(p + 1);
+      }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+      for (int i = 0; i < UPT; ++i)
+        vr[i] = __ldg(reinterpret_cast<const uint4*>(pool_h + pid[i] * page_stride + v_src));
+    };
+    float vinv = 0x1p126f;  // 2^-E
+    if (nj > 0) {
+      fetch_ids(j_lo);
+      load_k();
+      load_v();
+    }
+    for (int j = 0; j < nj; ++j) {
+      const int b = j & 1, ph = (j >> 1) & 1;
+      const bool more = j + 1 < nj;
+      if (more) fetch_ids(j_lo + j + 1);
+      if (j >= 2 && !mbar_wait_fast(&kfree[b], ph ^ 1, a.err)) break;
+      if (scales) {
+        const float kv[8] = {__uint_as_float(sr0.x), __uint_as_float(sr0.y), __uint_as_float(sr0.z),
+                             __uint_as_float(sr0.w), __uint_as_float(sr1.x), __uint_as_float(sr1.y),
+                             __uint_as_float(sr1.z), __uint_as_float(sr1.w)};
+        const int t0 = (j_lo + j) * kTN + 4 * lane;
+        float v[4], top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // tokens that no row of the CTA sees count for nothing
+          v[e] = t0 + e < kv_end && t0 + e >= kv_lo ? kv[2 * e + 1] : 0.f;
+          top = fmaxf(top, v[e]);
+        }
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        if (top * vinv > kInt8ScaleTop) vinv = int8_scale_inverse(top);
+        const int buf = j % 3;
+        *reinterpret_cast<float4*>(ks_s + buf * kTN + 4 * lane) = make_float4(kv[0], kv[2], kv[4], kv[6]);
+        *reinterpret_cast<float4*>(vs_s + buf * kTN + 4 * lane) =
+            make_float4(v[0] * vinv * kInt8WeightUp, v[1] * vinv * kInt8WeightUp,
+                        v[2] * vinv * kInt8WeightUp, v[3] * vinv * kInt8WeightUp);
+        if (lane == 0) vi_s[buf] = vinv;
+        mbar_arrive(&sready[buf]);
+      }
+      uint8_t* const kd = smem + SM::K_OFF + b * SM::K_BYTES + k_dst;
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        const uint32_t w[4] = {kr[i].x, kr[i].y, kr[i].z, kr[i].w};
+        uint32_t hv[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) int8_to_h2(w[e], hv[2 * e], hv[2 * e + 1]);
+        uint8_t* d = kd + (PSTEP * i + pg0) * (32 * D);
+        *reinterpret_cast<uint4*>(d) = make_uint4(hv[0], hv[1], hv[2], hv[3]);
+        *reinterpret_cast<uint4*>(d + 128) = make_uint4(hv[4], hv[5], hv[6], hv[7]);
+      }
+      umma::fence_smem_to_async();
+      mbar_arrive(&kready[b]);
+      if (more) load_k();
+      if (j >= 2 && !mbar_wait_fast(&vfree[b], ph ^ 1, a.err)) break;
+      uint8_t* const vd = smem + SM::V_OFF + b * SM::V_BYTES + v_dst;
+#pragma unroll
+      for (int i = 0; i < UPT; ++i) {
+        const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t lo, hi;
+          int8_to_h2(w[e], lo, hi);
+          *reinterpret_cast<uint2*>(vd + e * (16 * kTN) + (PSTEP * i + pg0) * 256) = make_uint2(lo, hi);
+        }
+      }
+      umma::fence_smem_to_async();
+      mbar_arrive(&vready[b]);
+      if (more) load_v();
+    }
+  } else if (ctid >= kSoftmax + kProducers) {
+    // ============================ the MMA warp ============================
+    if (lane == 0 && nj > 0) {
+      bool ok = true;
+      int last_s[2] = {-1, -1}, last_h[2][2] = {{-1, -1}, {-1, -1}};
+      const uint64_t dq = umma::smem_desc(smem_u32(smem + SM::Q_OFF), 128, 16 * D);
+      const uint64_t dk = umma::smem_desc(smem_u32(smem + SM::K_OFF), 128, 16 * D);
+      const uint64_t dv = umma::smem_desc(smem_u32(smem + SM::V_OFF), 128, 16 * kTN);
+      auto issue_s = [&](int w, int j) {
+        umma::fence_after_sync();
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          umma::mma_f16(tmem + w * SM::TWG, dq + w * (SM::Q_BYTES >> 4) + 16 * kk,
+                        dk + (j & 1) * (SM::K_BYTES >> 4) + 16 * kk, idS, kk > 0);
+        umma::commit(&sdone[w]);
+        if (w == wgs - 1) umma::commit(&kfree[j & 1]);
+        last_s[w] = j;
+      };
+      ok = mbar_wait(&kready[0], 0, a.err);
+      for (int w = 0; ok && w < wgs; ++w) issue_s(w, 0);
+      for (int j = 0; ok && j < nj; ++j) {
+        ok = mbar_wait(&vready[j & 1], (j >> 1) & 1, a.err);
+        for (int w = 0; ok && w < wgs; ++w) {
+          for (int hf = 0; ok && hf < 2; ++hf) {
+            ok = mbar_wait(&pready[2 * w + hf], j & 1, a.err);
+            if (!ok) break;
+            umma::fence_after_sync();
+#pragma unroll
+            for (int kk = 0; kk < kTN / 32; ++kk) {
+              const int k = hf * (kTN / 32) + kk;
+              umma::mma_f16_ta(tmem + w * SM::TWG + SM::TO, tmem + w * SM::TWG + 8 * k,
+                               dv + (j & 1) * (SM::V_BYTES >> 4) + 16 * k, idO, j > 0 || k > 0);
+            }
+            umma::commit(&odone[2 * w + hf]);
+            last_h[w][hf] = j;
+          }
+          if (!ok) break;
+          umma::commit(&vfree[j & 1]);
+          if (j + 1 < nj) {
+            // S of the next tile overwrites the scores and weights of this one
+            ok = mbar_wait(&kready[(j + 1) & 1], ((j + 1) >> 1) & 1, a.err) &&
+                 mbar_wait(&odone[2 * w + 1], j & 1, a.err);
+            if (ok) issue_s(w, j + 1);
+          }
+        }
+      }
+      // no MMA may still run when tensor memory is released
+      for (int w = 0; w < 2; ++w) {
+        if (last_s[w] >= 0) mbar_wait(&sdone[w], last_s[w] & 1, nullptr);
+        for (int hf = 0; hf < 2; ++hf)
+          if (last_h[w][hf] >= 0) mbar_wait(&odone[2 * w + hf], last_h[w][hf] & 1, nullptr);
+      }
+    }
+  } else if (wg < wgs) {
+    // ============================ softmax ============================
+    const uint32_t lane_base = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+    const uint32_t tS = tmem + wg * SM::TWG + lane_base, tO = tS + SM::TO;
+    const int plim = valid ? L - n + qi : -1;  // last position that the row sees
+    const int pmin = a.window > 0 ? max(0, plim - a.window + 1) : 0;
+    float m = -INFINITY, l = 0.f, vinv = 0x1p126f;
+    bool ok = true;
+    for (int j = 0; j < nj; ++j) {
+      const int buf = j % 3, t0 = (j_lo + j) * kTN;
+      ok = mbar_wait_fast(&sready[buf], (j / 3) & 1, a.err) &&
+           mbar_wait_fast(&sdone[wg], j & 1, a.err);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      umma::fence_after_sync();
+      const bool masked = t0 + kTN - 1 > plim || t0 < pmin;
+      const float vnew = vi_s[buf];
+      float fv = 1.f;
+      if (vnew != vinv) {
+        fv = vnew / vinv;
+        vinv = vnew;
+      }
+#pragma unroll 1
+      for (int hf = 0; hf < 2; ++hf) {
+        float x[64];
+        ld64_wait(tS + 64 * hf, x);
+        const float4* ks4 = reinterpret_cast<const float4*>(ks_s + buf * kTN + 64 * hf);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 64; c += 4) {
+          const float4 k4 = ks4[c / 4];
+          const float2 p0 = fmul2(make_float2(x[c], x[c + 1]), make_float2(k4.x, k4.y));
+          const float2 p1 = fmul2(make_float2(x[c + 2], x[c + 3]), make_float2(k4.z, k4.w));
+          x[c] = p0.x, x[c + 1] = p0.y, x[c + 2] = p1.x, x[c + 3] = p1.y;
+        }
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c) {
+            const int t = t0 + 64 * hf + c;
+            x[c] = t <= plim && t >= pmin ? x[c] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) mx = fmaxf(mx, fmaxf(x[c], x[c + 1]));
+        mx *= ra;  // ra > 0 keeps the order
+        const bool need = mx > m + kInt8Lazy;
+        if (__any_sync(0xffffffffu, need || fv != 1.f)) {
+          float f = need ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
+          m = need ? mx : m;
+          l *= f;
+          f *= fv;
+          fv = 1.f;
+          if (j > 0 || hf > 0) {
+            // O holds the tiles before (done: S of this tile was issued after
+            // them) and, in the second half, the first one's products
+            if (hf > 0) {
+              ok = __all_sync(0xffffffffu, mbar_wait_fast(&odone[2 * wg], j & 1, a.err));
+              if (!ok) break;
+              umma::fence_after_sync();
+            }
+#pragma unroll
+            for (int c0 = 0; c0 < D; c0 += 16) {
+              float o[16];
+              ld16_wait(tO + c0, o);
+#pragma unroll
+              for (int c = 0; c < 16; ++c) o[c] *= f;
+              umma::st16(tO + c0, o);
+            }
+            umma::wait_st();
+          }
+        }
+        const float nm = m == -INFINITY ? 0.f : -m;
+        const float2 ra2 = make_float2(ra, ra), nm2 = make_float2(nm, nm);
+        float2 sum = make_float2(0.f, 0.f);
+        const float4* vs4 = reinterpret_cast<const float4*>(vs_s + buf * kTN + 64 * hf);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t pw[16];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int c = 32 * q + 4 * e;
+            const float4 v4 = vs4[c / 4];
+            const float2 y0 = ffma2(make_float2(x[c], x[c + 1]), ra2, nm2);
+            const float2 y1 = ffma2(make_float2(x[c + 2], x[c + 3]), ra2, nm2);
+            const float2 p0 = make_float2(fast_exp2(y0.x), fast_exp2(y0.y));
+            const float2 p1 = make_float2(fast_exp2(y1.x), fast_exp2(y1.y));
+            sum = fadd2(sum, fadd2(p0, p1));
+            float2 w0 = fmul2(p0, make_float2(v4.x, v4.y)), w1 = fmul2(p1, make_float2(v4.z, v4.w));
+            if (masked) {  // whatever the scale holds
+              w0.x = x[c] == -INFINITY ? 0.f : w0.x;
+              w0.y = x[c + 1] == -INFINITY ? 0.f : w0.y;
+              w1.x = x[c + 2] == -INFINITY ? 0.f : w1.x;
+              w1.y = x[c + 3] == -INFINITY ? 0.f : w1.y;
+            }
+            pw[2 * e] = pack_h2(w0.x, w0.y);
+            pw[2 * e + 1] = pack_h2(w1.x, w1.y);
+          }
+          st16u(tS + 32 * hf + 16 * q, pw);
+        }
+        l += sum.x + sum.y;
+        umma::wait_st();
+        umma::fence_before_sync();
+        mbar_arrive(&pready[2 * wg + hf]);
+      }
+      if (!ok) break;
+    }
+    if (ok && nj > 0)
+      ok = mbar_wait(&odone[2 * wg], (nj - 1) & 1, a.err) && mbar_wait(&odone[2 * wg + 1], (nj - 1) & 1, a.err);
+    ok = __all_sync(0xffffffffu, ok);
+    umma::fence_after_sync();
+    // ---- normalise and write the row (a run's partial when the context is split) ----
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float vs = (1.f / vinv) / kInt8WeightUp;
+    const int64_t row = static_cast<int64_t>(q0 + qi) * a.num_q_heads + hq;
+    const int64_t slot = static_cast<int64_t>(blockIdx.x) * kSoftmax + ctid;
+    if (ok) {
+#pragma unroll 1
+      for (int u = 0; u < D / 32; ++u) {
+        float o[32];
+        __syncwarp();
+        if (nj > 0) {
+          ld32_wait(tO + 32 * u, o);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) o[c] = 0.f;
+        }
+        if (valid) {
+#pragma unroll
+          for (int g = 0; g < 8; g += 2) {  // channels 32 u + 4 g .. + 7
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = o[8 * (e & 3) + g + (e >> 2)] * inv * vs;
+            const int c = 32 * u + 4 * g;
+            if (sp.n > 1) {
+              float4* dst = reinterpret_cast<float4*>(sp.part_o + slot * D + c);
+              dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+              dst[1] = make_float4(v[4], v[5], v[6], v[7]);
+            } else {
+              uint4 w;
+              if (a.out_bf16)
+                w = make_uint4(pack2<true>(v[0], v[1]), pack2<true>(v[2], v[3]),
+                               pack2<true>(v[4], v[5]), pack2<true>(v[6], v[7]));
+              else
+                w = make_uint4(pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3]),
+                               pack2<false>(v[4], v[5]), pack2<false>(v[6], v[7]));
+              *reinterpret_cast<uint4*>(a.out + row * D + c) = w;
+            }
+          }
+        }
+      }
+      if (sp.n > 1 && valid) *reinterpret_cast<float2*>(sp.part_ml + slot * 2) = make_float2(m, l);
+    }
+  }
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  if (warp == 0) umma::dealloc(tmem, SM::TCOLS);
+}
+
+// Joins the runs of split contexts: a warp per row, the runs in order.
+template <int D>
+__global__ void __launch_bounds__(256) int8_chunk_join_kernel(const Int8AttendArgs a,
+                                                              const Int8ChunkSplits sp) {
+  const int lane = threadIdx.x & 31;
+  const long long wid = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const long long cta = wid / kSoftmax;  // (pair, row tile)
+  const int r = static_cast<int>(wid % kSoftmax);
+  const int rt = sp.row_tiles - 1 - static_cast<int>(cta % sp.row_tiles);
+  const int bh = static_cast<int>(cta / sp.row_tiles), s = bh / a.n_kv_heads, h = bh - s * a.n_kv_heads;
+  if (s >= a.num_seqs) return;
+  const int L = __ldg(a.seq_lens + s), q0 = __ldg(a.cu_q + s), n = __ldg(a.cu_q + s + 1) - q0;
+  if (!int8_attend_ok(a, L, q0, n)) return;
+  const long long rows = static_cast<long long>(n) * a.grp;
+  const long long rho = static_cast<long long>(rt) * kSoftmax + r;
+  if (rows <= kInt8DecodeRows || rho >= rows) return;
+  const long long slot0 = cta * sp.n * kSoftmax + r;
+  float M = -INFINITY;
+  for (int i = 0; i < sp.n; ++i) M = fmaxf(M, __ldcg(sp.part_ml + (slot0 + static_cast<long long>(i) * kSoftmax) * 2));
+  const float ref = M == -INFINITY ? 0.f : M;
+  float W = 0.f, acc[D / 32] = {};
+  for (int i = 0; i < sp.n; ++i) {
+    const long long slot = slot0 + static_cast<long long>(i) * kSoftmax;
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(sp.part_ml + slot * 2));
+    const float w = ml.y * fast_exp2(ml.x - ref);
+    W += w;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+      acc[c] = fmaf(w, __ldcg(sp.part_o + slot * D + (D / 32) * lane + c), acc[c]);
+  }
+  const float inv = W == 0.f ? 0.f : 1.f / W;
+  const int64_t at = (static_cast<int64_t>(q0 + rho / a.grp) * a.num_q_heads + h * a.grp + rho % a.grp) * D +
+                     (D / 32) * lane;
+#pragma unroll
+  for (int c = 0; c < D / 32; c += 2) {
+    const uint32_t w = a.out_bf16 ? pack2<true>(acc[c] * inv, acc[c + 1] * inv)
+                                  : pack2<false>(acc[c] * inv, acc[c + 1] * inv);
+    *reinterpret_cast<uint32_t*>(a.out + at + c) = w;
+  }
+}
+
+template <int D>
+int launch_t(const Int8AttendArgs& a, const Int8ChunkSplits& sp, cudaStream_t stream) {
+  static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit is raised
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return TKV_BACKEND_ERROR;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(int8_chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Sm<D>::BYTES) != cudaSuccess)
+      return TKV_BACKEND_ERROR;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  const long long ctas = static_cast<long long>(a.num_seqs) * a.n_kv_heads * sp.row_tiles;
+  if (ctas * std::max(sp.n, kSoftmax / 8) > INT_MAX) return TKV_INVALID_ARGUMENT;
+  int8_chunk_kernel<D><<<static_cast<unsigned int>(ctas * sp.n), kCtaThreads, Sm<D>::BYTES, stream>>>(a, sp);
+  if (cudaGetLastError() != cudaSuccess) return TKV_BACKEND_ERROR;
+  if (sp.n > 1) {
+    int8_chunk_join_kernel<D><<<static_cast<unsigned int>(ctas * (kSoftmax / 8)), 256, 0, stream>>>(a, sp);
+    if (cudaGetLastError() != cudaSuccess) return TKV_BACKEND_ERROR;
+  }
+  return TKV_OK;
+}
+
+}  // namespace
+
+int launch_int8_chunk(const Int8AttendArgs& a, const Int8ChunkSplits& sp, int head_dim,
+                      cudaStream_t stream) {
+  return head_dim == 128 ? launch_t<128>(a, sp, stream) : launch_t<64>(a, sp, stream);
+}
+
+}  // namespace tkv

@@ -492,67 +492,104 @@ def swap_ring_rows(cache: KiviPagedCache, images: torch.Tensor, mapping: torch.T
 # rotary positions with several axes, and the paged int8 cache
 # ---------------------------------------------------------------------------
 class _On:
-    """Makes a tensor's device and the call's stream current, so that what a
-    call allocates or copies belongs to the stream its kernel runs on."""
+    """Makes a device and the call's stream current, so that what a call
+    allocates or copies belongs to the stream its kernel runs on."""
 
-    def __init__(self, device: torch.device, stream):
+    def __init__(self, index: int, stream):
+        device = torch.device("cuda", index)
         if stream is not None and not isinstance(stream, torch.cuda.Stream):
             stream = torch.cuda.ExternalStream(int(stream), device=device)
         if stream is not None and stream.device != device:
             raise ValueError(f"stream is on {stream.device}, the tensors on {device}")
-        self._ctx = []
-        if torch.cuda.current_device() != device.index:
-            self._ctx.append(torch.cuda.device(device))
+        self._ctx = [torch.cuda.device(device)]
         if stream is not None:
             self._ctx.append(torch.cuda.stream(stream))
-        self._device = device
+        self._index = index
 
     def __enter__(self) -> int:
         for c in self._ctx:
             c.__enter__()
-        return torch.cuda.current_stream(self._device).cuda_stream
+        return torch.cuda.current_stream(self._index).cuda_stream
 
     def __exit__(self, *exc):
         for c in reversed(self._ctx):
             c.__exit__(*exc)
 
 
-def _same_device(device: torch.device, *ts) -> None:
+class _Here:
+    """_On's short form for the current device and its current stream: a call on
+    one token costs as much on the host as on the GPU."""
+
+    def __init__(self, stream: int):
+        self._stream = stream
+
+    def __enter__(self) -> int:
+        return self._stream
+
+    def __exit__(self, *exc):
+        pass
+
+
+def _on(index: int, stream):
+    if stream is None and torch.cuda.current_device() == index:
+        return _Here(torch._C._cuda_getCurrentRawStream(index))
+    return _On(index, stream)
+
+
+def _one_device(index: int, *ts) -> None:
     for t in ts:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensors are on {t.device} and {device}: one CUDA device is needed")
+        if t is not None and t.get_device() != index:
+            if not t.is_cuda:
+                raise ValueError("the kernels take CUDA tensors")
+            raise ValueError(f"tensors are on devices {t.get_device()} and {index}: one is needed")
 
 
-def _index(name: str, t: torch.Tensor, *shape) -> int:
-    """Address of a contiguous int32 tensor of this shape (None: any size)."""
-    if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != len(shape) or any(
-            n is not None and n != m for n, m in zip(shape, t.shape)):
-        want = ", ".join("*" if n is None else str(n) for n in shape)
-        raise ValueError(f"{name} must be a contiguous int32 [{want}] tensor")
+def _index(name: str, t: torch.Tensor, shape: tuple) -> int:
+    """Address of a contiguous int32 tensor of this shape."""
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 {list(shape)} tensor")
     return t.data_ptr()
+
+
+def _table(t: torch.Tensor, num_seqs: int) -> tuple:
+    """Address and width of a block table."""
+    if t.dim() != 2:
+        raise ValueError("block_tables must be an int32 [sequences, blocks] tensor")
+    n = t.shape[1]
+    return _index("block_tables", t, (num_seqs, n)), n
+
+
+def _count(t: torch.Tensor) -> int:
+    return t.shape[0] if t.dim() == 1 else -1
 
 
 def _err_ptr(err: Optional[torch.Tensor]):
     if err is None:
         return None
-    if err.dtype != torch.int32 or err.numel() < 1:
+    if err.dtype is not torch.int32 or err.numel() < 1:
         raise ValueError("err must be an int32 tensor of one word")
     return err.data_ptr()
+
+
+_HALF = (torch.float16, torch.bfloat16)
 
 
 def _heads(name: str, t: torch.Tensor) -> torch.Tensor:
     """[T, H, D] fp16/bf16 whose 16-byte vectors the kernels can address: any
     token and head strides that are multiples of 8 elements, else a copy."""
-    if t.dim() != 3 or t.dtype not in (torch.float16, torch.bfloat16):
+    if t.dim() != 3 or t.dtype not in _HALF:
         raise ValueError(f"{name} must be an fp16 or bf16 [tokens, heads, channels] tensor")
     st, sh, sd = t.stride()
-    if sd != 1 or st % 8 or sh % 8 or t.data_ptr() % 16:
+    if sd != 1 or (st | sh) & 7 or t.data_ptr() & 15:
         return t.contiguous()
     return t
 
 
+_I64x2, _I64x4, _I64x8 = C.c_int64 * 2, C.c_int64 * 4, C.c_int64 * 8
+
+
 def _no_grad_path(name: str, *ts) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+    if torch.is_grad_enabled() and any([t.requires_grad for t in ts]):
         raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
 
 
@@ -587,48 +624,45 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
     rotary_dim / 2), "adjacent" (2 i, 2 i + 1).  inverse turns back (and is the
     gradient; calls on tensors that require one are differentiable).  q_out /
     k_out may be q / k (in place).  Returns (q_out, k_out)."""
-    ts = (q,) if k is None else (q, k)
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         if q_out is not None or k_out is not None:
             raise ValueError("q_out / k_out cannot be given where a gradient is needed")
         got = _RopeAxes.apply(q, k, positions, tuple(sections), theta, order, pairing,
                               inverse, stream)
         return got if k is not None else (got[0], None)
-    _need_cuda(q, k, positions)
-    _same_device(q.device, k, positions, q_out, k_out)
-    sections = tuple(int(n) for n in sections)
-    rotary = 2 * sum(sections)
-    plan = _rope_plan(rotary, sections, float(theta), order, pairing)
-    with _On(q.device, stream) as s:
+    dev = q.get_device()
+    _one_device(max(dev, 0), q, k, positions, q_out, k_out)
+    sections = tuple(sections)
+    plan = _rope_plan(2 * sum(sections), sections, theta, order, pairing)
+    with _on(dev, stream) as s:
         qx = _heads("q", q)
         T, Hq, D = qx.shape
         kx = None if k is None else _heads("k", k)
         if kx is not None and (kx.shape[0] != T or kx.shape[2] != D or kx.dtype != qx.dtype):
             raise ValueError("k must have q's tokens, channels and type")
-        if (positions.dtype != torch.int32 or positions.dim() != 2 or
-                tuple(positions.shape) != (len(sections), T) or
+        if (positions.dtype is not torch.int32 or positions.shape != (len(sections), T) or
                 (T > 1 and positions.stride(1) != 1)):
             raise ValueError(f"positions must be an int32 [{len(sections)}, {T}] tensor")
         if q_out is None:
             q_out = torch.empty((T, Hq, D), dtype=qx.dtype, device=qx.device)
         if kx is not None and k_out is None:
-            k_out = torch.empty_like(kx, memory_format=torch.contiguous_format)
-        for name, o, x in (("q_out", q_out, qx), ("k_out", k_out, kx)):
-            if o is None or x is None:
-                if o is not None:
-                    raise ValueError("k_out without k")
-                continue
-            if o.shape != x.shape or o.dtype != x.dtype or _heads(name, o) is not o:
-                raise ValueError(f"{name} must have its input's shape and type, contiguous "
+            k_out = torch.empty(kx.shape, dtype=kx.dtype, device=kx.device)
+        if kx is None and k_out is not None:
+            raise ValueError("k_out without k")
+        for o, x in ((q_out, qx), (k_out, kx)):
+            if x is not None and (o.shape != x.shape or o.dtype is not x.dtype or
+                                  _heads("output", o) is not o):
+                raise ValueError("an output must have its input's shape and type, contiguous "
                                  "channels and strides that are multiples of 8")
-        Hk = 0 if kx is None else kx.shape[1]
-        kst, kos = ((0, 0), (0, 0)) if kx is None else (kx.stride(), k_out.stride())
         qst, qos = qx.stride(), q_out.stride()
-        strides = (C.c_int64 * 8)(qst[0], qst[1], kst[0], kst[1], qos[0], qos[1], kos[0], kos[1])
+        Hk, kst, kos = 0, (0, 0), (0, 0)
+        if kx is not None:
+            Hk, kst, kos = kx.shape[1], kx.stride(), k_out.stride()
+        strides = _I64x8(qst[0], qst[1], kst[0], kst[1], qos[0], qos[1], kos[0], kos[1])
         L.check("tkv_rope_axes", L.lib().tkv_rope_axes(
             C.byref(plan), qx.data_ptr(), None if kx is None else kx.data_ptr(),
             q_out.data_ptr(), None if kx is None else k_out.data_ptr(), _DT[qx.dtype], Hq, Hk, D,
-            T, strides, positions.data_ptr(), positions.stride(0), int(bool(inverse)), s))
+            T, strides, positions.data_ptr(), positions.stride(0), 1 if inverse else 0, s))
     return q_out, k_out
 
 
@@ -676,6 +710,8 @@ class Int8PagedCache:
         self.pool = pool
         self.num_pages = int(pool.shape[0])
         self._c = L.TkvInt8Cache(pool.data_ptr(), self.num_pages, self.n_kv_heads, self.head_dim, 0)
+        self._ref = C.byref(self._c)
+        self._device = pool.get_device()
 
     def c_struct(self) -> L.TkvInt8Cache:
         return self._c
@@ -691,25 +727,24 @@ def int8_append(cache: Int8PagedCache, k_new: torch.Tensor, v_new: torch.Tensor,
     strides that are multiples of 8 (slices of a fused projection are read where
     they lie); cu_new [B+1], seq_lens_old [B], block_tables [B, max_blocks]
     int32; max_new_tokens bounds a sequence's new tokens (default T)."""
-    _need_cuda(k_new, v_new, cu_new, seq_lens_old, block_tables)
     _no_grad_path("int8_append", k_new, v_new)
-    dev = cache.pool.device
-    _same_device(dev, k_new, v_new, cu_new, seq_lens_old, block_tables, err)
-    B = int(seq_lens_old.shape[0]) if seq_lens_old.dim() == 1 else -1
-    with _On(dev, stream) as s:
+    dev = cache._device
+    _one_device(max(dev, 0), cache.pool, k_new, v_new, cu_new, seq_lens_old, block_tables, err)
+    B = _count(seq_lens_old)
+    with _on(dev, stream) as s:
         k, v = _heads("k_new", k_new), _heads("v_new", v_new)
         if k.shape != v.shape or k.dtype != v.dtype or k.shape[1:] != (cache.n_kv_heads,
                                                                       cache.head_dim):
             raise ValueError(f"k_new and v_new must both be [tokens, {cache.n_kv_heads}, "
                              f"{cache.head_dim}] of one type")
-        T = int(k.shape[0])
+        T = k.shape[0]
         ks, vs = k.stride(), v.stride()
+        bt, mb = _table(block_tables, B)
         L.check("tkv_int8_append", L.lib().tkv_int8_append(
-            C.byref(cache._c), k.data_ptr(), v.data_ptr(), _DT[k.dtype],
-            (C.c_int64 * 4)(ks[0], ks[1], vs[0], vs[1]), _index("cu_new", cu_new, B + 1),
-            _index("seq_lens_old", seq_lens_old, B), _index("block_tables", block_tables, B, None),
-            block_tables.shape[1], B, T, T if max_new_tokens is None else int(max_new_tokens),
-            _err_ptr(err), s))
+            cache._ref, k.data_ptr(), v.data_ptr(), _DT[k.dtype],
+            _I64x4(ks[0], ks[1], vs[0], vs[1]), _index("cu_new", cu_new, (B + 1,)),
+            _index("seq_lens_old", seq_lens_old, (B,)), bt, mb, B, T,
+            T if max_new_tokens is None else int(max_new_tokens), _err_ptr(err), s))
 
 
 def int8_read(cache: Int8PagedCache, block_tables: torch.Tensor, starts: torch.Tensor,
@@ -720,28 +755,28 @@ def int8_read(cache: Int8PagedCache, block_tables: torch.Tensor, starts: torch.T
     """Reads tokens back from the int8 pages: row cu[s] + i of the returned K
     and V ([total_tokens, n_kv_heads, D] fp16, bf16 or fp32) is token starts[s]
     + i of sequence s.  Rows outside the sequences are not written."""
-    _need_cuda(block_tables, starts, cu, k_out, v_out)
-    dev = cache.pool.device
-    _same_device(dev, block_tables, starts, cu, k_out, v_out, err)
-    B = int(starts.shape[0]) if starts.dim() == 1 else -1
+    dev = cache._device
+    _one_device(max(dev, 0), cache.pool, block_tables, starts, cu, k_out, v_out, err)
+    B = _count(starts)
     shape = (int(total_tokens), cache.n_kv_heads, cache.head_dim)
-    with _On(dev, stream) as s:
-        given = [t for t in (k_out, v_out) if t is not None]
-        if given:
-            dtype = given[0].dtype
-        for t in given:
-            if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
-                raise ValueError(f"k_out / v_out must be contiguous {list(shape)} tensors of one type")
+    with _on(dev, stream) as s:
+        if k_out is not None or v_out is not None:
+            dtype = (v_out if k_out is None else k_out).dtype
+            for t in (k_out, v_out):
+                if t is not None and (t.shape != shape or t.dtype is not dtype or
+                                      not t.is_contiguous()):
+                    raise ValueError(f"k_out / v_out must be contiguous {list(shape)} tensors "
+                                     "of one type")
         if dtype not in _DT:
             raise ValueError("dtype must be fp16, bf16 or fp32")
         if k_out is None:
-            k_out = torch.empty(shape, dtype=dtype, device=dev)
+            k_out = torch.empty(shape, dtype=dtype, device=cache.pool.device)
         if v_out is None:
-            v_out = torch.empty(shape, dtype=dtype, device=dev)
+            v_out = torch.empty(shape, dtype=dtype, device=cache.pool.device)
+        bt, mb = _table(block_tables, B)
         L.check("tkv_int8_read", L.lib().tkv_int8_read(
-            C.byref(cache._c), k_out.data_ptr(), v_out.data_ptr(), _DT[dtype],
-            _index("block_tables", block_tables, B, None), block_tables.shape[1],
-            _index("starts", starts, B), _index("cu", cu, B + 1), B, shape[0],
+            cache._ref, k_out.data_ptr(), v_out.data_ptr(), _DT[dtype], bt, mb,
+            _index("starts", starts, (B,)), _index("cu", cu, (B + 1,)), B, shape[0],
             shape[0] if max_tokens is None else int(max_tokens), _err_ptr(err), s))
     return k_out, v_out
 
@@ -776,37 +811,35 @@ def int8_attend(cache: Int8PagedCache, q: torch.Tensor, cu_q: torch.Tensor,
     appended; each attends to itself and the tokens before it, or to the last
     `window` of them.  One row a sequence is a decode step.  Returns out [T, Hq,
     D] (fp16 or bf16); its rows outside the sequences are not written."""
-    _need_cuda(q, cu_q, block_tables, seq_lens, out, workspace)
     _no_grad_path("int8_attend", q)
-    dev = cache.pool.device
-    _same_device(dev, q, cu_q, block_tables, seq_lens, out, workspace, err)
-    B = int(seq_lens.shape[0]) if seq_lens.dim() == 1 else -1
-    with _On(dev, stream) as s:
+    dev = cache._device
+    _one_device(max(dev, 0), cache.pool, q, cu_q, block_tables, seq_lens, out, workspace, err)
+    B = _count(seq_lens)
+    with _on(dev, stream) as s:
         x = _heads("q", q)
         T, Hq, D = x.shape
         if D != cache.head_dim:
             raise ValueError(f"q has {D} channels, the cache {cache.head_dim}")
         if Hq % cache.n_kv_heads:
             raise ValueError(f"{Hq} q heads do not share {cache.n_kv_heads} kv heads evenly")
-        bt = _index("block_tables", block_tables, B, None)
-        mb = int(block_tables.shape[1])
+        bt, mb = _table(block_tables, B)
         mq = T if max_q_tokens is None else int(max_q_tokens)
         ml = mb * L.TKV_PAGE_SIZE if max_context_len is None else int(max_context_len)
         if out is None:
-            out = torch.empty((T, Hq, D), dtype=out_dtype or x.dtype, device=dev)
-        elif tuple(out.shape) != (T, Hq, D) or not out.is_contiguous():
+            out = torch.empty((T, Hq, D), dtype=out_dtype or x.dtype, device=x.device)
+        elif out.shape != (T, Hq, D) or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {[T, Hq, D]} tensor")
-        if out.dtype not in (torch.float16, torch.bfloat16):
+        if out.dtype not in _HALF:
             raise ValueError("out must be fp16 or bf16")
         if workspace is None:
-            workspace = int8_workspace(B, Hq, cache.n_kv_heads, D, mq, ml, dev)
+            workspace = int8_workspace(B, Hq, cache.n_kv_heads, D, mq, ml, x.device)
         elif not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
         st = x.stride()
         L.check("tkv_int8_attend", L.lib().tkv_int8_attend(
-            C.byref(cache._c), x.data_ptr(), _DT[x.dtype], (C.c_int64 * 2)(st[0], st[1]),
-            out.data_ptr(), _DT[out.dtype], _index("cu_q", cu_q, B + 1), bt, mb,
-            _index("seq_lens", seq_lens, B), B, Hq, T, mq, ml, int(window),
+            cache._ref, x.data_ptr(), _DT[x.dtype], _I64x2(st[0], st[1]),
+            out.data_ptr(), _DT[out.dtype], _index("cu_q", cu_q, (B + 1,)), bt, mb,
+            _index("seq_lens", seq_lens, (B,)), B, Hq, T, mq, ml, int(window),
             1.0 / math.sqrt(D) if scale is None else float(scale), workspace.data_ptr(),
-            workspace.numel() * workspace.element_size(), _err_ptr(err), s))
+            workspace.nbytes, _err_ptr(err), s))
     return out
