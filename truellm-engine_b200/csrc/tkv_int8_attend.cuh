@@ -6,9 +6,14 @@
 
 namespace tkv {
 
-constexpr float kInt8Lazy = 8.f;        // log2 units a score may exceed its row's reference by
-constexpr float kInt8ScaleTop = 4.f;    // largest value scale over 2^E
-constexpr float kInt8WeightUp = 32.f;   // f16 weights are held times this
+// Range of the f16 weights.  A row's softmax reference m is moved only when its
+// weights outgrow 2^kInt8Lazy; the value scales are divided by a power of two 2^E
+// that is raised when one exceeds it; weights are held times 2^5.  So they stay
+// at 2^15 or below, and lose bits (fp16 has steps of 2^-24 at the bottom) only
+// below 2^-19 of the largest value row.
+constexpr float kInt8Lazy = 10.f;
+constexpr float kInt8LazyWeight = 1024.f;  // 2^kInt8Lazy
+constexpr float kInt8WeightUp = 32.f;
 constexpr int kInt8DecodeRows = 16;     // most rows of the decode kernel
 
 // Runs of a context.  Decode: `n` runs at most per (sequence, kv head), each of
@@ -37,6 +42,32 @@ __device__ __forceinline__ bool int8_attend_ok(const Int8AttendArgs& a, int len,
          n <= len && n <= a.max_q && q0 >= 0 && q0 <= a.total_q - n;
 }
 
+// A bounded wait without the suspend hint of mbar_wait (whose sleep outlasts the
+// few hundred cycles between these kernels' hand-overs): gives up after about
+// two seconds of the global timer.
+__device__ __forceinline__ bool mbar_wait_near(uint64_t* bar, uint32_t parity, int* err) {
+  const uint32_t addr = smem_u32(bar);
+  uint64_t t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if ((i & 255u) == 0) {
+      const uint64_t now = global_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > 2000000000ull) break;
+    }
+  }
+  set_err(err, TKV_ERR_TIMEOUT);
+  return false;
+}
+
 // Powers of two that bring a row whose largest magnitude is m into fp16's
 // range: down = 2^-e, up = 2^e with m 2^-e in [1, 4); 1 for zeros, infinities.
 __device__ __forceinline__ void int8_row_power(float m, float& up, float& down) {
@@ -49,7 +80,8 @@ __device__ __forceinline__ void int8_row_power(float m, float& up, float& down) 
   }
 }
 
-// 2^-E with s 2^-E in [1/2, 1), s > 0 a finite scale (at most 2^121)
+// 2^-E with s 2^-E in [1/2, 1), s > 0 a finite scale (at most 2^121); E is raised
+// when a scale exceeds 2^E
 __device__ __forceinline__ float int8_scale_inverse(float s) {
   const int e = static_cast<int>(__float_as_uint(s) >> 23);  // 2^(e - 127) <= s
   return __uint_as_float(static_cast<uint32_t>(min(253, max(1, 253 - e))) << 23);

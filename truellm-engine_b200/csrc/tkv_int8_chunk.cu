@@ -38,40 +38,34 @@ constexpr int kTP = kTN / kPage; // pages per tile
 constexpr int kSoftmax = 256, kProducers = 128;
 constexpr int kCtaThreads = kSoftmax + kProducers + 32;
 
-// n 32-bit words to this thread's lane, n consecutive columns
-__device__ __forceinline__ void st16u(uint32_t taddr, const uint32_t (&v)[16]) {
+// 32 words to this thread's lane, 32 consecutive columns
+__device__ __forceinline__ void st32u(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
-      "%11, %12, %13, %14, %15, %16};\n" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {"
+      "%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, "
+      "%19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32 "
+      "};\n" ::"r"(taddr),
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+      "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+      "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+      "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
+}
+
+// Waits for the loads in flight; v's values come out of this statement, so no
+// use of them can move before it.
+__device__ __forceinline__ void wait_ld_of(float (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]),
+                 "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]),
+                 "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
+               :
+               : "memory");
 }
 
 // n consecutive 32-bit columns of this thread's lane; load and wait are one
 // statement, so nothing can use a value before it has arrived
-__device__ __forceinline__ void ld64_wait(uint32_t taddr, float (&v)[64]) {
-  asm volatile(
-      "{\n\ttcgen05.ld.sync.aligned.32x32b.x64.b32 {"
-      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
-      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, "
-      "%34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, "
-      "%50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63 "
-      "}, [%64];\n\ttcgen05.wait::ld.sync.aligned;\n\t}\n"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
-        "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
-        "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]),
-        "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]),
-        "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31]),
-        "=f"(v[32]), "=f"(v[33]), "=f"(v[34]), "=f"(v[35]), "=f"(v[36]), "=f"(v[37]),
-        "=f"(v[38]), "=f"(v[39]), "=f"(v[40]), "=f"(v[41]), "=f"(v[42]), "=f"(v[43]),
-        "=f"(v[44]), "=f"(v[45]), "=f"(v[46]), "=f"(v[47]), "=f"(v[48]), "=f"(v[49]),
-        "=f"(v[50]), "=f"(v[51]), "=f"(v[52]), "=f"(v[53]), "=f"(v[54]), "=f"(v[55]),
-        "=f"(v[56]), "=f"(v[57]), "=f"(v[58]), "=f"(v[59]), "=f"(v[60]), "=f"(v[61]),
-        "=f"(v[62]), "=f"(v[63])
-      : "r"(taddr)
-      : "memory");
-}
 __device__ __forceinline__ void ld32_wait(uint32_t taddr, float (&v)[32]) {
   asm volatile(
       "{\n\ttcgen05.ld.sync.aligned.32x32b.x32.b32 {"
@@ -104,6 +98,67 @@ __device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
       : "=l"(d)
       : "l"(*reinterpret_cast<const uint64_t*>(&a)), "l"(*reinterpret_cast<const uint64_t*>(&b)));
   return *reinterpret_cast<const float2*>(&d);
+}
+
+// 16 scores of a row (tokens t ..) times their key scales; MASKED: tokens that
+// the row does not see (outside [pmin, plim]) become -inf.
+template <bool MASKED>
+__device__ __forceinline__ void scale_scores(float (&x)[16], const float4* ks4, int t, int pmin,
+                                             int plim) {
+#pragma unroll
+  for (int c = 0; c < 16; c += 4) {
+    const float4 k4 = ks4[c / 4];
+    const float2 p0 = fmul2(make_float2(x[c], x[c + 1]), make_float2(k4.x, k4.y));
+    const float2 p1 = fmul2(make_float2(x[c + 2], x[c + 3]), make_float2(k4.z, k4.w));
+    x[c] = p0.x, x[c + 1] = p0.y, x[c + 2] = p1.x, x[c + 3] = p1.y;
+  }
+  if constexpr (MASKED) {
+#pragma unroll
+    for (int c = 0; c < 16; ++c) x[c] = t + c <= plim && t + c >= pmin ? x[c] : -INFINITY;
+  }
+}
+
+// Their weights 2^(x ra + nm): added to sum, and times the value scales (2^-E
+// 2^5 included) as f16 pairs.  A masked token's is 0 whatever its scale holds.
+template <bool MASKED>
+__device__ __forceinline__ void score_weights(const float (&x)[16], const float4* vs4, float2 ra2,
+                                              float2 nm2, float2& sum, uint32_t* pk) {
+#pragma unroll
+  for (int c = 0; c < 16; c += 4) {
+    const float4 v4 = vs4[c / 4];
+    const float2 y0 = ffma2(make_float2(x[c], x[c + 1]), ra2, nm2);
+    const float2 y1 = ffma2(make_float2(x[c + 2], x[c + 3]), ra2, nm2);
+    const float2 p0 = make_float2(fast_exp2(y0.x), fast_exp2(y0.y));
+    const float2 p1 = make_float2(fast_exp2(y1.x), fast_exp2(y1.y));
+    sum = fadd2(sum, fadd2(p0, p1));
+    float2 w0 = fmul2(p0, make_float2(v4.x, v4.y)), w1 = fmul2(p1, make_float2(v4.z, v4.w));
+    if constexpr (MASKED) {
+      w0.x = x[c] == -INFINITY ? 0.f : w0.x;
+      w0.y = x[c + 1] == -INFINITY ? 0.f : w0.y;
+      w1.x = x[c + 2] == -INFINITY ? 0.f : w1.x;
+      w1.y = x[c + 3] == -INFINITY ? 0.f : w1.y;
+    }
+    pk[c / 2] = pack_h2(w0.x, w0.y);
+    pk[c / 2 + 1] = pack_h2(w1.x, w1.y);
+  }
+}
+
+// The weights of 64 tokens (scores at tensor-memory column ts) with the
+// reference as it is, loads one step ahead.
+template <bool MASKED>
+__device__ __forceinline__ void half_weights(uint32_t ts, const float4* ks4, const float4* vs4, int t,
+                                             int pmin, int plim, float2 ra2, float nm, float2& sum,
+                                             uint32_t (&pk)[32]) {
+  const float2 nm2 = make_float2(nm, nm);
+  float x[2][16];
+  umma::ld16(ts, x[0]);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    wait_ld_of(x[q & 1]);
+    if (q < 3) umma::ld16(ts + 16 * (q + 1), x[(q + 1) & 1]);
+    scale_scores<MASKED>(x[q & 1], ks4 + 4 * q, t + 16 * q, pmin, plim);
+    score_weights<MASKED>(x[q & 1], vs4 + 4 * q, ra2, nm2, sum, &pk[8 * q]);
+  }
 }
 
 template <int D>
@@ -293,7 +348,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       const int b = j & 1, ph = (j >> 1) & 1;
       const bool more = j + 1 < nj;
       if (more) fetch_ids(j_lo + j + 1);
-      if (j >= 2 && !mbar_wait_fast(&kfree[b], ph ^ 1, a.err)) break;
+      if (j >= 2 && !mbar_wait_near(&kfree[b], ph ^ 1, a.err)) break;
       if (scales) {
         const float kv[8] = {__uint_as_float(sr0.x), __uint_as_float(sr0.y), __uint_as_float(sr0.z),
                              __uint_as_float(sr0.w), __uint_as_float(sr1.x), __uint_as_float(sr1.y),
@@ -307,7 +362,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         }
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        if (top * vinv > kInt8ScaleTop) vinv = int8_scale_inverse(top);
+        if (top * vinv > 1.f) vinv = int8_scale_inverse(top);
         const int buf = j % 3;
         *reinterpret_cast<float4*>(ks_s + buf * kTN + 4 * lane) = make_float4(kv[0], kv[2], kv[4], kv[6]);
         *reinterpret_cast<float4*>(vs_s + buf * kTN + 4 * lane) =
@@ -330,7 +385,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       umma::fence_smem_to_async();
       mbar_arrive(&kready[b]);
       if (more) load_k();
-      if (j >= 2 && !mbar_wait_fast(&vfree[b], ph ^ 1, a.err)) break;
+      if (j >= 2 && !mbar_wait_near(&vfree[b], ph ^ 1, a.err)) break;
       uint8_t* const vd = smem + SM::V_OFF + b * SM::V_BYTES + v_dst;
 #pragma unroll
       for (int i = 0; i < UPT; ++i) {
@@ -364,20 +419,24 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         if (w == wgs - 1) umma::commit(&kfree[j & 1]);
         last_s[w] = j;
       };
-      ok = mbar_wait(&kready[0], 0, a.err);
+      ok = mbar_wait_near(&kready[0], 0, a.err);
       for (int w = 0; ok && w < wgs; ++w) issue_s(w, 0);
       for (int j = 0; ok && j < nj; ++j) {
-        ok = mbar_wait(&vready[j & 1], (j >> 1) & 1, a.err);
-        for (int w = 0; ok && w < wgs; ++w) {
-          for (int hf = 0; ok && hf < 2; ++hf) {
-            ok = mbar_wait(&pready[2 * w + hf], j & 1, a.err);
+        ok = mbar_wait_near(&vready[j & 1], (j >> 1) & 1, a.err);
+        const uint64_t dvj = dv + (j & 1) * (SM::V_BYTES >> 4);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if (!ok || w >= wgs) break;
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {
+            ok = ok && mbar_wait_near(&pready[2 * w + hf], j & 1, a.err);
             if (!ok) break;
             umma::fence_after_sync();
 #pragma unroll
             for (int kk = 0; kk < kTN / 32; ++kk) {
               const int k = hf * (kTN / 32) + kk;
-              umma::mma_f16_ta(tmem + w * SM::TWG + SM::TO, tmem + w * SM::TWG + 8 * k,
-                               dv + (j & 1) * (SM::V_BYTES >> 4) + 16 * k, idO, j > 0 || k > 0);
+              umma::mma_f16_ta(tmem + w * SM::TWG + SM::TO, tmem + w * SM::TWG + 8 * k, dvj + 16 * k,
+                               idO, j > 0 || k > 0);
             }
             umma::commit(&odone[2 * w + hf]);
             last_h[w][hf] = j;
@@ -386,17 +445,17 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
           umma::commit(&vfree[j & 1]);
           if (j + 1 < nj) {
             // S of the next tile overwrites the scores and weights of this one
-            ok = mbar_wait(&kready[(j + 1) & 1], ((j + 1) >> 1) & 1, a.err) &&
-                 mbar_wait(&odone[2 * w + 1], j & 1, a.err);
+            ok = mbar_wait_near(&kready[(j + 1) & 1], ((j + 1) >> 1) & 1, a.err) &&
+                 mbar_wait_near(&odone[2 * w + 1], j & 1, a.err);
             if (ok) issue_s(w, j + 1);
           }
         }
       }
       // no MMA may still run when tensor memory is released
       for (int w = 0; w < 2; ++w) {
-        if (last_s[w] >= 0) mbar_wait(&sdone[w], last_s[w] & 1, nullptr);
+        if (last_s[w] >= 0) mbar_wait_near(&sdone[w], last_s[w] & 1, nullptr);
         for (int hf = 0; hf < 2; ++hf)
-          if (last_h[w][hf] >= 0) mbar_wait(&odone[2 * w + hf], last_h[w][hf] & 1, nullptr);
+          if (last_h[w][hf] >= 0) mbar_wait_near(&odone[2 * w + hf], last_h[w][hf] & 1, nullptr);
       }
     }
   } else if (wg < wgs) {
@@ -409,45 +468,51 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     bool ok = true;
     for (int j = 0; j < nj; ++j) {
       const int buf = j % 3, t0 = (j_lo + j) * kTN;
-      ok = mbar_wait_fast(&sready[buf], (j / 3) & 1, a.err) &&
-           mbar_wait_fast(&sdone[wg], j & 1, a.err);
+      ok = mbar_wait_near(&sready[buf], (j / 3) & 1, a.err) &&
+           mbar_wait_near(&sdone[wg], j & 1, a.err);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       umma::fence_after_sync();
-      const bool masked = t0 + kTN - 1 > plim || t0 < pmin;
+      const bool masked = __any_sync(0xffffffffu, t0 + kTN - 1 > plim || t0 < pmin);
       const float vnew = vi_s[buf];
       float fv = 1.f;
       if (vnew != vinv) {
         fv = vnew / vinv;
         vinv = vnew;
       }
+      const float2 ra2 = make_float2(ra, ra);
 #pragma unroll 1
       for (int hf = 0; hf < 2; ++hf) {
-        float x[64];
-        ld64_wait(tS + 64 * hf, x);
         const float4* ks4 = reinterpret_cast<const float4*>(ks_s + buf * kTN + 64 * hf);
-        float mx = -INFINITY;
+        const float4* vs4 = reinterpret_cast<const float4*>(vs_s + buf * kTN + 64 * hf);
+        const int th = t0 + 64 * hf;
+        // One pass with the reference as it is: no maximum is taken.  A sum of
+        // 2^kInt8Lazy or less shows that no weight has outgrown it.
+        float2 sum = make_float2(0.f, 0.f);
+        uint32_t pk[32];
+        if (masked)
+          half_weights<true>(tS + 64 * hf, ks4, vs4, th, pmin, plim, ra2, m == -INFINITY ? 0.f : -m,
+                             sum, pk);
+        else
+          half_weights<false>(tS + 64 * hf, ks4, vs4, th, pmin, plim, ra2, m == -INFINITY ? 0.f : -m,
+                              sum, pk);
+        if (__any_sync(0xffffffffu, sum.x + sum.y > kInt8LazyWeight || m == -INFINITY || fv != 1.f)) {
+          // The reference has to move (or the value scales' power of two has):
+          // the half's maximum, O and l brought to the new reference, and the
+          // half's weights again (its scores are still in tensor memory).
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+            float x[16];
+            ld16_wait(tS + 64 * hf + 16 * q, x);
+            scale_scores<true>(x, ks4 + 4 * q, th + 16 * q, pmin, plim);
 #pragma unroll
-        for (int c = 0; c < 64; c += 4) {
-          const float4 k4 = ks4[c / 4];
-          const float2 p0 = fmul2(make_float2(x[c], x[c + 1]), make_float2(k4.x, k4.y));
-          const float2 p1 = fmul2(make_float2(x[c + 2], x[c + 3]), make_float2(k4.z, k4.w));
-          x[c] = p0.x, x[c + 1] = p0.y, x[c + 2] = p1.x, x[c + 3] = p1.y;
-        }
-        if (masked) {
-#pragma unroll
-          for (int c = 0; c < 64; ++c) {
-            const int t = t0 + 64 * hf + c;
-            x[c] = t <= plim && t >= pmin ? x[c] : -INFINITY;
+            for (int c = 0; c < 16; c += 2) mx = fmaxf(mx, fmaxf(x[c], x[c + 1]));
           }
-        }
-#pragma unroll
-        for (int c = 0; c < 64; c += 2) mx = fmaxf(mx, fmaxf(x[c], x[c + 1]));
-        mx *= ra;  // ra > 0 keeps the order
-        const bool need = mx > m + kInt8Lazy;
-        if (__any_sync(0xffffffffu, need || fv != 1.f)) {
-          float f = need ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
-          m = need ? mx : m;
+          mx *= ra;  // ra > 0 keeps the order
+          const bool up = mx > m;
+          float f = up ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
+          m = up ? mx : m;
           l *= f;
           f *= fv;
           fv = 1.f;
@@ -455,11 +520,11 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
             // O holds the tiles before (done: S of this tile was issued after
             // them) and, in the second half, the first one's products
             if (hf > 0) {
-              ok = __all_sync(0xffffffffu, mbar_wait_fast(&odone[2 * wg], j & 1, a.err));
+              ok = __all_sync(0xffffffffu, mbar_wait_near(&odone[2 * wg], j & 1, a.err));
               if (!ok) break;
               umma::fence_after_sync();
             }
-#pragma unroll
+#pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 16) {
               float o[16];
               ld16_wait(tO + c0, o);
@@ -469,36 +534,12 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
             }
             umma::wait_st();
           }
-        }
-        const float nm = m == -INFINITY ? 0.f : -m;
-        const float2 ra2 = make_float2(ra, ra), nm2 = make_float2(nm, nm);
-        float2 sum = make_float2(0.f, 0.f);
-        const float4* vs4 = reinterpret_cast<const float4*>(vs_s + buf * kTN + 64 * hf);
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          uint32_t pw[16];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int c = 32 * q + 4 * e;
-            const float4 v4 = vs4[c / 4];
-            const float2 y0 = ffma2(make_float2(x[c], x[c + 1]), ra2, nm2);
-            const float2 y1 = ffma2(make_float2(x[c + 2], x[c + 3]), ra2, nm2);
-            const float2 p0 = make_float2(fast_exp2(y0.x), fast_exp2(y0.y));
-            const float2 p1 = make_float2(fast_exp2(y1.x), fast_exp2(y1.y));
-            sum = fadd2(sum, fadd2(p0, p1));
-            float2 w0 = fmul2(p0, make_float2(v4.x, v4.y)), w1 = fmul2(p1, make_float2(v4.z, v4.w));
-            if (masked) {  // whatever the scale holds
-              w0.x = x[c] == -INFINITY ? 0.f : w0.x;
-              w0.y = x[c + 1] == -INFINITY ? 0.f : w0.y;
-              w1.x = x[c + 2] == -INFINITY ? 0.f : w1.x;
-              w1.y = x[c + 3] == -INFINITY ? 0.f : w1.y;
-            }
-            pw[2 * e] = pack_h2(w0.x, w0.y);
-            pw[2 * e + 1] = pack_h2(w1.x, w1.y);
-          }
-          st16u(tS + 32 * hf + 16 * q, pw);
+          sum = make_float2(0.f, 0.f);
+          half_weights<true>(tS + 64 * hf, ks4, vs4, th, pmin, plim, ra2, m == -INFINITY ? 0.f : -m,
+                             sum, pk);
         }
         l += sum.x + sum.y;
+        st32u(tS + 32 * hf, pk);
         umma::wait_st();
         umma::fence_before_sync();
         mbar_arrive(&pready[2 * wg + hf]);
@@ -506,7 +547,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       if (!ok) break;
     }
     if (ok && nj > 0)
-      ok = mbar_wait(&odone[2 * wg], (nj - 1) & 1, a.err) && mbar_wait(&odone[2 * wg + 1], (nj - 1) & 1, a.err);
+      ok = mbar_wait_near(&odone[2 * wg], (nj - 1) & 1, a.err) && mbar_wait_near(&odone[2 * wg + 1], (nj - 1) & 1, a.err);
     ok = __all_sync(0xffffffffu, ok);
     umma::fence_after_sync();
     // ---- normalise and write the row (a run's partial when the context is split) ----

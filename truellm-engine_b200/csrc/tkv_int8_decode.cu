@@ -15,12 +15,6 @@
 // A masked token's weight is exactly 0 whatever its scales hold (codes are
 // always finite numbers), so a NaN reaches only the rows that see it.
 //
-// Range of the f16 weights: the softmax reference m of a row moves only when a
-// score exceeds it by 2^kLazy, and the value scales are divided by a running
-// power of two 2^E >= the largest scale / 4; weights are held times 2^5, so they
-// stay below 2^kLazy 2^2 2^5 = 2^15 and lose bits (fp16 has steps of 2^-24 at
-// the bottom) only below 2^-19 of the largest value row.
-//
 // Runs of one pair are joined by the CTA that finishes last (partials in the
 // workspace, a counter per pair that the last CTA zeroes again); the order of
 // the sum is that of the runs, so the result does not depend on who is last.
@@ -282,12 +276,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
         need |= mx[nt][e] > m[nt][e] + kInt8Lazy;
       }
     float svm = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
-    need |= svm * vinv > kInt8ScaleTop;
+    need |= svm * vinv > 1.f;
     if (__any_sync(0xffffffffu, need)) {
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) svm = fmaxf(svm, __shfl_xor_sync(0xffffffffu, svm, d));
       float fv = 1.f;
-      if (svm * vinv > kInt8ScaleTop) {
+      if (svm * vinv > 1.f) {
         const float v2 = int8_scale_inverse(svm);
         fv = v2 / vinv;
         vinv = v2;
