@@ -7,20 +7,25 @@
 //                        become exact f16 integers in the K-major operands K
 //                        [128 tokens][D] and V^T [D][128 tokens] (double
 //                        buffered); one of the warps also brings the scales
-//   MMA (1 warp, 1 lane) S = Q K^T per softmax warpgroup into tensor memory
-//                        (M = N = 128), O += P V with P read from tensor memory
+//   MMA (2 warps, 1 lane each, one per softmax warpgroup) steps of 64 tokens: S =
+//                        Q K^T into tensor memory (two buffers), O += P V with P
+//                        read from tensor memory
 //   softmax (2 x 4 warps) one thread per query row: score x key scale, online
 //                        softmax, weight x value scale rounded once to f16 and
-//                        written to tensor memory over the scores (in two
-//                        halves of 64 tokens, so O += P V starts at the first)
-// The two warpgroups alternate: while one computes its weights the tensor cores
-// run the other's products.  Scales multiply finished 32-bit numbers only, so
-// the codes enter both products exactly; a masked token's weight is exactly 0.
-// References of the softmax and of the value scales as in tkv_int8_decode.cu.
+//                        written to tensor memory over the scores
+// S of step i + 1 is in tensor memory while the weights of step i are computed;
+// S of step i + 2 takes the buffer of step i once O += P V of step i is done.
+// Steps of 64 tokens cost half again as much for S as steps of 128 (N = 64 reads
+// more shared memory per product: 49 cycles where 32 would do), but with 128
+// there is room for one buffer only, and every warpgroup then waits for its
+// products' latency in each step (measured: 4800 cycles per 128 tokens).
+// Scales multiply finished 32-bit numbers only, so the codes enter both products
+// exactly; a masked token's weight is exactly 0.
 //
-// Tensor memory of warpgroup w (256 columns): S at 0 (its weights P, f16 pairs,
-// over columns 0 .. 63), O at 128.  Column 8 (4 u + j) + g of O is channel 32 u
-// + 4 g + j: the order in which a V unit's words are stored without conflicts.
+// Tensor memory of warpgroup w (256 columns): S of even and odd steps at 0 and 64
+// (their weights P, f16 pairs, over the first 32 columns), O at 128.  Column 8 (4
+// u + j) + g of O is channel 32 u + 4 g + j: the order in which a V unit's words
+// are stored without conflicts.
 #include <limits.h>
 
 #include <algorithm>
@@ -36,7 +41,8 @@ constexpr int kRows = 128;       // rows of a softmax warpgroup (the MMA's M)
 constexpr int kTN = 128;         // tokens per tile
 constexpr int kTP = kTN / kPage; // pages per tile
 constexpr int kSoftmax = 256, kProducers = 128;
-constexpr int kCtaThreads = kSoftmax + kProducers + 32;
+constexpr int kStep = 64;        // tokens of one S / O += P V step
+constexpr int kCtaThreads = kSoftmax + kProducers + 64;
 
 // 32 words to this thread's lane, 32 consecutive columns
 __device__ __forceinline__ void st32u(uint32_t taddr, const uint32_t (&v)[32]) {
@@ -143,10 +149,10 @@ __device__ __forceinline__ void score_weights(const float (&x)[16], const float4
   }
 }
 
-// The weights of 64 tokens (scores at tensor-memory column ts) with the
-// reference as it is, loads one step ahead.
+// The weights of a step's 64 tokens (scores at tensor-memory column ts), its
+// loads one ahead.
 template <bool MASKED>
-__device__ __forceinline__ void half_weights(uint32_t ts, const float4* ks4, const float4* vs4, int t,
+__device__ __forceinline__ void step_weights(uint32_t ts, const float4* ks4, const float4* vs4, int t,
                                              int pmin, int plim, float2 ra2, float nm, float2& sum,
                                              uint32_t (&pk)[32]) {
   const float2 nm2 = make_float2(nm, nm);
@@ -188,22 +194,22 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   // Barriers (tile j counted from the CTA's first; b = j % 2):
   //   kready[b], vready[b]  operands stored (128 producer arrivals)
-  //   kfree[b]              S of tile j done in every warpgroup (commit)
-  //   vfree[b]              O += P V of tile j done (a commit per warpgroup)
+  //   kfree[b], vfree[b]    S, O += P V of tile j done (a commit per warpgroup)
   //   sready[j % 3]         scales stored (32 arrivals)
-  //   sdone[w]              S of tile j done (commit)
-  //   pready[w][h]          half h of P of tile j written (128 arrivals)
-  //   odone[w][h]           O += P V of that half done (commit)
+  // and of warpgroup w, step i (two a tile), in turn for even and odd steps:
+  //   sdone[w][i % 2]       S done (commit)
+  //   pready[w][i % 2]      P written (128 arrivals)
+  //   odone[w][i % 2]       O += P V done (commit)
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + SM::BAR_OFF);
   uint64_t* const kready = bars;
   uint64_t* const vready = bars + 2;
   uint64_t* const kfree = bars + 4;
   uint64_t* const vfree = bars + 6;
   uint64_t* const sready = bars + 8;
-  uint64_t* const sdone = bars + 11;
-  uint64_t* const pready = bars + 13;  // [2 w + h]
-  uint64_t* const odone = bars + 17;   // [2 w + h]
-  uint32_t* const tslot = reinterpret_cast<uint32_t*>(bars + 21);
+  uint64_t* const sdone = bars + 11;   // [2 w + i % 2]
+  uint64_t* const pready = bars + 15;  // [2 w + i % 2]
+  uint64_t* const odone = bars + 19;   // [2 w + i % 2]
+  uint32_t* const tslot = reinterpret_cast<uint32_t*>(bars + 23);
   float* const ks_s = reinterpret_cast<float*>(smem + SM::KS_OFF);
   float* const vs_s = reinterpret_cast<float*>(smem + SM::VS_OFF);
   float* const vi_s = reinterpret_cast<float*>(smem + SM::VI_OFF);
@@ -231,12 +237,11 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   if (warp == 0) umma::alloc(tslot, SM::TCOLS);
   if (ctid == 0) {
     for (int i = 0; i < 4; ++i) mbar_init(&bars[i], kProducers);      // kready, vready
-    for (int i = 4; i < 6; ++i) mbar_init(&bars[i], 1);               // kfree
-    for (int i = 6; i < 8; ++i) mbar_init(&bars[i], wgs);             // vfree
+    for (int i = 4; i < 8; ++i) mbar_init(&bars[i], wgs);             // kfree, vfree
     for (int i = 8; i < 11; ++i) mbar_init(&bars[i], 32);             // sready
-    for (int i = 11; i < 13; ++i) mbar_init(&bars[i], 1);             // sdone
-    for (int i = 13; i < 17; ++i) mbar_init(&bars[i], kRows);         // pready
-    for (int i = 17; i < 21; ++i) mbar_init(&bars[i], 1);             // odone
+    for (int i = 11; i < 15; ++i) mbar_init(&bars[i], 1);             // sdone
+    for (int i = 15; i < 19; ++i) mbar_init(&bars[i], kRows);         // pready
+    for (int i = 19; i < 23; ++i) mbar_init(&bars[i], 1);             // odone
     fence_mbar_init();
   }
 
@@ -285,7 +290,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = *tslot;
-  constexpr uint32_t idS = umma::idesc_f16(kRows, kTN, false);
+  constexpr uint32_t idS = umma::idesc_f16(kRows, kStep, false);
   constexpr uint32_t idO = umma::idesc_f16(kRows, D, false);
 
   if (ctid >= kSoftmax && ctid < kSoftmax + kProducers) {
@@ -402,61 +407,53 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       if (more) load_v();
     }
   } else if (ctid >= kSoftmax + kProducers) {
-    // ============================ the MMA warp ============================
-    if (lane == 0 && nj > 0) {
+    // ============================ an MMA warp ============================
+    const int w = warp - (kSoftmax + kProducers) / 32;  // its softmax warpgroup
+    if (lane == 0 && w < wgs && nj > 0) {
+      const int steps = 2 * nj;
       bool ok = true;
-      int last_s[2] = {-1, -1}, last_h[2][2] = {{-1, -1}, {-1, -1}};
-      const uint64_t dq = umma::smem_desc(smem_u32(smem + SM::Q_OFF), 128, 16 * D);
+      int last_s = -1, last_o = -1;
+      const uint64_t dq = umma::smem_desc(smem_u32(smem + SM::Q_OFF + w * SM::Q_BYTES), 128, 16 * D);
       const uint64_t dk = umma::smem_desc(smem_u32(smem + SM::K_OFF), 128, 16 * D);
       const uint64_t dv = umma::smem_desc(smem_u32(smem + SM::V_OFF), 128, 16 * kTN);
-      auto issue_s = [&](int w, int j) {
+      const uint32_t tS = tmem + w * SM::TWG, tO = tS + SM::TO;
+      auto issue_s = [&](int i) {  // step i: tokens 64 (i % 2) .. of K buffer (i / 2) % 2
+        if ((i & 1) == 0) ok = mbar_wait_near(&kready[(i >> 1) & 1], (i >> 2) & 1, a.err);
+        if (!ok) return;
         umma::fence_after_sync();
+        const uint64_t d = dk + ((i >> 1) & 1) * (SM::K_BYTES >> 4) + (i & 1) * (SM::K_BYTES >> 5);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma::mma_f16(tmem + w * SM::TWG, dq + w * (SM::Q_BYTES >> 4) + 16 * kk,
-                        dk + (j & 1) * (SM::K_BYTES >> 4) + 16 * kk, idS, kk > 0);
-        umma::commit(&sdone[w]);
-        if (w == wgs - 1) umma::commit(&kfree[j & 1]);
-        last_s[w] = j;
+          umma::mma_f16(tS + (i & 1) * kStep, dq + 16 * kk, d + 16 * kk, idS, kk > 0);
+        umma::commit(&sdone[2 * w + (i & 1)]);
+        if (i & 1) umma::commit(&kfree[(i >> 1) & 1]);
+        last_s = i;
       };
-      ok = mbar_wait_near(&kready[0], 0, a.err);
-      for (int w = 0; ok && w < wgs; ++w) issue_s(w, 0);
-      for (int j = 0; ok && j < nj; ++j) {
-        ok = mbar_wait_near(&vready[j & 1], (j >> 1) & 1, a.err);
-        const uint64_t dvj = dv + (j & 1) * (SM::V_BYTES >> 4);
+      issue_s(0);
+      if (ok) issue_s(1);
+      for (int i = 0; ok && i < steps; ++i) {
+        if ((i & 1) == 0) ok = mbar_wait_near(&vready[(i >> 1) & 1], (i >> 2) & 1, a.err);
+        ok = ok && mbar_wait_near(&pready[2 * w + (i & 1)], (i >> 1) & 1, a.err);
+        if (!ok) break;
+        umma::fence_after_sync();
+        const uint64_t d = dv + ((i >> 1) & 1) * (SM::V_BYTES >> 4) + (i & 1) * (16 * kStep / 16);
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          if (!ok || w >= wgs) break;
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            ok = ok && mbar_wait_near(&pready[2 * w + hf], j & 1, a.err);
-            if (!ok) break;
-            umma::fence_after_sync();
-#pragma unroll
-            for (int kk = 0; kk < kTN / 32; ++kk) {
-              const int k = hf * (kTN / 32) + kk;
-              umma::mma_f16_ta(tmem + w * SM::TWG + SM::TO, tmem + w * SM::TWG + 8 * k, dvj + 16 * k,
-                               idO, j > 0 || k > 0);
-            }
-            umma::commit(&odone[2 * w + hf]);
-            last_h[w][hf] = j;
-          }
-          if (!ok) break;
-          umma::commit(&vfree[j & 1]);
-          if (j + 1 < nj) {
-            // S of the next tile overwrites the scores and weights of this one
-            ok = mbar_wait_near(&kready[(j + 1) & 1], ((j + 1) >> 1) & 1, a.err) &&
-                 mbar_wait_near(&odone[2 * w + 1], j & 1, a.err);
-            if (ok) issue_s(w, j + 1);
-          }
+        for (int kk = 0; kk < kStep / 16; ++kk)
+          umma::mma_f16_ta(tO, tS + (i & 1) * kStep + 8 * kk, d + 16 * kk, idO, i > 0 || kk > 0);
+        umma::commit(&odone[2 * w + (i & 1)]);
+        if (i & 1) umma::commit(&vfree[(i >> 1) & 1]);
+        last_o = i;
+        if (i + 2 < steps) {
+          // S of step i + 2 overwrites the scores and weights of this one
+          ok = mbar_wait_near(&odone[2 * w + (i & 1)], (i >> 1) & 1, a.err);
+          if (ok) issue_s(i + 2);
         }
       }
       // no MMA may still run when tensor memory is released
-      for (int w = 0; w < 2; ++w) {
-        if (last_s[w] >= 0) mbar_wait_near(&sdone[w], last_s[w] & 1, nullptr);
-        for (int hf = 0; hf < 2; ++hf)
-          if (last_h[w][hf] >= 0) mbar_wait_near(&odone[2 * w + hf], last_h[w][hf] & 1, nullptr);
-      }
+      for (int i = max(0, last_s - 1); i <= last_s; ++i)
+        mbar_wait_near(&sdone[2 * w + (i & 1)], (i >> 1) & 1, nullptr);
+      for (int i = max(0, last_o - 1); i <= last_o; ++i)
+        mbar_wait_near(&odone[2 * w + (i & 1)], (i >> 1) & 1, nullptr);
     }
   } else if (wg < wgs) {
     // ============================ softmax ============================
@@ -466,88 +463,79 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     const int pmin = a.window > 0 ? max(0, plim - a.window + 1) : 0;
     float m = -INFINITY, l = 0.f, vinv = 0x1p126f;
     bool ok = true;
-    for (int j = 0; j < nj; ++j) {
-      const int buf = j % 3, t0 = (j_lo + j) * kTN;
-      ok = mbar_wait_near(&sready[buf], (j / 3) & 1, a.err) &&
-           mbar_wait_near(&sdone[wg], j & 1, a.err);
+    const float2 ra2 = make_float2(ra, ra);
+    for (int i = 0; i < 2 * nj; ++i) {
+      const int j = i >> 1, buf = j % 3, t0 = (j_lo + j) * kTN + (i & 1) * kStep;
+      ok = ((i & 1) || mbar_wait_near(&sready[buf], (j / 3) & 1, a.err)) &&
+           mbar_wait_near(&sdone[2 * wg + (i & 1)], j & 1, a.err);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       umma::fence_after_sync();
-      const bool masked = __any_sync(0xffffffffu, t0 + kTN - 1 > plim || t0 < pmin);
+      bool masked = __any_sync(0xffffffffu, t0 + kStep - 1 > plim || t0 < pmin);
       const float vnew = vi_s[buf];
       float fv = 1.f;
       if (vnew != vinv) {
         fv = vnew / vinv;
         vinv = vnew;
       }
-      const float2 ra2 = make_float2(ra, ra);
+      const uint32_t tSi = tS + (i & 1) * kStep;
+      const float4* ks4 = reinterpret_cast<const float4*>(ks_s + buf * kTN + (i & 1) * kStep);
+      const float4* vs4 = reinterpret_cast<const float4*>(vs_s + buf * kTN + (i & 1) * kStep);
+      float2 sum;
+      uint32_t pk[32];
+      // A pass with the reference as it is: no maximum is taken.  A sum of
+      // 2^kInt8Lazy or less shows that no weight has outgrown it.
 #pragma unroll 1
-      for (int hf = 0; hf < 2; ++hf) {
-        const float4* ks4 = reinterpret_cast<const float4*>(ks_s + buf * kTN + 64 * hf);
-        const float4* vs4 = reinterpret_cast<const float4*>(vs_s + buf * kTN + 64 * hf);
-        const int th = t0 + 64 * hf;
-        // One pass with the reference as it is: no maximum is taken.  A sum of
-        // 2^kInt8Lazy or less shows that no weight has outgrown it.
-        float2 sum = make_float2(0.f, 0.f);
-        uint32_t pk[32];
+      for (int pass = 0;; ++pass) {
+        sum = make_float2(0.f, 0.f);
+        const float nm = m == -INFINITY ? 0.f : -m;
         if (masked)
-          half_weights<true>(tS + 64 * hf, ks4, vs4, th, pmin, plim, ra2, m == -INFINITY ? 0.f : -m,
-                             sum, pk);
+          step_weights<true>(tSi, ks4, vs4, t0, pmin, plim, ra2, nm, sum, pk);
         else
-          half_weights<false>(tS + 64 * hf, ks4, vs4, th, pmin, plim, ra2, m == -INFINITY ? 0.f : -m,
-                              sum, pk);
-        if (__any_sync(0xffffffffu, sum.x + sum.y > kInt8LazyWeight || m == -INFINITY || fv != 1.f)) {
-          // The reference has to move (or the value scales' power of two has):
-          // the half's maximum, O and l brought to the new reference, and the
-          // half's weights again (its scores are still in tensor memory).
-          float mx = -INFINITY;
+          step_weights<false>(tSi, ks4, vs4, t0, pmin, plim, ra2, nm, sum, pk);
+        if (pass || !__any_sync(0xffffffffu, sum.x + sum.y > kInt8LazyWeight || m == -INFINITY || fv != 1.f))
+          break;
+        // The reference has to move (or the value scales' power of two has): the
+        // step's maximum, O and l brought to the new reference, and the weights
+        // again (the scores are still in tensor memory).
+        float mx = -INFINITY;
 #pragma unroll 1
-          for (int q = 0; q < 4; ++q) {
-            float x[16];
-            ld16_wait(tS + 64 * hf + 16 * q, x);
-            scale_scores<true>(x, ks4 + 4 * q, th + 16 * q, pmin, plim);
+        for (int q = 0; q < 4; ++q) {
+          float x[16];
+          ld16_wait(tSi + 16 * q, x);
+          scale_scores<true>(x, ks4 + 4 * q, t0 + 16 * q, pmin, plim);
 #pragma unroll
-            for (int c = 0; c < 16; c += 2) mx = fmaxf(mx, fmaxf(x[c], x[c + 1]));
-          }
-          mx *= ra;  // ra > 0 keeps the order
-          const bool up = mx > m;
-          float f = up ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
-          m = up ? mx : m;
-          l *= f;
-          f *= fv;
-          fv = 1.f;
-          if (j > 0 || hf > 0) {
-            // O holds the tiles before (done: S of this tile was issued after
-            // them) and, in the second half, the first one's products
-            if (hf > 0) {
-              ok = __all_sync(0xffffffffu, mbar_wait_near(&odone[2 * wg], j & 1, a.err));
-              if (!ok) break;
-              umma::fence_after_sync();
-            }
-#pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 16) {
-              float o[16];
-              ld16_wait(tO + c0, o);
-#pragma unroll
-              for (int c = 0; c < 16; ++c) o[c] *= f;
-              umma::st16(tO + c0, o);
-            }
-            umma::wait_st();
-          }
-          sum = make_float2(0.f, 0.f);
-          half_weights<true>(tS + 64 * hf, ks4, vs4, th, pmin, plim, ra2, m == -INFINITY ? 0.f : -m,
-                             sum, pk);
+          for (int c = 0; c < 16; c += 2) mx = fmaxf(mx, fmaxf(x[c], x[c + 1]));
         }
-        l += sum.x + sum.y;
-        st32u(tS + 32 * hf, pk);
-        umma::wait_st();
-        umma::fence_before_sync();
-        mbar_arrive(&pready[2 * wg + hf]);
+        mx *= ra;  // ra > 0 keeps the order
+        const bool up = mx > m;
+        const float f = up ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
+        m = up ? mx : m;
+        l *= f;
+        if (i > 0) {  // O holds the steps before, once the last one's products are in
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait_near(&odone[2 * wg + ((i - 1) & 1)], ((i - 1) >> 1) & 1, a.err));
+          if (!ok) break;
+          umma::fence_after_sync();
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += 16) {
+            float o[16];
+            ld16_wait(tO + c0, o);
+#pragma unroll
+            for (int c = 0; c < 16; ++c) o[c] *= f * fv;
+            umma::st16(tO + c0, o);
+          }
+          umma::wait_st();
+        }
       }
       if (!ok) break;
+      l += sum.x + sum.y;
+      st32u(tSi, pk);
+      umma::wait_st();
+      umma::fence_before_sync();
+      mbar_arrive(&pready[2 * wg + (i & 1)]);
     }
-    if (ok && nj > 0)
-      ok = mbar_wait_near(&odone[2 * wg], (nj - 1) & 1, a.err) && mbar_wait_near(&odone[2 * wg + 1], (nj - 1) & 1, a.err);
+    if (ok && nj > 0) ok = mbar_wait_near(&odone[2 * wg + 1], (nj - 1) & 1, a.err);
     ok = __all_sync(0xffffffffu, ok);
     umma::fence_after_sync();
     // ---- normalise and write the row (a run's partial when the context is split) ----
