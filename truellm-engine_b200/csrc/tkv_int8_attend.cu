@@ -43,14 +43,14 @@ size_t decode_bytes(const Int8Splits& sp, int num_seqs, int num_kv_heads, int he
 }
 
 constexpr int kSMs = 148;       // CTAs of the chunk kernel: one per SM
-constexpr int kMinTiles = 4;    // 128-token tiles of a run
+constexpr int kMinTiles = 8;    // 64-token tiles of a run
 
 // How chunk contexts are cut: not at all when the row tiles alone fill the GPU.
 void chunk_splits(Int8ChunkSplits& sp, int num_seqs, int num_kv_heads, int grp, int max_q, int max_len) {
   const long long rows = static_cast<long long>(max_q) * grp;
   sp.row_tiles = static_cast<int>(std::min<long long>(INT_MAX, (rows + kInt8ChunkRows - 1) / kInt8ChunkRows));
   const long long ctas = std::max<long long>(1, static_cast<long long>(num_seqs) * num_kv_heads * sp.row_tiles);
-  const long long tiles = (static_cast<long long>(max_len) + 127) / 128;
+  const long long tiles = (static_cast<long long>(max_len) + 63) / 64;
   sp.n = static_cast<int>(std::max<long long>(1, std::min(kSMs / ctas, tiles / kMinTiles)));
 }
 

@@ -2,27 +2,26 @@
 // rows, on the 5th-generation tensor cores (tcgen05).
 //
 // A CTA takes 256 query rows (query token x q head of the kv head's group) of a
-// (sequence, kv head) and a run of 128-token tiles of its pages.  Roles:
+// (sequence, kv head) and a run of 64-token tiles of its pages.  Roles:
 //   producers (4 warps)  tiles of codes, loaded one tile ahead into registers,
 //                        become exact f16 integers in the K-major operands K
-//                        [128 tokens][D] and V^T [D][128 tokens] (double
-//                        buffered); one of the warps also brings the scales
-//   MMA (2 warps, 1 lane each, one per softmax warpgroup) steps of 64 tokens: S =
-//                        Q K^T into tensor memory (two buffers), O += P V with P
-//                        read from tensor memory
+//                        [64 tokens][D] and V^T [D][64 tokens] (four buffers);
+//                        one of the warps also brings the scales
+//   MMA (2 warps, 1 lane each, one per softmax warpgroup)  S = Q K^T into tensor
+//                        memory (two buffers), O += P V with P read from there
 //   softmax (2 x 4 warps) one thread per query row: score x key scale, online
 //                        softmax, weight x value scale rounded once to f16 and
 //                        written to tensor memory over the scores
-// S of step i + 1 is in tensor memory while the weights of step i are computed;
-// S of step i + 2 takes the buffer of step i once O += P V of step i is done.
-// Steps of 64 tokens cost half again as much for S as steps of 128 (N = 64 reads
+// S of tile i + 1 is in tensor memory while the weights of tile i are computed;
+// S of tile i + 2 takes the buffer of tile i once O += P V of tile i is done.
+// Tiles of 64 tokens cost half again as much for S as tiles of 128 (N = 64 reads
 // more shared memory per product: 49 cycles where 32 would do), but with 128
 // there is room for one buffer only, and every warpgroup then waits for its
-// products' latency in each step (measured: 4800 cycles per 128 tokens).
+// products' latency at each tile (measured: 4800 cycles per 128 tokens).
 // Scales multiply finished 32-bit numbers only, so the codes enter both products
 // exactly; a masked token's weight is exactly 0.
 //
-// Tensor memory of warpgroup w (256 columns): S of even and odd steps at 0 and 64
+// Tensor memory of warpgroup w (256 columns): S of even and odd tiles at 0 and 64
 // (their weights P, f16 pairs, over the first 32 columns), O at 128.  Column 8 (4
 // u + j) + g of O is channel 32 u + 4 g + j: the order in which a V unit's words
 // are stored without conflicts.
@@ -38,11 +37,15 @@ namespace tkv {
 namespace {
 
 constexpr int kRows = 128;       // rows of a softmax warpgroup (the MMA's M)
-constexpr int kTN = 128;         // tokens per tile
+constexpr int kTN = 64;          // tokens per tile
+constexpr int kStages = 4;       // K and V buffers
 constexpr int kTP = kTN / kPage; // pages per tile
 constexpr int kSoftmax = 256, kProducers = 128;
-constexpr int kStep = 64;        // tokens of one S / O += P V step
-constexpr int kCtaThreads = kSoftmax + kProducers + 64;
+constexpr int kCtaThreads = kSoftmax + kProducers + 128;  // the MMA warps' warpgroup: two idle
+// Registers a thread: launched with 128, then shared out by warpgroup
+constexpr int kRegsSoftmax = 176, kRegsProducer = 96, kRegsMma = 64;
+static_assert(kSoftmax * kRegsSoftmax + kProducers * kRegsProducer + 128 * kRegsMma <= kCtaThreads * 128,
+              "the shares are no more than the launch has");
 
 // 32 words to this thread's lane, 32 consecutive columns
 __device__ __forceinline__ void st32u(uint32_t taddr, const uint32_t (&v)[32]) {
@@ -59,6 +62,18 @@ __device__ __forceinline__ void st32u(uint32_t taddr, const uint32_t (&v)[32]) {
       : "memory");
 }
 
+// 16 consecutive columns of this thread's lane, in flight until wait_ld_of.
+// (No memory clobber on either: only tensor memory is read, and the compiler may
+// move shared-memory loads across them.)
+__device__ __forceinline__ void ld16_issue(uint32_t taddr, float (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];\n"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+        "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
+        "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr));
+}
 // Waits for the loads in flight; v's values come out of this statement, so no
 // use of them can move before it.
 __device__ __forceinline__ void wait_ld_of(float (&v)[16]) {
@@ -66,8 +81,7 @@ __device__ __forceinline__ void wait_ld_of(float (&v)[16]) {
                : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]),
                  "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]),
                  "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15])
-               :
-               : "memory");
+               :);
 }
 
 // n consecutive 32-bit columns of this thread's lane; load and wait are one
@@ -124,58 +138,73 @@ __device__ __forceinline__ void scale_scores(float (&x)[16], const float4* ks4, 
   }
 }
 
-// Their weights 2^(x ra + nm): added to sum, and times the value scales (2^-E
-// 2^5 included) as f16 pairs.  A masked token's is 0 whatever its scale holds.
+// The weights of a tile's 64 tokens (scores at tensor-memory column ts): 2^(x ra
+// + nm), added to sum, and times the value scales (2^-E 2^5 included) as f16
+// pairs.  A masked token's is 0 whatever its scale holds.  Sixteen tokens at a
+// time, one group's exponentials while the next one's scores are scaled.
 template <bool MASKED>
-__device__ __forceinline__ void score_weights(const float (&x)[16], const float4* vs4, float2 ra2,
-                                              float2 nm2, float2& sum, uint32_t* pk) {
-#pragma unroll
-  for (int c = 0; c < 16; c += 4) {
-    const float4 v4 = vs4[c / 4];
-    const float2 y0 = ffma2(make_float2(x[c], x[c + 1]), ra2, nm2);
-    const float2 y1 = ffma2(make_float2(x[c + 2], x[c + 3]), ra2, nm2);
-    const float2 p0 = make_float2(fast_exp2(y0.x), fast_exp2(y0.y));
-    const float2 p1 = make_float2(fast_exp2(y1.x), fast_exp2(y1.y));
-    sum = fadd2(sum, fadd2(p0, p1));
-    float2 w0 = fmul2(p0, make_float2(v4.x, v4.y)), w1 = fmul2(p1, make_float2(v4.z, v4.w));
-    if constexpr (MASKED) {
-      w0.x = x[c] == -INFINITY ? 0.f : w0.x;
-      w0.y = x[c + 1] == -INFINITY ? 0.f : w0.y;
-      w1.x = x[c + 2] == -INFINITY ? 0.f : w1.x;
-      w1.y = x[c + 3] == -INFINITY ? 0.f : w1.y;
-    }
-    pk[c / 2] = pack_h2(w0.x, w0.y);
-    pk[c / 2 + 1] = pack_h2(w1.x, w1.y);
-  }
-}
-
-// The weights of a step's 64 tokens (scores at tensor-memory column ts), its
-// loads one ahead.
-template <bool MASKED>
-__device__ __forceinline__ void step_weights(uint32_t ts, const float4* ks4, const float4* vs4, int t,
+__device__ __forceinline__ void tile_weights(uint32_t ts, const float4* ks4, const float4* vs4, int t,
                                              int pmin, int plim, float2 ra2, float nm, float2& sum,
                                              uint32_t (&pk)[32]) {
   const float2 nm2 = make_float2(nm, nm);
   float x[2][16];
-  umma::ld16(ts, x[0]);
+  float2 s1 = make_float2(0.f, 0.f);
+  ld16_issue(ts, x[0]);
+  wait_ld_of(x[0]);
+  ld16_issue(ts + 16, x[1]);
+  scale_scores<MASKED>(x[0], ks4, t, pmin, plim);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    wait_ld_of(x[q & 1]);
-    if (q < 3) umma::ld16(ts + 16 * (q + 1), x[(q + 1) & 1]);
-    scale_scores<MASKED>(x[q & 1], ks4 + 4 * q, t + 16 * q, pmin, plim);
-    score_weights<MASKED>(x[q & 1], vs4 + 4 * q, ra2, nm2, sum, &pk[8 * q]);
+    float(&y)[16] = x[q & 1];
+    float2 w[8];
+#pragma unroll
+    for (int c = 0; c < 16; c += 2) {
+      const float2 e = ffma2(make_float2(y[c], y[c + 1]), ra2, nm2);
+      w[c / 2] = make_float2(fast_exp2(e.x), fast_exp2(e.y));
+    }
+    if (q < 3) {
+      wait_ld_of(x[(q + 1) & 1]);
+      scale_scores<MASKED>(x[(q + 1) & 1], ks4 + 4 * (q + 1), t + 16 * (q + 1), pmin, plim);
+    }
+#pragma unroll
+    for (int c = 0; c < 16; c += 4) {
+      const float4 v4 = vs4[4 * q + c / 4];
+      sum = fadd2(sum, w[c / 2]);
+      s1 = fadd2(s1, w[c / 2 + 1]);
+      float2 w0 = fmul2(w[c / 2], make_float2(v4.x, v4.y));
+      float2 w1 = fmul2(w[c / 2 + 1], make_float2(v4.z, v4.w));
+      if constexpr (MASKED) {
+        w0.x = y[c] == -INFINITY ? 0.f : w0.x;
+        w0.y = y[c + 1] == -INFINITY ? 0.f : w0.y;
+        w1.x = y[c + 2] == -INFINITY ? 0.f : w1.x;
+        w1.y = y[c + 3] == -INFINITY ? 0.f : w1.y;
+      }
+      pk[8 * q + c / 2] = pack_h2(w0.x, w0.y);
+      pk[8 * q + c / 2 + 1] = pack_h2(w1.x, w1.y);
+    }
+    if (q < 2) ld16_issue(ts + 16 * (q + 2), y);
   }
+  sum = fadd2(sum, s1);
+}
+
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N));
 }
 
 template <int D>
 struct Sm {
   static constexpr int Q_BYTES = kRows * D * 2, K_BYTES = kTN * D * 2, V_BYTES = D * kTN * 2;
   static constexpr int Q_OFF = 0;                      // one operand per warpgroup
-  static constexpr int K_OFF = Q_OFF + 2 * Q_BYTES;    // two buffers
-  static constexpr int V_OFF = K_OFF + 2 * K_BYTES;    // two buffers
-  static constexpr int KS_OFF = V_OFF + 2 * V_BYTES;   // [3][128] f32 key scales
-  static constexpr int VS_OFF = KS_OFF + 3 * kTN * 4;  // [3][128] value scales 2^-E 2^5
-  static constexpr int VI_OFF = VS_OFF + 3 * kTN * 4;  // [3] 2^-E of the tile
+  static constexpr int K_OFF = Q_OFF + 2 * Q_BYTES;
+  static constexpr int V_OFF = K_OFF + kStages * K_BYTES;
+  static constexpr int KS_OFF = V_OFF + kStages * V_BYTES;   // [stage][64] f32 key scales
+  static constexpr int VS_OFF = KS_OFF + kStages * kTN * 4;  // [stage][64] value scales 2^-E 2^5
+  static constexpr int VI_OFF = VS_OFF + kStages * kTN * 4;  // [stage] 2^-E of the tile
   static constexpr int BAR_OFF = VI_OFF + 32;
   static constexpr int BYTES = BAR_OFF + 256;
   static_assert(BYTES <= 227 * 1024, "one CTA's shared memory");
@@ -191,25 +220,26 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   constexpr int UNITS = kPage * D / 16;           // 16-byte units of a page's K (or V) codes
   constexpr int UPT = kTP * UNITS / kProducers;   // units per producer thread and tile
   constexpr int PSTEP = kProducers / UNITS;       // pages covered by one unit of every thread
+  static_assert(8 * kTP == 32, "a window of page ids is a lane each");
   extern __shared__ __align__(1024) uint8_t smem[];
-  // Barriers (tile j counted from the CTA's first; b = j % 2):
-  //   kready[b], vready[b]  operands stored (128 producer arrivals)
-  //   kfree[b], vfree[b]    S, O += P V of tile j done (a commit per warpgroup)
-  //   sready[j % 3]         scales stored (32 arrivals)
-  // and of warpgroup w, step i (two a tile), in turn for even and odd steps:
-  //   sdone[w][i % 2]       S done (commit)
-  //   pready[w][i % 2]      P written (128 arrivals)
-  //   odone[w][i % 2]       O += P V done (commit)
+  // Barriers (tile i counted from the CTA's first), of stage i % 4:
+  //   kready          K stored (128 producer arrivals)
+  //   vready          V and the scales stored (128 producer arrivals)
+  //   kfree, vfree    S, O += P V of the tile done (a commit per warpgroup)
+  // and of warpgroup w, [2 w + i % 2]:
+  //   sdone           S done (commit)
+  //   pready          P written (128 arrivals)
+  //   odone           O += P V done (commit)
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + SM::BAR_OFF);
   uint64_t* const kready = bars;
-  uint64_t* const vready = bars + 2;
-  uint64_t* const kfree = bars + 4;
-  uint64_t* const vfree = bars + 6;
-  uint64_t* const sready = bars + 8;
-  uint64_t* const sdone = bars + 11;   // [2 w + i % 2]
-  uint64_t* const pready = bars + 15;  // [2 w + i % 2]
-  uint64_t* const odone = bars + 19;   // [2 w + i % 2]
-  uint32_t* const tslot = reinterpret_cast<uint32_t*>(bars + 23);
+  uint64_t* const vready = bars + kStages;
+  uint64_t* const kfree = bars + 2 * kStages;
+  uint64_t* const vfree = bars + 3 * kStages;
+  uint64_t* const sdone = bars + 4 * kStages;
+  uint64_t* const pready = sdone + 4;
+  uint64_t* const odone = pready + 4;
+  uint32_t* const tslot = reinterpret_cast<uint32_t*>(odone + 4);
+  static_assert((4 * kStages + 12) * 8 + 4 <= 256, "the barriers fit their area");
   float* const ks_s = reinterpret_cast<float*>(smem + SM::KS_OFF);
   float* const vs_s = reinterpret_cast<float*>(smem + SM::VS_OFF);
   float* const vi_s = reinterpret_cast<float*>(smem + SM::VI_OFF);
@@ -236,12 +266,17 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
 
   if (warp == 0) umma::alloc(tslot, SM::TCOLS);
   if (ctid == 0) {
-    for (int i = 0; i < 4; ++i) mbar_init(&bars[i], kProducers);      // kready, vready
-    for (int i = 4; i < 8; ++i) mbar_init(&bars[i], wgs);             // kfree, vfree
-    for (int i = 8; i < 11; ++i) mbar_init(&bars[i], 32);             // sready
-    for (int i = 11; i < 15; ++i) mbar_init(&bars[i], 1);             // sdone
-    for (int i = 15; i < 19; ++i) mbar_init(&bars[i], kRows);         // pready
-    for (int i = 19; i < 23; ++i) mbar_init(&bars[i], 1);             // odone
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&kready[i], kProducers);
+      mbar_init(&vready[i], kProducers);
+      mbar_init(&kfree[i], wgs);
+      mbar_init(&vfree[i], wgs);
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(&sdone[i], 1);
+      mbar_init(&pready[i], kRows);
+      mbar_init(&odone[i], 1);
+    }
     fence_mbar_init();
   }
 
@@ -290,26 +325,32 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   __syncthreads();
   umma::fence_after_sync();
   const uint32_t tmem = *tslot;
-  constexpr uint32_t idS = umma::idesc_f16(kRows, kStep, false);
+  constexpr uint32_t idS = umma::idesc_f16(kRows, kTN, false);
   constexpr uint32_t idO = umma::idesc_f16(kRows, D, false);
 
   if (ctid >= kSoftmax && ctid < kSoftmax + kProducers) {
     // ============================ producers ============================
+    regs_down<kRegsProducer>();
     const int tid = ctid - kSoftmax;
-    const bool scales = tid < 32;  // this warp brings the scales: lane l tokens 4 l ..
+    const bool scales = tid < 32;  // this warp brings the scales: lane l tokens 2 l, 2 l + 1
     const int32_t* bt = a.block_tables + static_cast<int64_t>(s) * a.max_blocks;
     const int n_pages = (kv_end + kPage - 1) / kPage;
     const uint8_t* const pool_h = a.pool + static_cast<int64_t>(h) * F::BYTES;
     const int64_t page_stride = static_cast<int64_t>(a.n_kv_heads) * F::BYTES;
     const int first_page = kv_lo / kPage;  // the table may have dropped what the window passed
-    auto page_at = [&](int p) {  // page p of the sequence, checked; 0 outside the seen pages
-      int id = p >= first_page && p < n_pages ? __ldg(bt + p) : 0;
-      if (id < 0 || id >= a.num_pages) {
-        set_err(a.err, TKV_ERR_BAD_PAGE);
-        id = 0;  // read in bounds; the sequence's output is not meaningful
-      }
-      return id;
+    // lane l holds the id of page 32 w + l of the run (window w: 8 tiles), checked
+    // against the pool, and of the next window as loaded: no load of codes waits
+    // for a load of the table
+    auto load_ids = [&](int w) {
+      const int p = j_lo * kTP + 32 * w + lane;
+      return p >= first_page && p < n_pages ? __ldg(bt + p) : 0;
     };
+    auto checked = [&](int id) {
+      if (id >= 0 && id < a.num_pages) return id;
+      set_err(a.err, TKV_ERR_BAD_PAGE);
+      return 0;  // read in bounds; the sequence's output is not meaningful
+    };
+    int ids = checked(load_ids(0)), ids_next = load_ids(1);
     // K unit of this thread in page PSTEP i + tid / UNITS: slot x % 16 of chunk
     // x / 16 (x = tid % UNITS): 8 lanes read 128 bytes and fill one core matrix.
     const int x = tid % UNITS, pg0 = tid / UNITS;
@@ -321,130 +362,125 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     const uint32_t v_src = F::V_OFF + int8_v_unit(vu, vg, vt);
     const uint32_t v_dst = 4 * vu * (16 * kTN) + (vt >> 1) * 128 + vg * 16 + (vt & 1) * 8;
     int pid[UPT], spid = 0;
-    uint4 kr[UPT], vr[UPT], sr0 = make_uint4(0, 0, 0, 0), sr1 = sr0;
-    auto fetch_ids = [&](int j) {
+    uint4 kr[UPT], vr[UPT];
+    float4 sr = make_float4(0.f, 0.f, 0.f, 0.f);  // key, value scale of two tokens
+    auto fetch_ids = [&](int i) {  // the pages of tile i of the run, in order of i
+      if (i > 0 && (i & 7) == 0) {
+        ids = checked(ids_next);
+        ids_next = load_ids((i >> 3) + 1);
+      }
 #pragma unroll
-      for (int i = 0; i < UPT; ++i) pid[i] = page_at(j * kTP + PSTEP * i + pg0);
-      if (scales) spid = page_at(j * kTP + (lane >> 2));
+      for (int k = 0; k < UPT; ++k)
+        pid[k] = __shfl_sync(0xffffffffu, ids, (i & 7) * kTP + PSTEP * k + pg0);
+      if (scales) spid = __shfl_sync(0xffffffffu, ids, (i & 7) * kTP + (lane >> 3));
     };
     auto load_k = [&]() {
 #pragma unroll
       for (int i = 0; i < UPT; ++i)
         kr[i] = __ldg(reinterpret_cast<const uint4*>(pool_h + pid[i] * page_stride) + x);
-      if (scales) {
-        const uint4* p = reinterpret_cast<const uint4*>(pool_h + spid * page_stride + F::SCALE_OFF) +
-                         2 * (lane & 3);
-        sr0 = __ldg(p);
-        sr1 = __ldg(p + 1);
-      }
     };
     auto load_v = [&]() {
 #pragma unroll
       for (int i = 0; i < UPT; ++i)
         vr[i] = __ldg(reinterpret_cast<const uint4*>(pool_h + pid[i] * page_stride + v_src));
+      if (scales)
+        sr = __ldg(reinterpret_cast<const float4*>(pool_h + spid * page_stride + F::SCALE_OFF) + (lane & 7));
     };
     float vinv = 0x1p126f;  // 2^-E
     if (nj > 0) {
-      fetch_ids(j_lo);
+      fetch_ids(0);
       load_k();
       load_v();
     }
-    for (int j = 0; j < nj; ++j) {
-      const int b = j & 1, ph = (j >> 1) & 1;
-      const bool more = j + 1 < nj;
-      if (more) fetch_ids(j_lo + j + 1);
-      if (j >= 2 && !mbar_wait_near(&kfree[b], ph ^ 1, a.err)) break;
-      if (scales) {
-        const float kv[8] = {__uint_as_float(sr0.x), __uint_as_float(sr0.y), __uint_as_float(sr0.z),
-                             __uint_as_float(sr0.w), __uint_as_float(sr1.x), __uint_as_float(sr1.y),
-                             __uint_as_float(sr1.z), __uint_as_float(sr1.w)};
-        const int t0 = (j_lo + j) * kTN + 4 * lane;
-        float v[4], top = 0.f;
+    for (int i = 0; i < nj; ++i) {
+      const int st = i % kStages;
+      const uint32_t before = ((i / kStages) & 1) ^ 1;  // parity of the stage's last use
+      const bool more = i + 1 < nj;
+      if (more) fetch_ids(i + 1);
+      if (i >= kStages && !mbar_wait_near(&kfree[st], before, a.err)) break;
+      uint8_t* const kd = smem + SM::K_OFF + st * SM::K_BYTES + k_dst;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {  // tokens that no row of the CTA sees count for nothing
-          v[e] = t0 + e < kv_end && t0 + e >= kv_lo ? kv[2 * e + 1] : 0.f;
-          top = fmaxf(top, v[e]);
-        }
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        if (top * vinv > 1.f) vinv = int8_scale_inverse(top);
-        const int buf = j % 3;
-        *reinterpret_cast<float4*>(ks_s + buf * kTN + 4 * lane) = make_float4(kv[0], kv[2], kv[4], kv[6]);
-        *reinterpret_cast<float4*>(vs_s + buf * kTN + 4 * lane) =
-            make_float4(v[0] * vinv * kInt8WeightUp, v[1] * vinv * kInt8WeightUp,
-                        v[2] * vinv * kInt8WeightUp, v[3] * vinv * kInt8WeightUp);
-        if (lane == 0) vi_s[buf] = vinv;
-        mbar_arrive(&sready[buf]);
-      }
-      uint8_t* const kd = smem + SM::K_OFF + b * SM::K_BYTES + k_dst;
-#pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-        const uint32_t w[4] = {kr[i].x, kr[i].y, kr[i].z, kr[i].w};
+      for (int k = 0; k < UPT; ++k) {
+        const uint32_t w[4] = {kr[k].x, kr[k].y, kr[k].z, kr[k].w};
         uint32_t hv[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) int8_to_h2(w[e], hv[2 * e], hv[2 * e + 1]);
-        uint8_t* d = kd + (PSTEP * i + pg0) * (32 * D);
+        uint8_t* d = kd + (PSTEP * k + pg0) * (32 * D);
         *reinterpret_cast<uint4*>(d) = make_uint4(hv[0], hv[1], hv[2], hv[3]);
         *reinterpret_cast<uint4*>(d + 128) = make_uint4(hv[4], hv[5], hv[6], hv[7]);
       }
       umma::fence_smem_to_async();
-      mbar_arrive(&kready[b]);
+      mbar_arrive(&kready[st]);
       if (more) load_k();
-      if (j >= 2 && !mbar_wait_near(&vfree[b], ph ^ 1, a.err)) break;
-      uint8_t* const vd = smem + SM::V_OFF + b * SM::V_BYTES + v_dst;
+      if (i >= kStages && !mbar_wait_near(&vfree[st], before, a.err)) break;
+      uint8_t* const vd = smem + SM::V_OFF + st * SM::V_BYTES + v_dst;
 #pragma unroll
-      for (int i = 0; i < UPT; ++i) {
-        const uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+      for (int k = 0; k < UPT; ++k) {
+        const uint32_t w[4] = {vr[k].x, vr[k].y, vr[k].z, vr[k].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           uint32_t lo, hi;
           int8_to_h2(w[e], lo, hi);
-          *reinterpret_cast<uint2*>(vd + e * (16 * kTN) + (PSTEP * i + pg0) * 256) = make_uint2(lo, hi);
+          *reinterpret_cast<uint2*>(vd + e * (16 * kTN) + (PSTEP * k + pg0) * 256) = make_uint2(lo, hi);
         }
       }
+      if (scales) {
+        // tokens that no row of the CTA sees count for nothing
+        const int t0 = (j_lo + i) * kTN + 2 * lane;
+        const float v0 = t0 < kv_end && t0 >= kv_lo ? sr.y : 0.f;
+        const float v1 = t0 + 1 < kv_end && t0 + 1 >= kv_lo ? sr.w : 0.f;
+        float top = fmaxf(fmaxf(v0, v1), 0.f);
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        if (top * vinv > 1.f) vinv = int8_scale_inverse(top);
+        *reinterpret_cast<float2*>(ks_s + st * kTN + 2 * lane) = make_float2(sr.x, sr.z);
+        *reinterpret_cast<float2*>(vs_s + st * kTN + 2 * lane) =
+            make_float2(v0 * vinv * kInt8WeightUp, v1 * vinv * kInt8WeightUp);
+        if (lane == 0) vi_s[st] = vinv;
+      }
       umma::fence_smem_to_async();
-      mbar_arrive(&vready[b]);
+      mbar_arrive(&vready[st]);
       if (more) load_v();
     }
   } else if (ctid >= kSoftmax + kProducers) {
     // ============================ an MMA warp ============================
+    regs_down<kRegsMma>();
     const int w = warp - (kSoftmax + kProducers) / 32;  // its softmax warpgroup
     if (lane == 0 && w < wgs && nj > 0) {
-      const int steps = 2 * nj;
       bool ok = true;
       int last_s = -1, last_o = -1;
       const uint64_t dq = umma::smem_desc(smem_u32(smem + SM::Q_OFF + w * SM::Q_BYTES), 128, 16 * D);
       const uint64_t dk = umma::smem_desc(smem_u32(smem + SM::K_OFF), 128, 16 * D);
       const uint64_t dv = umma::smem_desc(smem_u32(smem + SM::V_OFF), 128, 16 * kTN);
       const uint32_t tS = tmem + w * SM::TWG, tO = tS + SM::TO;
-      auto issue_s = [&](int i) {  // step i: tokens 64 (i % 2) .. of K buffer (i / 2) % 2
-        if ((i & 1) == 0) ok = mbar_wait_near(&kready[(i >> 1) & 1], (i >> 2) & 1, a.err);
+      auto issue_s = [&](int i) {
+        ok = mbar_wait_near(&kready[i % kStages], (i / kStages) & 1, a.err);
         if (!ok) return;
         umma::fence_after_sync();
-        const uint64_t d = dk + ((i >> 1) & 1) * (SM::K_BYTES >> 4) + (i & 1) * (SM::K_BYTES >> 5);
+        const uint64_t d = dk + (i % kStages) * (SM::K_BYTES >> 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          umma::mma_f16(tS + (i & 1) * kStep, dq + 16 * kk, d + 16 * kk, idS, kk > 0);
+          umma::mma_f16(tS + (i & 1) * kTN, dq + 16 * kk, d + 16 * kk, idS, kk > 0);
         umma::commit(&sdone[2 * w + (i & 1)]);
-        if (i & 1) umma::commit(&kfree[(i >> 1) & 1]);
+        umma::commit(&kfree[i % kStages]);
         last_s = i;
       };
       issue_s(0);
-      if (ok) issue_s(1);
-      for (int i = 0; ok && i < steps; ++i) {
-        if ((i & 1) == 0) ok = mbar_wait_near(&vready[(i >> 1) & 1], (i >> 2) & 1, a.err);
-        ok = ok && mbar_wait_near(&pready[2 * w + (i & 1)], (i >> 1) & 1, a.err);
+      if (ok && nj > 1) issue_s(1);
+      for (int i = 0; ok && i < nj; ++i) {
+        ok = mbar_wait_near(&vready[i % kStages], (i / kStages) & 1, a.err) &&
+             mbar_wait_near(&pready[2 * w + (i & 1)], (i >> 1) & 1, a.err);
         if (!ok) break;
         umma::fence_after_sync();
-        const uint64_t d = dv + ((i >> 1) & 1) * (SM::V_BYTES >> 4) + (i & 1) * (16 * kStep / 16);
+        const uint64_t d = dv + (i % kStages) * (SM::V_BYTES >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kStep / 16; ++kk)
-          umma::mma_f16_ta(tO, tS + (i & 1) * kStep + 8 * kk, d + 16 * kk, idO, i > 0 || kk > 0);
+        for (int kk = 0; kk < kTN / 16; ++kk)
+          umma::mma_f16_ta(tO, tS + (i & 1) * kTN + 8 * kk, d + 16 * kk, idO, i > 0 || kk > 0);
         umma::commit(&odone[2 * w + (i & 1)]);
-        if (i & 1) umma::commit(&vfree[(i >> 1) & 1]);
+        umma::commit(&vfree[i % kStages]);
         last_o = i;
-        if (i + 2 < steps) {
-          // S of step i + 2 overwrites the scores and weights of this one
+        if (i + 2 < nj) {
+          // S of tile i + 2 overwrites the scores and weights of this one
           ok = mbar_wait_near(&odone[2 * w + (i & 1)], (i >> 1) & 1, a.err);
           if (ok) issue_s(i + 2);
         }
@@ -455,8 +491,10 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       for (int i = max(0, last_o - 1); i <= last_o; ++i)
         mbar_wait_near(&odone[2 * w + (i & 1)], (i >> 1) & 1, nullptr);
     }
-  } else if (wg < wgs) {
+  } else {
     // ============================ softmax ============================
+    regs_up<kRegsSoftmax>();
+    if (wg < wgs) {
     const uint32_t lane_base = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t tS = tmem + wg * SM::TWG + lane_base, tO = tS + SM::TO;
     const int plim = valid ? L - n + qi : -1;  // last position that the row sees
@@ -464,23 +502,23 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     float m = -INFINITY, l = 0.f, vinv = 0x1p126f;
     bool ok = true;
     const float2 ra2 = make_float2(ra, ra);
-    for (int i = 0; i < 2 * nj; ++i) {
-      const int j = i >> 1, buf = j % 3, t0 = (j_lo + j) * kTN + (i & 1) * kStep;
-      ok = ((i & 1) || mbar_wait_near(&sready[buf], (j / 3) & 1, a.err)) &&
-           mbar_wait_near(&sdone[2 * wg + (i & 1)], j & 1, a.err);
+    for (int i = 0; i < nj; ++i) {
+      const int st = i % kStages, t0 = (j_lo + i) * kTN;
+      ok = mbar_wait_near(&vready[st], (i / kStages) & 1, a.err) &&
+           mbar_wait_near(&sdone[2 * wg + (i & 1)], (i >> 1) & 1, a.err);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       umma::fence_after_sync();
-      bool masked = __any_sync(0xffffffffu, t0 + kStep - 1 > plim || t0 < pmin);
-      const float vnew = vi_s[buf];
+      bool masked = __any_sync(0xffffffffu, t0 + kTN - 1 > plim || t0 < pmin);
+      const float vnew = vi_s[st];
       float fv = 1.f;
       if (vnew != vinv) {
         fv = vnew / vinv;
         vinv = vnew;
       }
-      const uint32_t tSi = tS + (i & 1) * kStep;
-      const float4* ks4 = reinterpret_cast<const float4*>(ks_s + buf * kTN + (i & 1) * kStep);
-      const float4* vs4 = reinterpret_cast<const float4*>(vs_s + buf * kTN + (i & 1) * kStep);
+      const uint32_t tSi = tS + (i & 1) * kTN;
+      const float4* ks4 = reinterpret_cast<const float4*>(ks_s + st * kTN);
+      const float4* vs4 = reinterpret_cast<const float4*>(vs_s + st * kTN);
       float2 sum;
       uint32_t pk[32];
       // A pass with the reference as it is: no maximum is taken.  A sum of
@@ -490,13 +528,13 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         sum = make_float2(0.f, 0.f);
         const float nm = m == -INFINITY ? 0.f : -m;
         if (masked)
-          step_weights<true>(tSi, ks4, vs4, t0, pmin, plim, ra2, nm, sum, pk);
+          tile_weights<true>(tSi, ks4, vs4, t0, pmin, plim, ra2, nm, sum, pk);
         else
-          step_weights<false>(tSi, ks4, vs4, t0, pmin, plim, ra2, nm, sum, pk);
+          tile_weights<false>(tSi, ks4, vs4, t0, pmin, plim, ra2, nm, sum, pk);
         if (pass || !__any_sync(0xffffffffu, sum.x + sum.y > kInt8LazyWeight || m == -INFINITY || fv != 1.f))
           break;
         // The reference has to move (or the value scales' power of two has): the
-        // step's maximum, O and l brought to the new reference, and the weights
+        // tile's maximum, O and l brought to the new reference, and the weights
         // again (the scores are still in tensor memory).
         float mx = -INFINITY;
 #pragma unroll 1
@@ -512,7 +550,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         const float f = up ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
         m = up ? mx : m;
         l *= f;
-        if (i > 0) {  // O holds the steps before, once the last one's products are in
+        if (i > 0) {  // O holds the tiles before, once the last one's products are in
           ok = __all_sync(0xffffffffu,
                           mbar_wait_near(&odone[2 * wg + ((i - 1) & 1)], ((i - 1) >> 1) & 1, a.err));
           if (!ok) break;
@@ -535,7 +573,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       umma::fence_before_sync();
       mbar_arrive(&pready[2 * wg + (i & 1)]);
     }
-    if (ok && nj > 0) ok = mbar_wait_near(&odone[2 * wg + 1], (nj - 1) & 1, a.err);
+    if (ok && nj > 0)
+      ok = mbar_wait_near(&odone[2 * wg + ((nj - 1) & 1)], ((nj - 1) >> 1) & 1, a.err);
     ok = __all_sync(0xffffffffu, ok);
     umma::fence_after_sync();
     // ---- normalise and write the row (a run's partial when the context is split) ----
@@ -579,6 +618,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         }
       }
       if (sp.n > 1 && valid) *reinterpret_cast<float2*>(sp.part_ml + slot * 2) = make_float2(m, l);
+    }
     }
   }
   umma::fence_before_sync();
