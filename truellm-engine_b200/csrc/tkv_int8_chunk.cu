@@ -494,12 +494,19 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   } else {
     // ============================ softmax ============================
     regs_up<kRegsSoftmax>();
-    if (wg < wgs) {
+    if (wg < wgs && kRows * wg + 32 * (warp & 3) >= rows) {
+      // no row of this warp exists: it only keeps the hand-overs going
+      for (int i = 0; i < nj; ++i) {
+        if (!mbar_wait_near(&sdone[2 * wg + (i & 1)], (i >> 1) & 1, a.err)) break;
+        mbar_arrive(&pready[2 * wg + (i & 1)]);
+      }
+    } else if (wg < wgs) {
     const uint32_t lane_base = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t tS = tmem + wg * SM::TWG + lane_base, tO = tS + SM::TO;
     const int plim = valid ? L - n + qi : -1;  // last position that the row sees
     const int pmin = a.window > 0 ? max(0, plim - a.window + 1) : 0;
-    float m = -INFINITY, l = 0.f, vinv = 0x1p126f;
+    // a row that does not exist sees nothing and has no reference to move
+    float m = valid ? -INFINITY : 0.f, l = 0.f, vinv = 0x1p126f;
     bool ok = true;
     const float2 ra2 = make_float2(ra, ra);
     for (int i = 0; i < nj; ++i) {
@@ -509,7 +516,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       umma::fence_after_sync();
-      bool masked = __any_sync(0xffffffffu, t0 + kTN - 1 > plim || t0 < pmin);
+      bool masked = __any_sync(0xffffffffu, valid && (t0 + kTN - 1 > plim || t0 < pmin));
       const float vnew = vi_s[st];
       float fv = 1.f;
       if (vnew != vinv) {
