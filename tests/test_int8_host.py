@@ -156,6 +156,7 @@ def test_workspace_sizes():
     ws = lib.tkv_int8_attend_workspace_bytes
     assert ws(2, 7, 2, 128, 1, 64) == ws(-1, 8, 2, 128, 1, 64) == ws(2, 8, 2, 96, 1, 64) == 0
     assert ws(2, 8, 2, 128, 1, -1) == ws(2, 8, 2, 128, 1, 2 ** 31 - 1) == 0
+    assert ws(2, 8, 2, 128, 2 ** 28, 64) == 0  # 2^30 query rows of a kv head
     # serving sizes stay small beside a cache
     assert 0 < ws(64, 32, 8, 128, 1, 8192) < 64 << 20
     assert 0 < ws(1, 64, 8, 128, 1, 1 << 20) < 64 << 20

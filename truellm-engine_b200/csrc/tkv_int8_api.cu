@@ -167,7 +167,8 @@ static bool attend_sizes_ok(int num_seqs, int num_q_heads, int num_kv_heads, int
                             int max_q_tokens, int max_context_len) {
   return num_seqs >= 0 && num_seqs <= 65535 && num_q_heads > 0 && num_kv_heads > 0 &&
          num_q_heads % num_kv_heads == 0 && (head_dim == 64 || head_dim == 128) &&
-         max_q_tokens >= 0 && max_context_len >= 0 && max_context_len <= INT_MAX - 1024;
+         max_q_tokens >= 0 && max_context_len >= 0 && max_context_len <= INT_MAX - 1024 &&
+         static_cast<long long>(max_q_tokens) * (num_q_heads / num_kv_heads) < 1ll << 30;
 }
 
 size_t tkv_int8_attend_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads,

@@ -86,20 +86,6 @@ __device__ __forceinline__ void wait_ld_of(float (&v)[16]) {
 
 // n consecutive 32-bit columns of this thread's lane; load and wait are one
 // statement, so nothing can use a value before it has arrived
-__device__ __forceinline__ void ld32_wait(uint32_t taddr, float (&v)[32]) {
-  asm volatile(
-      "{\n\ttcgen05.ld.sync.aligned.32x32b.x32.b32 {"
-      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
-      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31 "
-      "}, [%32];\n\ttcgen05.wait::ld.sync.aligned;\n\t}\n"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
-        "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
-        "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]), "=f"(v[19]),
-        "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]),
-        "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
-      : "r"(taddr)
-      : "memory");
-}
 __device__ __forceinline__ void ld16_wait(uint32_t taddr, float (&v)[16]) {
   asm volatile(
       "{\n\ttcgen05.ld.sync.aligned.32x32b.x16.b32 {"
@@ -108,6 +94,21 @@ __device__ __forceinline__ void ld16_wait(uint32_t taddr, float (&v)[16]) {
       : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
         "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
         "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// 32 columns in the layout of an MMA accumulator fragment: 16 lanes (rows), lane l of
+// the warp holding row l / 4 and columns 2 (l % 4), + 1 of every 8-column group (v[4
+// g], v[4 g + 1]), and the same of row l / 4 + 8 (v[4 g + 2], v[4 g + 3])
+__device__ __forceinline__ void ld_frag32(uint32_t taddr, float (&v)[16]) {
+  asm volatile(
+      "{\n\ttcgen05.ld.sync.aligned.16x256b.x4.b32 {"
+      "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15 "
+      "}, [%16];\n\ttcgen05.wait::ld.sync.aligned;\n\t}\n"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+        "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]),
+        "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
       : "r"(taddr)
       : "memory");
 }
@@ -205,7 +206,8 @@ struct Sm {
   static constexpr int KS_OFF = V_OFF + kStages * V_BYTES;   // [stage][64] f32 key scales
   static constexpr int VS_OFF = KS_OFF + kStages * kTN * 4;  // [stage][64] value scales 2^-E 2^5
   static constexpr int VI_OFF = VS_OFF + kStages * kTN * 4;  // [stage] 2^-E of the tile
-  static constexpr int BAR_OFF = VI_OFF + 32;
+  static constexpr int ROW_OFF = VI_OFF + 32;                // [256] f32 of the rows
+  static constexpr int BAR_OFF = ROW_OFF + kSoftmax * 4;
   static constexpr int BYTES = BAR_OFF + 256;
   static_assert(BYTES <= 227 * 1024, "one CTA's shared memory");
   static_assert(BYTES <= (1 << 18), "descriptor address fields never carry");
@@ -230,6 +232,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   //   sdone           S done (commit)
   //   pready          P written (128 arrivals)
   //   odone           O += P V done (commit)
+  // and qready: the Q operands staged (256 arrivals).
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + SM::BAR_OFF);
   uint64_t* const kready = bars;
   uint64_t* const vready = bars + kStages;
@@ -238,11 +241,13 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   uint64_t* const sdone = bars + 4 * kStages;
   uint64_t* const pready = sdone + 4;
   uint64_t* const odone = pready + 4;
-  uint32_t* const tslot = reinterpret_cast<uint32_t*>(odone + 4);
-  static_assert((4 * kStages + 12) * 8 + 4 <= 256, "the barriers fit their area");
+  uint64_t* const qready = odone + 4;
+  uint32_t* const tslot = reinterpret_cast<uint32_t*>(qready + 1);
+  static_assert((4 * kStages + 13) * 8 + 4 <= 256, "the barriers fit their area");
   float* const ks_s = reinterpret_cast<float*>(smem + SM::KS_OFF);
   float* const vs_s = reinterpret_cast<float*>(smem + SM::VS_OFF);
   float* const vi_s = reinterpret_cast<float*>(smem + SM::VI_OFF);
+  float* const row_s = reinterpret_cast<float*>(smem + SM::ROW_OFF);
 
   const int ctid = threadIdx.x, warp = ctid >> 5, lane = ctid & 31;
   const int split = blockIdx.x % sp.n;
@@ -251,18 +256,18 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   const int bh = rest / sp.row_tiles, s = bh / a.n_kv_heads, h = bh - s * a.n_kv_heads;
   const int L = __ldg(a.seq_lens + s), q0 = __ldg(a.cu_q + s), n = __ldg(a.cu_q + s + 1) - q0;
   if (!int8_attend_ok(a, L, q0, n)) return;  // flagged by the decode kernel
-  const long long rows_l = static_cast<long long>(n) * a.grp;
-  const long long r0 = static_cast<long long>(rt) * kSoftmax;
-  if (rows_l <= kInt8DecodeRows || r0 >= rows_l) return;
-  const int rows = static_cast<int>(min(rows_l - r0, static_cast<long long>(kSoftmax)));
+  // rows of a (sequence, kv head) are below 2^30 (checked on the host)
+  const uint32_t grp = a.grp, all_rows = static_cast<uint32_t>(n) * grp, r0 = rt * kSoftmax;
+  if (all_rows <= kInt8DecodeRows || r0 >= all_rows) return;
+  const int rows = min(all_rows - r0, static_cast<uint32_t>(kSoftmax));
   const int wgs = rows > kRows ? 2 : 1;
   // tiles that some row of this CTA sees, cut into sp.n runs
-  const int p_first = L - n + static_cast<int>(r0 / a.grp);
-  const int kv_end = L - n + static_cast<int>((r0 + rows - 1) / a.grp) + 1;
+  const int p_first = L - n + static_cast<int>(r0 / grp);
+  const int kv_end = L - n + static_cast<int>((r0 + rows - 1) / grp) + 1;
   const int kv_lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
   const int tile0 = kv_lo / kTN, tiles = (kv_end + kTN - 1) / kTN - tile0;
-  const int j_lo = tile0 + static_cast<int>(static_cast<long long>(tiles) * split / sp.n);
-  const int nj = tile0 + static_cast<int>(static_cast<long long>(tiles) * (split + 1) / sp.n) - j_lo;
+  const int per = tiles / sp.n, more = tiles - per * sp.n;  // the first `more` runs have one more
+  const int j_lo = tile0 + split * per + min(split, more), nj = per + (split < more ? 1 : 0);
 
   if (warp == 0) umma::alloc(tslot, SM::TCOLS);
   if (ctid == 0) {
@@ -277,50 +282,10 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       mbar_init(&pready[i], kRows);
       mbar_init(&odone[i], 1);
     }
+    mbar_init(qready, kSoftmax);
     fence_mbar_init();
   }
 
-  // ---- the Q operands: softmax thread ctid stages its row ----
-  const bool softmax = ctid < kSoftmax;
-  const int wg = ctid >> 7, wt = ctid & 127;
-  const bool valid = softmax && ctid < rows;
-  const int qi = valid ? static_cast<int>((r0 + ctid) / a.grp) : 0;
-  const int hq = h * a.grp + (valid ? static_cast<int>((r0 + ctid) % a.grp) : 0);
-  float ra = a.alpha;  // 2^e * scale * log2(e) of this row
-  if (softmax) {
-    const uint4* src = reinterpret_cast<const uint4*>(a.q + (q0 + qi) * a.q_t + hq * a.q_h);
-    float up = 1.f, down = 1.f;
-    if (a.q_bf16 && valid) {
-      float m = 0.f;
-#pragma unroll 4
-      for (int c = 0; c < D / 8; ++c) {
-        const uint4 x = __ldg(src + c);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = unpack2<true>(w[e]);
-          m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
-      }
-      int8_row_power(m, up, down);
-    }
-    ra *= up;
-#pragma unroll 4
-    for (int c = 0; c < D / 8; ++c) {
-      uint4 x = valid ? __ldg(src + c) : make_uint4(0, 0, 0, 0);
-      if (a.q_bf16) {
-        uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = unpack2<true>(w[e]);
-          w[e] = pack_h2(f.x * down, f.y * down);
-        }
-        x = make_uint4(w[0], w[1], w[2], w[3]);
-      }
-      *reinterpret_cast<uint4*>(smem + SM::Q_OFF + wg * SM::Q_BYTES + umma::umma_off(wt, 8 * c, D)) = x;
-    }
-    umma::fence_smem_to_async();
-  }
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
@@ -465,7 +430,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         umma::commit(&kfree[i % kStages]);
         last_s = i;
       };
-      issue_s(0);
+      ok = mbar_wait_near(qready, 0, a.err);
+      if (ok) issue_s(0);
       if (ok && nj > 1) issue_s(1);
       for (int i = 0; ok && i < nj; ++i) {
         ok = mbar_wait_near(&vready[i % kStages], (i / kStages) & 1, a.err) &&
@@ -494,6 +460,68 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   } else {
     // ============================ softmax ============================
     regs_up<kRegsSoftmax>();
+    const int wg = ctid >> 7;
+    // ---- the Q operands: each warp stages its 32 rows, 8 rows x 4 vectors at a time
+    // (64 contiguous bytes a row; 8 lanes' 16-byte stores fill a core matrix)
+    {
+      constexpr int NC = D / 32;  // such loads of a group of 8 rows
+#pragma unroll
+      for (int g2 = 0; g2 < 4; g2 += 2) {
+        uint4 x[2][NC];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const int r = 32 * warp + 8 * (g2 + g) + (lane & 7);
+          const uint32_t rho = r0 + r, tok = rho / grp;
+          const uint4* src = reinterpret_cast<const uint4*>(
+              a.q + static_cast<int64_t>(q0 + tok) * a.q_t + (h * grp + rho - tok * grp) * a.q_h);
+#pragma unroll
+          for (int c = 0; c < NC; ++c)
+            x[g][c] = r < rows ? __ldg(src + 4 * c + (lane >> 3)) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const int r = 32 * warp + 8 * (g2 + g) + (lane & 7);
+          float up = 1.f, down = 1.f;
+          if (a.q_bf16) {
+            float m = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+              const uint32_t w[4] = {x[g][c].x, x[g][c].y, x[g][c].z, x[g][c].w};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack2<true>(w[e]);
+                m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
+              }
+            }
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            int8_row_power(m, up, down);
+          }
+          if (lane < 8) row_s[r] = up;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) {
+            uint32_t w[4] = {x[g][c].x, x[g][c].y, x[g][c].z, x[g][c].w};
+            if (a.q_bf16) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 f = unpack2<true>(w[e]);
+                w[e] = pack_h2(f.x * down, f.y * down);
+              }
+            }
+            *reinterpret_cast<uint4*>(smem + SM::Q_OFF + wg * SM::Q_BYTES +
+                                      umma::umma_off(r & 127, 8 * (4 * c + (lane >> 3)), D)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      umma::fence_smem_to_async();
+      mbar_arrive(qready);
+      __syncwarp();
+    }
+    // thread ctid owns row ctid
+    const bool valid = ctid < rows;
+    const int qi = valid ? static_cast<int>((r0 + ctid) / grp) : 0;
+    const float ra = row_s[ctid] * a.alpha;  // 2^e * scale * log2(e)
     if (wg < wgs && kRows * wg + 32 * (warp & 3) >= rows) {
       // no row of this warp exists: it only keeps the hand-overs going
       for (int i = 0; i < nj; ++i) {
@@ -509,6 +537,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     float m = valid ? -INFINITY : 0.f, l = 0.f, vinv = 0x1p126f;
     bool ok = true;
     const float2 ra2 = make_float2(ra, ra);
+    bool fresh = true;  // a row of the warp has no reference yet
     for (int i = 0; i < nj; ++i) {
       const int st = i % kStages, t0 = (j_lo + i) * kTN;
       ok = mbar_wait_near(&vready[st], (i / kStages) & 1, a.err) &&
@@ -531,47 +560,48 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       // A pass with the reference as it is: no maximum is taken.  A sum of
       // 2^kInt8Lazy or less shows that no weight has outgrown it.
 #pragma unroll 1
-      for (int pass = 0;; ++pass) {
+      for (int pass = fresh || fv != 1.f ? 1 : 0;; ++pass) {
+        if (pass) {
+          // The reference has to move (or the value scales' power of two has): the
+          // tile's maximum, and O and l brought to the new reference.
+          float mx = -INFINITY;
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+            float x[16];
+            ld16_wait(tSi + 16 * q, x);
+            scale_scores<true>(x, ks4 + 4 * q, t0 + 16 * q, pmin, plim);
+#pragma unroll
+            for (int c = 0; c < 16; c += 2) mx = fmaxf(mx, fmaxf(x[c], x[c + 1]));
+          }
+          mx *= ra;  // ra > 0 keeps the order
+          const bool up = mx > m;
+          const float f = up ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
+          m = up ? mx : m;
+          l *= f;
+          fresh = __any_sync(0xffffffffu, m == -INFINITY);
+          if (i > 0) {  // O holds the tiles before, once the last one's products are in
+            ok = __all_sync(0xffffffffu,
+                            mbar_wait_near(&odone[2 * wg + ((i - 1) & 1)], ((i - 1) >> 1) & 1, a.err));
+            if (!ok) break;
+            umma::fence_after_sync();
+#pragma unroll 1
+            for (int c0 = 0; c0 < D; c0 += 16) {
+              float o[16];
+              ld16_wait(tO + c0, o);
+#pragma unroll
+              for (int c = 0; c < 16; ++c) o[c] *= f * fv;
+              umma::st16(tO + c0, o);
+            }
+            umma::wait_st();
+          }
+        }
         sum = make_float2(0.f, 0.f);
         const float nm = m == -INFINITY ? 0.f : -m;
         if (masked)
           tile_weights<true>(tSi, ks4, vs4, t0, pmin, plim, ra2, nm, sum, pk);
         else
           tile_weights<false>(tSi, ks4, vs4, t0, pmin, plim, ra2, nm, sum, pk);
-        if (pass || !__any_sync(0xffffffffu, sum.x + sum.y > kInt8LazyWeight || m == -INFINITY || fv != 1.f))
-          break;
-        // The reference has to move (or the value scales' power of two has): the
-        // tile's maximum, O and l brought to the new reference, and the weights
-        // again (the scores are still in tensor memory).
-        float mx = -INFINITY;
-#pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          float x[16];
-          ld16_wait(tSi + 16 * q, x);
-          scale_scores<true>(x, ks4 + 4 * q, t0 + 16 * q, pmin, plim);
-#pragma unroll
-          for (int c = 0; c < 16; c += 2) mx = fmaxf(mx, fmaxf(x[c], x[c + 1]));
-        }
-        mx *= ra;  // ra > 0 keeps the order
-        const bool up = mx > m;
-        const float f = up ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
-        m = up ? mx : m;
-        l *= f;
-        if (i > 0) {  // O holds the tiles before, once the last one's products are in
-          ok = __all_sync(0xffffffffu,
-                          mbar_wait_near(&odone[2 * wg + ((i - 1) & 1)], ((i - 1) >> 1) & 1, a.err));
-          if (!ok) break;
-          umma::fence_after_sync();
-#pragma unroll 1
-          for (int c0 = 0; c0 < D; c0 += 16) {
-            float o[16];
-            ld16_wait(tO + c0, o);
-#pragma unroll
-            for (int c = 0; c < 16; ++c) o[c] *= f * fv;
-            umma::st16(tO + c0, o);
-          }
-          umma::wait_st();
-        }
+        if (pass || !__any_sync(0xffffffffu, sum.x + sum.y > kInt8LazyWeight)) break;
       }
       if (!ok) break;
       l += sum.x + sum.y;
@@ -584,31 +614,45 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       ok = mbar_wait_near(&odone[2 * wg + ((nj - 1) & 1)], ((nj - 1) >> 1) & 1, a.err);
     ok = __all_sync(0xffffffffu, ok);
     umma::fence_after_sync();
-    // ---- normalise and write the row (a run's partial when the context is split) ----
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    // ---- normalise and write the rows (a run's partial when the context is split),
+    // eight channels a thread, 64 contiguous bytes a quad ----
+    row_s[ctid] = l == 0.f ? 0.f : 1.f / l;
+    __syncwarp();
     const float vs = (1.f / vinv) / kInt8WeightUp;
-    const int64_t row = static_cast<int64_t>(q0 + qi) * a.num_q_heads + hq;
-    const int64_t slot = static_cast<int64_t>(blockIdx.x) * kSoftmax + ctid;
+    const int64_t slot0 = static_cast<int64_t>(blockIdx.x) * kSoftmax;
     if (ok) {
 #pragma unroll 1
-      for (int u = 0; u < D / 32; ++u) {
-        float o[32];
-        __syncwarp();
-        if (nj > 0) {
-          ld32_wait(tO + 32 * u, o);
-        } else {
+      for (int hh = 0; hh < 2; ++hh) {
+        const int row0 = (ctid & ~31) + 16 * hh + (lane >> 2);  // and + 8
+        float inv[2];
+        int64_t at[2];
 #pragma unroll
-          for (int c = 0; c < 32; ++c) o[c] = 0.f;
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t rho = r0 + row0 + 8 * k, tok = rho / grp;
+          inv[k] = row_s[row0 + 8 * k] * vs;
+          at[k] = (static_cast<int64_t>(q0 + tok) * a.num_q_heads + h * grp + rho - tok * grp) * D;
         }
-        if (valid) {
 #pragma unroll
-          for (int g = 0; g < 8; g += 2) {  // channels 32 u + 4 g .. + 7
+        for (int u = 0; u < D / 32; ++u) {
+          float o[16];
+          __syncwarp();
+          if (nj > 0) {
+            ld_frag32(tO + 32 * u + (static_cast<uint32_t>(16 * hh) << 16), o);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) o[c] = 0.f;
+          }
+          // column 8 j + g of the 32 is channel 4 g + j: this thread's g are 2 (lane %
+          // 4) and + 1, eight channels in a row
+          const int c = 32 * u + 8 * (lane & 3);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (row0 + 8 * k >= rows) continue;
             float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = o[8 * (e & 3) + g + (e >> 2)] * inv * vs;
-            const int c = 32 * u + 4 * g;
+            for (int e = 0; e < 8; ++e) v[e] = o[4 * (e & 3) + 2 * k + (e >> 2)] * inv[k];
             if (sp.n > 1) {
-              float4* dst = reinterpret_cast<float4*>(sp.part_o + slot * D + c);
+              float4* dst = reinterpret_cast<float4*>(sp.part_o + (slot0 + row0 + 8 * k) * D + c);
               dst[0] = make_float4(v[0], v[1], v[2], v[3]);
               dst[1] = make_float4(v[4], v[5], v[6], v[7]);
             } else {
@@ -619,12 +663,13 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
               else
                 w = make_uint4(pack2<false>(v[0], v[1]), pack2<false>(v[2], v[3]),
                                pack2<false>(v[4], v[5]), pack2<false>(v[6], v[7]));
-              *reinterpret_cast<uint4*>(a.out + row * D + c) = w;
+              *reinterpret_cast<uint4*>(a.out + at[k] + c) = w;
             }
           }
         }
       }
-      if (sp.n > 1 && valid) *reinterpret_cast<float2*>(sp.part_ml + slot * 2) = make_float2(m, l);
+      if (sp.n > 1 && valid)
+        *reinterpret_cast<float2*>(sp.part_ml + (slot0 + ctid) * 2) = make_float2(m, l);
     }
     }
   }
@@ -639,18 +684,16 @@ template <int D>
 __global__ void __launch_bounds__(256) int8_chunk_join_kernel(const Int8AttendArgs a,
                                                               const Int8ChunkSplits sp) {
   const int lane = threadIdx.x & 31;
-  const long long wid = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const long long cta = wid / kSoftmax;  // (pair, row tile)
-  const int r = static_cast<int>(wid % kSoftmax);
-  const int rt = sp.row_tiles - 1 - static_cast<int>(cta % sp.row_tiles);
-  const int bh = static_cast<int>(cta / sp.row_tiles), s = bh / a.n_kv_heads, h = bh - s * a.n_kv_heads;
+  const int cta = blockIdx.x / (kSoftmax / 8);  // (pair, row tile)
+  const int r = blockIdx.x % (kSoftmax / 8) * 8 + (threadIdx.x >> 5);
+  const int rt = sp.row_tiles - 1 - cta % sp.row_tiles;
+  const int bh = cta / sp.row_tiles, s = bh / a.n_kv_heads, h = bh - s * a.n_kv_heads;
   if (s >= a.num_seqs) return;
   const int L = __ldg(a.seq_lens + s), q0 = __ldg(a.cu_q + s), n = __ldg(a.cu_q + s + 1) - q0;
   if (!int8_attend_ok(a, L, q0, n)) return;
-  const long long rows = static_cast<long long>(n) * a.grp;
-  const long long rho = static_cast<long long>(rt) * kSoftmax + r;
+  const uint32_t grp = a.grp, rows = static_cast<uint32_t>(n) * grp, rho = rt * kSoftmax + r;
   if (rows <= kInt8DecodeRows || rho >= rows) return;
-  const long long slot0 = cta * sp.n * kSoftmax + r;
+  const long long slot0 = static_cast<long long>(cta) * sp.n * kSoftmax + r;
   float M = -INFINITY;
   for (int i = 0; i < sp.n; ++i) M = fmaxf(M, __ldcg(sp.part_ml + (slot0 + static_cast<long long>(i) * kSoftmax) * 2));
   const float ref = M == -INFINITY ? 0.f : M;
@@ -665,7 +708,8 @@ __global__ void __launch_bounds__(256) int8_chunk_join_kernel(const Int8AttendAr
       acc[c] = fmaf(w, __ldcg(sp.part_o + slot * D + (D / 32) * lane + c), acc[c]);
   }
   const float inv = W == 0.f ? 0.f : 1.f / W;
-  const int64_t at = (static_cast<int64_t>(q0 + rho / a.grp) * a.num_q_heads + h * a.grp + rho % a.grp) * D +
+  const uint32_t tok = rho / grp;
+  const int64_t at = (static_cast<int64_t>(q0 + tok) * a.num_q_heads + h * grp + rho - tok * grp) * D +
                      (D / 32) * lane;
 #pragma unroll
   for (int c = 0; c < D / 32; c += 2) {

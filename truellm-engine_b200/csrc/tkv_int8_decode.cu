@@ -71,16 +71,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
     if (h == 0 && split == 0 && threadIdx.x == 0) set_err(a.err, TKV_ERR_BAD_LENGTH);
     return;
   }
-  const long long rows_l = static_cast<long long>(n) * a.grp;
-  if (rows_l == 0 || rows_l > RB) return;  // nothing, or the chunk kernel's
-  const int rows = static_cast<int>(rows_l);
+  // rows of a (sequence, kv head) are below 2^30 (checked on the host)
+  const int rows = n * a.grp;
+  if (rows == 0 || rows > RB) return;  // nothing, or the chunk kernel's
   // pages that some row sees, cut into ns runs of equal length
   const int first = a.window > 0 ? max(0, len - n - a.window + 1) : 0;
   const int pg0 = first / kPage, npg = (len + kPage - 1) / kPage - pg0;
   const int ns = min(sp.n, (npg + sp.pages - 1) / sp.pages);
   if (split >= ns) return;
-  const int p_lo = pg0 + static_cast<int>(static_cast<long long>(npg) * split / ns);
-  const int p_hi = pg0 + static_cast<int>(static_cast<long long>(npg) * (split + 1) / ns);
+  const int per = npg / ns, more = npg - per * ns;  // the first `more` runs have one more
+  const int p_lo = pg0 + split * per + min(split, more), p_hi = p_lo + per + (split < more ? 1 : 0);
 
   uint8_t* const ring = smem + warp * (kStages * kSP * F::BYTES);
   uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + ring_bytes<D>()) + warp * kStages;
