@@ -121,6 +121,21 @@ __device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
   return *reinterpret_cast<const float2*>(&d);
 }
 
+// 16 bytes global -> shared, or zeros
+__device__ __forceinline__ void cp_async16_or_zero(void* dst_smem, const void* src_gmem, bool copy) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(dst_smem)),
+               "l"(src_gmem), "r"(copy ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ float absmax2(uint32_t bf16_pair) {
+  const float2 f = unpack2<true>(bf16_pair);
+  return fmaxf(fabsf(f.x), fabsf(f.y));
+}
+__device__ __forceinline__ uint32_t bf16_to_h2(uint32_t bf16_pair, float factor) {
+  const float2 f = unpack2<true>(bf16_pair);
+  return pack_h2(f.x * factor, f.y * factor);
+}
+
 // 16 scores of a row (tokens t ..) times their key scales; MASKED: tokens that
 // the row does not see (outside [pmin, plim]) become -inf.
 template <bool MASKED>
@@ -139,21 +154,19 @@ __device__ __forceinline__ void scale_scores(float (&x)[16], const float4* ks4, 
   }
 }
 
-// The weights of a tile's 64 tokens (scores at tensor-memory column ts): 2^(x ra
-// + nm), added to sum, and times the value scales (2^-E 2^5 included) as f16
-// pairs.  A masked token's is 0 whatever its scale holds.  Sixteen tokens at a
-// time, one group's exponentials while the next one's scores are scaled.
-template <bool MASKED>
-__device__ __forceinline__ void tile_weights(uint32_t ts, const float4* ks4, const float4* vs4, int t,
-                                             int pmin, int plim, float2 ra2, float nm, float2& sum,
-                                             uint32_t (&pk)[32]) {
+// The weights of a tile's 64 tokens (scores at tensor-memory column ts), every one
+// of which the row sees: 2^(x ra + nm), added to sum, and times the value scales
+// (2^-E 2^5 included) as f16 pairs.  Sixteen tokens at a time, one group's
+// exponentials while the next one's scores are scaled.
+__device__ __forceinline__ void tile_weights(uint32_t ts, const float4* ks4, const float4* vs4,
+                                             float2 ra2, float nm, float2& sum, uint32_t (&pk)[32]) {
   const float2 nm2 = make_float2(nm, nm);
   float x[2][16];
   float2 s1 = make_float2(0.f, 0.f);
   ld16_issue(ts, x[0]);
   wait_ld_of(x[0]);
   ld16_issue(ts + 16, x[1]);
-  scale_scores<MASKED>(x[0], ks4, t, pmin, plim);
+  scale_scores<false>(x[0], ks4, 0, 0, 0);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     float(&y)[16] = x[q & 1];
@@ -165,21 +178,15 @@ __device__ __forceinline__ void tile_weights(uint32_t ts, const float4* ks4, con
     }
     if (q < 3) {
       wait_ld_of(x[(q + 1) & 1]);
-      scale_scores<MASKED>(x[(q + 1) & 1], ks4 + 4 * (q + 1), t + 16 * (q + 1), pmin, plim);
+      scale_scores<false>(x[(q + 1) & 1], ks4 + 4 * (q + 1), 0, 0, 0);
     }
 #pragma unroll
     for (int c = 0; c < 16; c += 4) {
       const float4 v4 = vs4[4 * q + c / 4];
       sum = fadd2(sum, w[c / 2]);
       s1 = fadd2(s1, w[c / 2 + 1]);
-      float2 w0 = fmul2(w[c / 2], make_float2(v4.x, v4.y));
-      float2 w1 = fmul2(w[c / 2 + 1], make_float2(v4.z, v4.w));
-      if constexpr (MASKED) {
-        w0.x = y[c] == -INFINITY ? 0.f : w0.x;
-        w0.y = y[c + 1] == -INFINITY ? 0.f : w0.y;
-        w1.x = y[c + 2] == -INFINITY ? 0.f : w1.x;
-        w1.y = y[c + 3] == -INFINITY ? 0.f : w1.y;
-      }
+      const float2 w0 = fmul2(w[c / 2], make_float2(v4.x, v4.y));
+      const float2 w1 = fmul2(w[c / 2 + 1], make_float2(v4.z, v4.w));
       pk[8 * q + c / 2] = pack_h2(w0.x, w0.y);
       pk[8 * q + c / 2 + 1] = pack_h2(w1.x, w1.y);
     }
@@ -462,57 +469,49 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     regs_up<kRegsSoftmax>();
     const int wg = ctid >> 7;
     // ---- the Q operands: each warp stages its 32 rows, 8 rows x 4 vectors at a time
-    // (64 contiguous bytes a row; 8 lanes' 16-byte stores fill a core matrix)
+    // (64 contiguous bytes a row; 8 lanes' 16-byte stores fill a core matrix), copied
+    // to their places as they are; bf16 becomes f16 there ----
+    uint8_t* const qs = smem + SM::Q_OFF + wg * SM::Q_BYTES;
     {
-      constexpr int NC = D / 32;  // such loads of a group of 8 rows
+      uint32_t tok[4], head[4];
 #pragma unroll
-      for (int g2 = 0; g2 < 4; g2 += 2) {
-        uint4 x[2][NC];
+      for (int g = 0; g < 4; ++g) {
+        const uint32_t rho = r0 + min(32 * warp + 8 * g + (lane & 7), rows - 1);
+        tok[g] = rho / grp;
+        head[g] = h * grp + rho - tok[g] * grp;
+      }
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const int r = 32 * warp + 8 * (g2 + g) + (lane & 7);
-          const uint32_t rho = r0 + r, tok = rho / grp;
-          const uint4* src = reinterpret_cast<const uint4*>(
-              a.q + static_cast<int64_t>(q0 + tok) * a.q_t + (h * grp + rho - tok * grp) * a.q_h);
+      for (int g = 0; g < 4; ++g) {
+        const int r = 32 * warp + 8 * g + (lane & 7);
+        const uint16_t* src = a.q + static_cast<int64_t>(q0 + tok[g]) * a.q_t + head[g] * a.q_h;
 #pragma unroll
-          for (int c = 0; c < NC; ++c)
-            x[g][c] = r < rows ? __ldg(src + 4 * c + (lane >> 3)) : make_uint4(0, 0, 0, 0);
-        }
+        for (int c = 0; c < D / 32; ++c)
+          cp_async16_or_zero(qs + umma::umma_off(r & 127, 8 * (4 * c + (lane >> 3)), D),
+                             src + 8 * (4 * c + (lane >> 3)), r < rows);
+      }
+      cp_async_wait_all();
+      __syncwarp();
+#pragma unroll 1
+      for (int g = 0; g < 4; ++g) {
+        const int r = 32 * warp + 8 * g + (lane & 7);
+        uint4* const at = reinterpret_cast<uint4*>(qs + umma::umma_off(r & 127, 8 * (lane >> 3), D));
+        float up = 1.f, down = 1.f, m = 0.f;
+        if (a.q_bf16) {
+          uint4 x[D / 32];
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const int r = 32 * warp + 8 * (g2 + g) + (lane & 7);
-          float up = 1.f, down = 1.f;
-          if (a.q_bf16) {
-            float m = 0.f;
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-              const uint32_t w[4] = {x[g][c].x, x[g][c].y, x[g][c].z, x[g][c].w};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 f = unpack2<true>(w[e]);
-                m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
-              }
-            }
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
-            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            int8_row_power(m, up, down);
+          for (int c = 0; c < D / 32; ++c) {
+            x[c] = at[32 * c];  // 4 core matrices of 8 channels on
+            m = fmaxf(fmaxf(m, absmax2(x[c].x)), fmaxf(absmax2(x[c].y), fmaxf(absmax2(x[c].z), absmax2(x[c].w))));
           }
-          if (lane < 8) row_s[r] = up;
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+          int8_row_power(m, up, down);
 #pragma unroll
-          for (int c = 0; c < NC; ++c) {
-            uint32_t w[4] = {x[g][c].x, x[g][c].y, x[g][c].z, x[g][c].w};
-            if (a.q_bf16) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 f = unpack2<true>(w[e]);
-                w[e] = pack_h2(f.x * down, f.y * down);
-              }
-            }
-            *reinterpret_cast<uint4*>(smem + SM::Q_OFF + wg * SM::Q_BYTES +
-                                      umma::umma_off(r & 127, 8 * (4 * c + (lane >> 3)), D)) =
-                make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          for (int c = 0; c < D / 32; ++c)
+            at[32 * c] = make_uint4(bf16_to_h2(x[c].x, down), bf16_to_h2(x[c].y, down),
+                                    bf16_to_h2(x[c].z, down), bf16_to_h2(x[c].w, down));
         }
+        if (lane < 8) row_s[r] = up;
       }
       umma::fence_smem_to_async();
       mbar_arrive(qready);
@@ -545,7 +544,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       umma::fence_after_sync();
-      bool masked = __any_sync(0xffffffffu, valid && (t0 + kTN - 1 > plim || t0 < pmin));
+      const bool masked = __any_sync(0xffffffffu, valid && (t0 + kTN - 1 > plim || t0 < pmin));
       const float vnew = vi_s[st];
       float fv = 1.f;
       if (vnew != vinv) {
@@ -555,57 +554,79 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       const uint32_t tSi = tS + (i & 1) * kTN;
       const float4* ks4 = reinterpret_cast<const float4*>(ks_s + st * kTN);
       const float4* vs4 = reinterpret_cast<const float4*>(vs_s + st * kTN);
-      float2 sum;
-      uint32_t pk[32];
-      // A pass with the reference as it is: no maximum is taken.  A sum of
-      // 2^kInt8Lazy or less shows that no weight has outgrown it.
+      bool plain = !masked && !fresh && fv == 1.f;
+      if (plain) {
+        // A pass with the reference as it is: no maximum is taken.  A sum of
+        // 2^kInt8Lazy or less shows that no weight has outgrown it.
+        float2 sum = make_float2(0.f, 0.f);
+        uint32_t pk[32];
+        tile_weights(tSi, ks4, vs4, ra2, -m, sum, pk);
+        plain = !__any_sync(0xffffffffu, sum.x + sum.y > kInt8LazyWeight);
+        if (plain) {
+          l += sum.x + sum.y;
+          st32u(tSi, pk);
+        }
+      }
+      if (!plain) {
+        // Masked tokens, a first reference, one that has to move, or the value
+        // scales' power of two has: the tile's maximum, O and l brought to the new
+        // reference, then the weights.  (Compact code: it is rare, and instruction
+        // fetches cost the CTA's start and end more than its loops.)
+        float mx = -INFINITY;
 #pragma unroll 1
-      for (int pass = fresh || fv != 1.f ? 1 : 0;; ++pass) {
-        if (pass) {
-          // The reference has to move (or the value scales' power of two has): the
-          // tile's maximum, and O and l brought to the new reference.
-          float mx = -INFINITY;
-#pragma unroll 1
-          for (int q = 0; q < 4; ++q) {
-            float x[16];
-            ld16_wait(tSi + 16 * q, x);
-            scale_scores<true>(x, ks4 + 4 * q, t0 + 16 * q, pmin, plim);
+        for (int q = 0; q < 4; ++q) {
+          float x[16];
+          ld16_wait(tSi + 16 * q, x);
+          scale_scores<true>(x, ks4 + 4 * q, t0 + 16 * q, pmin, plim);
 #pragma unroll
-            for (int c = 0; c < 16; c += 2) mx = fmaxf(mx, fmaxf(x[c], x[c + 1]));
-          }
-          mx *= ra;  // ra > 0 keeps the order
-          const bool up = mx > m;
-          const float f = up ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
-          m = up ? mx : m;
-          l *= f;
-          fresh = __any_sync(0xffffffffu, m == -INFINITY);
-          if (i > 0) {  // O holds the tiles before, once the last one's products are in
-            ok = __all_sync(0xffffffffu,
-                            mbar_wait_near(&odone[2 * wg + ((i - 1) & 1)], ((i - 1) >> 1) & 1, a.err));
-            if (!ok) break;
-            umma::fence_after_sync();
+          for (int c = 0; c < 16; c += 2) mx = fmaxf(mx, fmaxf(x[c], x[c + 1]));
+        }
+        mx *= ra;  // ra > 0 keeps the order
+        const bool up = mx > m;
+        const float f = up ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
+        m = up ? mx : m;
+        l *= f;
+        fresh = __any_sync(0xffffffffu, m == -INFINITY);
+        if (i > 0 && __any_sync(0xffffffffu, f * fv != 1.f)) {
+          // O holds the tiles before, once the last one's products are in
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait_near(&odone[2 * wg + ((i - 1) & 1)], ((i - 1) >> 1) & 1, a.err));
+          if (!ok) break;
+          umma::fence_after_sync();
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += 16) {
-              float o[16];
-              ld16_wait(tO + c0, o);
+          for (int c0 = 0; c0 < D; c0 += 16) {
+            float o[16];
+            ld16_wait(tO + c0, o);
 #pragma unroll
-              for (int c = 0; c < 16; ++c) o[c] *= f * fv;
-              umma::st16(tO + c0, o);
-            }
-            umma::wait_st();
+            for (int c = 0; c < 16; ++c) o[c] *= f * fv;
+            umma::st16(tO + c0, o);
           }
         }
-        sum = make_float2(0.f, 0.f);
         const float nm = m == -INFINITY ? 0.f : -m;
-        if (masked)
-          tile_weights<true>(tSi, ks4, vs4, t0, pmin, plim, ra2, nm, sum, pk);
-        else
-          tile_weights<false>(tSi, ks4, vs4, t0, pmin, plim, ra2, nm, sum, pk);
-        if (pass || !__any_sync(0xffffffffu, sum.x + sum.y > kInt8LazyWeight)) break;
+        // P of tokens 16 q .. goes over columns 8 q .., whose scores have been read
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          float x[16];
+          uint32_t pw[8];
+          ld16_wait(tSi + 16 * q, x);
+          scale_scores<true>(x, ks4 + 4 * q, t0 + 16 * q, pmin, plim);
+#pragma unroll
+          for (int c = 0; c < 16; c += 4) {
+            const float4 v4 = vs4[4 * q + c / 4];
+            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+            float w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float p = fast_exp2(fmaf(x[c + e], ra, nm));
+              l += p;
+              w[e] = x[c + e] == -INFINITY ? 0.f : p * v[e];  // masked: whatever the scale holds
+            }
+            pw[c / 2] = pack_h2(w[0], w[1]);
+            pw[c / 2 + 1] = pack_h2(w[2], w[3]);
+          }
+          umma::st8(tSi + 8 * q, pw);
+        }
       }
-      if (!ok) break;
-      l += sum.x + sum.y;
-      st32u(tSi, pk);
       umma::wait_st();
       umma::fence_before_sync();
       mbar_arrive(&pready[2 * wg + (i & 1)]);
@@ -632,7 +653,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
           inv[k] = row_s[row0 + 8 * k] * vs;
           at[k] = (static_cast<int64_t>(q0 + tok) * a.num_q_heads + h * grp + rho - tok * grp) * D;
         }
-#pragma unroll
+#pragma unroll 1
         for (int u = 0; u < D / 32; ++u) {
           float o[16];
           __syncwarp();
