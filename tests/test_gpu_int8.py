@@ -625,6 +625,22 @@ def test_one_workspace_serves_smaller_calls(ops, cuda):
         b.check(q, out, rows=4)
 
 
+def test_a_workspace_shared_by_calls_of_very_different_sizes(ops, cuda):
+    """Few pairs with many runs, many pairs with few, chunks: in turn, twice."""
+    shapes = [([20000], [1], 1, 8), ([600] * 40, [1] * 40, 4, 8), ([900, 40], [50, 3], 1, 4),
+              ([9, 3000], [1, 1], 2, 32)]
+    bs, need = [], 0
+    for i, (old, new, H, Hq) in enumerate(shapes):
+        b = Batch(ops, cuda, old, new, H, 64, BF16, seed=i)
+        b.fill()
+        bs.append((b, b.query(Hq)))
+        need = max(need, ops.int8_workspace_bytes(len(old), Hq, H, 64, max(new), int(b.lens.max())))
+    ws = torch.zeros(need, dtype=torch.uint8, device=cuda)
+    for _ in range(2):
+        for b, q in bs:
+            assert torch.equal(b.attend(q, workspace=ws), b.attend(q))
+
+
 def test_no_tokens(ops, cuda):
     b = Batch(ops, cuda, [4, 0], [0, 0], 1, 64, F16)
     q = torch.empty(0, 4, 64, device=cuda, dtype=F16)

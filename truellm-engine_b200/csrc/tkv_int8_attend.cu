@@ -18,6 +18,12 @@ constexpr int kSlots = 148 * 3;  // resident CTAs of the decode kernel
 constexpr int kMinRun = 8;       // pages: one step of each of a CTA's warps
 constexpr int kMaxRun = 64;
 constexpr int kMaxRuns = 512;
+// The workspace starts with the counters of this many (sequence, kv head) pairs,
+// whatever the call's sizes, so calls of different sizes that take turns with one
+// workspace never write partials over each other's counters.  Calls with more
+// pairs have no need to split.
+constexpr int kMaxPairs = 65536;
+constexpr size_t kCounterBytes = kMaxPairs * sizeof(unsigned int);
 
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
@@ -26,38 +32,41 @@ size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 // longer than kMaxRun pages.
 void decode_splits(Int8Splits& sp, int num_seqs, int num_kv_heads, int grp, int max_q, int max_len) {
   const long long pages = (static_cast<long long>(max_len) + kPage - 1) / kPage;
-  const long long total = pages * num_seqs * num_kv_heads;
+  const long long pairs = static_cast<long long>(num_seqs) * num_kv_heads, total = pages * pairs;
   long long run = (total + kSlots - 1) / kSlots;
   run = std::min<long long>(kMaxRun, std::max<long long>(kMinRun, (run + kMinRun - 1) / kMinRun * kMinRun));
-  run = std::max(run, (pages + kMaxRuns - 1) / kMaxRuns);
+  run = std::max(run, pairs > kMaxPairs ? pages : (pages + kMaxRuns - 1) / kMaxRuns);
   sp.pages = static_cast<int>(run);
   sp.n = static_cast<int>(std::max<long long>(1, (pages + run - 1) / run));
   sp.rows = static_cast<int>(std::min<long long>(kInt8DecodeRows, static_cast<long long>(max_q) * grp));
 }
 
-// bytes of the decode kernel's share of the workspace
+// bytes of the decode kernel's partials
 size_t decode_bytes(const Int8Splits& sp, int num_seqs, int num_kv_heads, int head_dim) {
   const size_t pairs = static_cast<size_t>(num_seqs) * num_kv_heads;
   const size_t rb = sp.rows <= 8 ? 8 : 16;
-  return round256(pairs * 4) + (sp.n > 1 ? round256(pairs * sp.n * rb * 8) + pairs * sp.n * rb * head_dim * 4 : 0);
+  return sp.n > 1 ? round256(pairs * sp.n * rb * 8) + pairs * sp.n * rb * head_dim * 4 : 0;
 }
 
-constexpr int kSMs = 148;       // CTAs of the chunk kernel: one per SM
 constexpr int kMinTiles = 8;    // 64-token tiles of a run
 
-// How chunk contexts are cut: not at all when the row tiles alone fill the GPU.
+// How chunk items are cut: those that fill whole rounds of the SMs not at all; the
+// rest (or all, when there are few) into as many runs as leave no SM idle.
 void chunk_splits(Int8ChunkSplits& sp, int num_seqs, int num_kv_heads, int grp, int max_q, int max_len) {
   const long long rows = static_cast<long long>(max_q) * grp;
-  sp.row_tiles = static_cast<int>(std::min<long long>(INT_MAX, (rows + kInt8ChunkRows - 1) / kInt8ChunkRows));
-  const long long ctas = std::max<long long>(1, static_cast<long long>(num_seqs) * num_kv_heads * sp.row_tiles);
+  sp.row_tiles = static_cast<int>(std::max<long long>(1, (rows + kInt8ChunkRows - 1) / kInt8ChunkRows));
+  const long long items = std::min<long long>(INT_MAX, static_cast<long long>(num_seqs) * num_kv_heads * sp.row_tiles);
+  const long long rest = items % kInt8ChunkSMs;
   const long long tiles = (static_cast<long long>(max_len) + 63) / 64;
-  sp.n = static_cast<int>(std::max<long long>(1, std::min(kSMs / ctas, tiles / kMinTiles)));
+  sp.n = rest == 0 ? 1 : static_cast<int>(std::max<long long>(1, std::min(kInt8ChunkSMs / rest, tiles / kMinTiles)));
+  sp.whole = static_cast<int>(sp.n > 1 ? items - rest : items);
 }
 
 // bytes of the chunk kernel's share of the workspace
 size_t chunk_bytes(const Int8ChunkSplits& sp, int num_seqs, int num_kv_heads, int head_dim) {
   if (sp.n <= 1) return 0;
-  const size_t slots = static_cast<size_t>(num_seqs) * num_kv_heads * sp.row_tiles * sp.n * kInt8ChunkRows;
+  const size_t items = static_cast<size_t>(num_seqs) * num_kv_heads * sp.row_tiles - sp.whole;
+  const size_t slots = items * sp.n * kInt8ChunkRows;
   return round256(slots * 8) + slots * head_dim * 4;
 }
 
@@ -71,7 +80,7 @@ size_t int8_attend_workspace(int num_seqs, int num_q_heads, int num_kv_heads, in
                              int max_q, int max_len) {
   Int8Splits sp;
   decode_splits(sp, num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_q, max_len);
-  size_t n = 256 + round256(decode_bytes(sp, num_seqs, num_kv_heads, head_dim));
+  size_t n = kCounterBytes + round256(decode_bytes(sp, num_seqs, num_kv_heads, head_dim));
   if (has_chunks(num_q_heads / num_kv_heads, max_q)) {
     Int8ChunkSplits cs;
     chunk_splits(cs, num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_q, max_len);
@@ -85,10 +94,9 @@ int launch_int8_attend(const Int8AttendArgs& a, int head_dim, void* workspace, s
   Int8Splits sp;
   decode_splits(sp, a.num_seqs, a.n_kv_heads, a.grp, a.max_q, a.max_len);
   const size_t pairs = static_cast<size_t>(a.num_seqs) * a.n_kv_heads;
-  uint8_t* ws = static_cast<uint8_t*>(workspace) + 256;
+  sp.count = static_cast<unsigned int*>(workspace);
+  uint8_t* ws = static_cast<uint8_t*>(workspace) + kCounterBytes;
   uint8_t* chunk_ws = ws + round256(decode_bytes(sp, a.num_seqs, a.n_kv_heads, head_dim));
-  sp.count = reinterpret_cast<unsigned int*>(ws);
-  ws += round256(pairs * 4);
   sp.part_ml = reinterpret_cast<float*>(ws);
   sp.part_o = reinterpret_cast<float*>(ws + round256(pairs * sp.n * (sp.rows <= 8 ? 8 : 16) * 8));
   const int st = launch_int8_decode(a, sp, head_dim, stream);
@@ -97,7 +105,7 @@ int launch_int8_attend(const Int8AttendArgs& a, int head_dim, void* workspace, s
   chunk_splits(cs, a.num_seqs, a.n_kv_heads, a.grp, a.max_q, a.max_len);
   cs.part_ml = reinterpret_cast<float*>(chunk_ws);
   cs.part_o = reinterpret_cast<float*>(
-      chunk_ws + round256(pairs * cs.row_tiles * cs.n * kInt8ChunkRows * 8));
+      chunk_ws + round256((pairs * cs.row_tiles - cs.whole) * cs.n * kInt8ChunkRows * 8));
   return launch_int8_chunk(a, cs, head_dim, stream);
 }
 

@@ -26,13 +26,30 @@ struct Int8Splits {
   float* part_o;        // [pair][run][row block][D]  normalised
 };
 
-// Chunk kernel: 256-row tiles of a (sequence, kv head), each over n runs of
-// equal length of its context.
+// Chunk kernel: an item is a 256-row tile of a (sequence, kv head).  CTA i < whole
+// takes item i; the items from `whole` on are cut into n runs of equal length of
+// their contexts, one CTA each, and joined by a second launch.
 constexpr int kInt8ChunkRows = 256;
+constexpr int kInt8ChunkSMs = 148;  // CTAs at a time: one per SM
 struct Int8ChunkSplits {
-  int n, row_tiles;
-  float* part_ml;  // [pair][row tile][run][256][2]
-  float* part_o;   // [pair][row tile][run][256][D]  normalised
+  int whole, n, row_tiles;
+  float* part_ml;  // [item - whole][run][256][2]
+  float* part_o;   // [item - whole][run][256][D]  normalised
+};
+struct Int8ChunkItem {
+  int item, split, runs;
+  __device__ __forceinline__ Int8ChunkItem(const Int8ChunkSplits& sp, int cta) {
+    const bool one = cta < sp.whole;
+    const int e = cta - sp.whole, q = one ? 0 : e / sp.n;
+    item = one ? cta : sp.whole + q;
+    split = one ? 0 : e - q * sp.n;
+    runs = one ? 1 : sp.n;
+  }
+  __device__ __forceinline__ int pair(const Int8ChunkSplits& sp) const { return item / sp.row_tiles; }
+  // longest contexts first
+  __device__ __forceinline__ int row_tile(const Int8ChunkSplits& sp) const {
+    return sp.row_tiles - 1 - item % sp.row_tiles;
+  }
 };
 
 // the lengths of one sequence (see tkv_int8_attend)

@@ -221,6 +221,25 @@ struct Sm {
   static constexpr uint32_t TWG = 256, TO = 128, TCOLS = 512;
 };
 
+// Brings the query rows of a later CTA into L2: they come from DRAM otherwise, and
+// a CTA can do nothing before it has them (about 4 us at 128 channels).
+template <int D>
+__device__ __forceinline__ void prefetch_q(const Int8AttendArgs& a, const Int8ChunkSplits& sp, int cta,
+                                           int lane) {
+  if (cta >= static_cast<int>(gridDim.x)) return;
+  const Int8ChunkItem it(sp, cta);
+  const int bh = it.pair(sp), s = bh / a.n_kv_heads, h = bh - s * a.n_kv_heads;
+  const int L = __ldg(a.seq_lens + s), q0 = __ldg(a.cu_q + s), n = __ldg(a.cu_q + s + 1) - q0;
+  if (!int8_attend_ok(a, L, q0, n)) return;
+  const uint32_t grp = a.grp, all_rows = static_cast<uint32_t>(n) * grp, r0 = it.row_tile(sp) * kSoftmax;
+  for (uint32_t r = lane; r < kSoftmax && r0 + r < all_rows; r += 32) {
+    const uint32_t rho = r0 + r, tok = rho / grp;
+    const uint16_t* src = a.q + static_cast<int64_t>(q0 + tok) * a.q_t + (h * grp + rho - tok * grp) * a.q_h;
+#pragma unroll
+    for (int c = 0; c < D; c += 64) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(src + c));
+  }
+}
+
 template <int D>
 __global__ void __launch_bounds__(kCtaThreads, 1)
     int8_chunk_kernel(const Int8AttendArgs a, const Int8ChunkSplits sp) {
@@ -257,10 +276,9 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   float* const row_s = reinterpret_cast<float*>(smem + SM::ROW_OFF);
 
   const int ctid = threadIdx.x, warp = ctid >> 5, lane = ctid & 31;
-  const int split = blockIdx.x % sp.n;
-  const int rest = blockIdx.x / sp.n;
-  const int rt = sp.row_tiles - 1 - rest % sp.row_tiles;  // longest contexts first
-  const int bh = rest / sp.row_tiles, s = bh / a.n_kv_heads, h = bh - s * a.n_kv_heads;
+  const Int8ChunkItem it(sp, blockIdx.x);
+  const int split = it.split, runs = it.runs;
+  const int rt = it.row_tile(sp), bh = it.pair(sp), s = bh / a.n_kv_heads, h = bh - s * a.n_kv_heads;
   const int L = __ldg(a.seq_lens + s), q0 = __ldg(a.cu_q + s), n = __ldg(a.cu_q + s + 1) - q0;
   if (!int8_attend_ok(a, L, q0, n)) return;  // flagged by the decode kernel
   // rows of a (sequence, kv head) are below 2^30 (checked on the host)
@@ -268,15 +286,32 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   if (all_rows <= kInt8DecodeRows || r0 >= all_rows) return;
   const int rows = min(all_rows - r0, static_cast<uint32_t>(kSoftmax));
   const int wgs = rows > kRows ? 2 : 1;
-  // tiles that some row of this CTA sees, cut into sp.n runs
+  // tiles that some row of this CTA sees, cut into runs
   const int p_first = L - n + static_cast<int>(r0 / grp);
   const int kv_end = L - n + static_cast<int>((r0 + rows - 1) / grp) + 1;
   const int kv_lo = a.window > 0 ? max(0, p_first - a.window + 1) : 0;
   const int tile0 = kv_lo / kTN, tiles = (kv_end + kTN - 1) / kTN - tile0;
-  const int per = tiles / sp.n, more = tiles - per * sp.n;  // the first `more` runs have one more
+  const int per = tiles / runs, more = tiles - per * runs;  // the first `more` runs have one more
   const int j_lo = tile0 + split * per + min(split, more), nj = per + (split < more ? 1 : 0);
 
-  if (warp == 0) umma::alloc(tslot, SM::TCOLS);
+  // ---- the Q operands: each softmax warp copies its 32 rows, 8 rows x 4 vectors at a
+  // time (64 contiguous bytes a row; 8 lanes' 16-byte stores fill a core matrix), to
+  // their places as they are ----
+  const int wg = ctid >> 7;
+  uint8_t* const qs = smem + SM::Q_OFF + wg * SM::Q_BYTES;
+  if (ctid < kSoftmax) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int r = 32 * warp + 8 * g + (lane & 7);
+      const uint32_t rho = r0 + min(r, rows - 1), tok = rho / grp;
+      const uint16_t* src = a.q + static_cast<int64_t>(q0 + tok) * a.q_t + (h * grp + rho - tok * grp) * a.q_h;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c)
+        cp_async16_or_zero(qs + umma::umma_off(r & 127, 8 * (4 * c + (lane >> 3)), D),
+                           src + 8 * (4 * c + (lane >> 3)), r < rows);
+    }
+  }
+  if (warp == 8) umma::alloc(tslot, SM::TCOLS);
   if (ctid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&kready[i], kProducers);
@@ -418,6 +453,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     // ============================ an MMA warp ============================
     regs_down<kRegsMma>();
     const int w = warp - (kSoftmax + kProducers) / 32;  // its softmax warpgroup
+    if (w == 3) prefetch_q<D>(a, sp, blockIdx.x + kInt8ChunkSMs, lane);
     if (lane == 0 && w < wgs && nj > 0) {
       bool ok = true;
       int last_s = -1, last_o = -1;
@@ -467,28 +503,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   } else {
     // ============================ softmax ============================
     regs_up<kRegsSoftmax>();
-    const int wg = ctid >> 7;
-    // ---- the Q operands: each warp stages its 32 rows, 8 rows x 4 vectors at a time
-    // (64 contiguous bytes a row; 8 lanes' 16-byte stores fill a core matrix), copied
-    // to their places as they are; bf16 becomes f16 there ----
-    uint8_t* const qs = smem + SM::Q_OFF + wg * SM::Q_BYTES;
+    // ---- the Q operands: bf16 becomes f16 where it is ----
     {
-      uint32_t tok[4], head[4];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const uint32_t rho = r0 + min(32 * warp + 8 * g + (lane & 7), rows - 1);
-        tok[g] = rho / grp;
-        head[g] = h * grp + rho - tok[g] * grp;
-      }
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int r = 32 * warp + 8 * g + (lane & 7);
-        const uint16_t* src = a.q + static_cast<int64_t>(q0 + tok[g]) * a.q_t + head[g] * a.q_h;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c)
-          cp_async16_or_zero(qs + umma::umma_off(r & 127, 8 * (4 * c + (lane >> 3)), D),
-                             src + 8 * (4 * c + (lane >> 3)), r < rows);
-      }
       cp_async_wait_all();
       __syncwarp();
 #pragma unroll 1
@@ -640,7 +656,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     row_s[ctid] = l == 0.f ? 0.f : 1.f / l;
     __syncwarp();
     const float vs = (1.f / vinv) / kInt8WeightUp;
-    const int64_t slot0 = static_cast<int64_t>(blockIdx.x) * kSoftmax;
+    const int64_t slot0 = static_cast<int64_t>(blockIdx.x - sp.whole) * kSoftmax;  // of a split item
     if (ok) {
 #pragma unroll 1
       for (int hh = 0; hh < 2; ++hh) {
@@ -672,7 +688,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = o[4 * (e & 3) + 2 * k + (e >> 2)] * inv[k];
-            if (sp.n > 1) {
+            if (runs > 1) {
               float4* dst = reinterpret_cast<float4*>(sp.part_o + (slot0 + row0 + 8 * k) * D + c);
               dst[0] = make_float4(v[0], v[1], v[2], v[3]);
               dst[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -689,7 +705,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
           }
         }
       }
-      if (sp.n > 1 && valid)
+      if (runs > 1 && valid)
         *reinterpret_cast<float2*>(sp.part_ml + (slot0 + ctid) * 2) = make_float2(m, l);
     }
     }
@@ -697,7 +713,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
-  if (warp == 0) umma::dealloc(tmem, SM::TCOLS);
+  if (warp == 8) umma::dealloc(tmem, SM::TCOLS);
 }
 
 // Joins the runs of split contexts: a warp per row, the runs in order.
@@ -705,16 +721,15 @@ template <int D>
 __global__ void __launch_bounds__(256) int8_chunk_join_kernel(const Int8AttendArgs a,
                                                               const Int8ChunkSplits sp) {
   const int lane = threadIdx.x & 31;
-  const int cta = blockIdx.x / (kSoftmax / 8);  // (pair, row tile)
+  const int item = blockIdx.x / (kSoftmax / 8);  // of the split ones
   const int r = blockIdx.x % (kSoftmax / 8) * 8 + (threadIdx.x >> 5);
-  const int rt = sp.row_tiles - 1 - cta % sp.row_tiles;
-  const int bh = cta / sp.row_tiles, s = bh / a.n_kv_heads, h = bh - s * a.n_kv_heads;
-  if (s >= a.num_seqs) return;
+  const Int8ChunkItem it(sp, sp.whole + item * sp.n);
+  const int rt = it.row_tile(sp), bh = it.pair(sp), s = bh / a.n_kv_heads, h = bh - s * a.n_kv_heads;
   const int L = __ldg(a.seq_lens + s), q0 = __ldg(a.cu_q + s), n = __ldg(a.cu_q + s + 1) - q0;
   if (!int8_attend_ok(a, L, q0, n)) return;
   const uint32_t grp = a.grp, rows = static_cast<uint32_t>(n) * grp, rho = rt * kSoftmax + r;
   if (rows <= kInt8DecodeRows || rho >= rows) return;
-  const long long slot0 = static_cast<long long>(cta) * sp.n * kSoftmax + r;
+  const long long slot0 = static_cast<long long>(item) * sp.n * kSoftmax + r;
   float M = -INFINITY;
   for (int i = 0; i < sp.n; ++i) M = fmaxf(M, __ldcg(sp.part_ml + (slot0 + static_cast<long long>(i) * kSoftmax) * 2));
   const float ref = M == -INFINITY ? 0.f : M;
@@ -752,12 +767,13 @@ int launch_t(const Int8AttendArgs& a, const Int8ChunkSplits& sp, cudaStream_t st
       return TKV_BACKEND_ERROR;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  const long long ctas = static_cast<long long>(a.num_seqs) * a.n_kv_heads * sp.row_tiles;
-  if (ctas * std::max(sp.n, kSoftmax / 8) > INT_MAX) return TKV_INVALID_ARGUMENT;
-  int8_chunk_kernel<D><<<static_cast<unsigned int>(ctas * sp.n), kCtaThreads, Sm<D>::BYTES, stream>>>(a, sp);
+  const long long items = static_cast<long long>(a.num_seqs) * a.n_kv_heads * sp.row_tiles;
+  const long long ctas = sp.whole + (items - sp.whole) * sp.n, joins = (items - sp.whole) * (kSoftmax / 8);
+  if (items > INT_MAX || ctas > INT_MAX || joins > INT_MAX) return TKV_INVALID_ARGUMENT;
+  int8_chunk_kernel<D><<<static_cast<unsigned int>(ctas), kCtaThreads, Sm<D>::BYTES, stream>>>(a, sp);
   if (cudaGetLastError() != cudaSuccess) return TKV_BACKEND_ERROR;
   if (sp.n > 1) {
-    int8_chunk_join_kernel<D><<<static_cast<unsigned int>(ctas * (kSoftmax / 8)), 256, 0, stream>>>(a, sp);
+    int8_chunk_join_kernel<D><<<static_cast<unsigned int>(joins), 256, 0, stream>>>(a, sp);
     if (cudaGetLastError() != cudaSuccess) return TKV_BACKEND_ERROR;
   }
   return TKV_OK;
