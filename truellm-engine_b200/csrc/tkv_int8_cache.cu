@@ -2,9 +2,10 @@
 // reshape_and_cache slot of third_party/vllm_kernels/cache_kernels.cu:202-232)
 // and reading it back as dense K/V.
 //
-// One CTA per (16-token page of a sequence's range, kv head): half of its
-// threads take the keys, half the values, one thread per (token, 16 channels).
-// Lanes 4 c + i of a warp hold token 4 t + i, chunk c, so the four tokens of a
+// One CTA per 16-token page of a sequence's range and run of kv heads: half of
+// its threads take the keys, half the values, one thread per (token, 16
+// channels), one head after another with the next one's loads in flight.  Lanes 4
+// c + i of a warp hold token 4 t + i, chunk c, so the four tokens of a
 // V word sit in one quad: a 4 x 4 transpose of words over the quad and of bytes
 // within a thread turns four rows into 16-byte units of the V layout (and back).
 //
@@ -12,21 +13,37 @@
 // from cu[s] / 16 + 2 s on (a range of n tokens touches at most n / 16 + 2
 // pages), so a ragged batch launches (tokens / 16 + 2 sequences) x heads CTAs
 // whatever its longest sequence; a CTA finds its sequence by a 32-way search.
+// Where that is more than the tokens there are (a decode step), sequence s owns
+// the units from cu[s] on: a page that is touched holds a token of the range.
+// 256 sequences of one token, 8 heads: @TOKENUNIT us against 19.9.
+//
+// Both kernels are bound by memory: 2 bytes a channel on the dense side, 1 and a
+// scale on the paged one.  64 x 2048 tokens of 8 heads of 128 channels: append
+// @APP us, read @READ us.
 #include <limits.h>
 
+#include <algorithm>
+
 #include "tkv_int8.cuh"
+#include "tkv_umma.cuh"  // packed f32x2 arithmetic
 
 namespace tkv {
 namespace {
 
+// first page unit of sequence s
+__device__ __forceinline__ long long first_unit(int32_t cu_s, int s, bool per_token) {
+  return per_token ? cu_s : static_cast<long long>(cu_s / kPage) + 2ll * s;
+}
+
 // the last sequence whose first page unit is <= u (all lanes of a warp take part)
-__device__ __forceinline__ int find_seq(const int32_t* cu, int num_seqs, long long u) {
+__device__ __forceinline__ int find_seq(const int32_t* cu, int num_seqs, long long u,
+                                        bool per_token) {
   int lo = 0, hi = num_seqs;  // the answer is in [lo, hi)
   const int lane = threadIdx.x & 31;
   while (hi - lo > 1) {
     const int step = (hi - lo + 31) / 32;
     const int s = lo + lane * step;
-    const bool le = s < hi && static_cast<long long>(__ldg(cu + s) / kPage) + 2ll * s <= u;
+    const bool le = s < hi && first_unit(__ldg(cu + s), s, per_token) <= u;
     const unsigned int m = __ballot_sync(0xffffffffu, le);
     // offsets are non-decreasing in a valid call; any answer is in range otherwise
     const int last = m ? 31 - __clz(m) : 0;
@@ -35,6 +52,15 @@ __device__ __forceinline__ int find_seq(const int32_t* cu, int num_seqs, long lo
   }
   return lo;
 }
+
+// How a launch is cut up.  heads: kv heads a CTA takes one after another;
+// per_token: the numbering of page units; wide: the dense rows and their strides
+// are multiples of 32 bytes, so 16 channels are one access of a whole sector
+// (64 x 2048 tokens of 8 heads: read @WIDE).
+struct Plan {
+  int heads;
+  bool per_token, wide;
+};
 
 // what a CTA works on: page `page` (index in the sequence) of sequence s, and
 // the tokens [t_lo, t_hi) of it, which are rows row + (token - t_lo)
@@ -45,11 +71,11 @@ struct PageUnit {
 // false: nothing to do.  `lens` holds the first token of each sequence's range.
 __device__ __forceinline__ bool page_unit(const int32_t* cu, const int32_t* lens, int num_seqs,
                                           int total, int max_n, int max_blocks, long long u,
-                                          PageUnit& p) {
-  p.s = find_seq(cu, num_seqs, u);
+                                          bool per_token, PageUnit& p) {
+  p.s = find_seq(cu, num_seqs, u, per_token);
   const int r0 = __ldg(cu + p.s), n = __ldg(cu + p.s + 1) - r0, pos = __ldg(lens + p.s);
   if (!int8_seq_ok(pos, n, r0, total, max_n, max_blocks)) return false;
-  const long long j = u - (static_cast<long long>(r0 / kPage) + 2ll * p.s);
+  const long long j = u - first_unit(r0, p.s, per_token);
   if (j < 0 || j > INT_MAX / kPage) return false;
   const long long pg = pos / kPage + j;
   if (n == 0 || pg * kPage >= static_cast<long long>(pos) + n) return false;
@@ -74,32 +100,43 @@ __device__ __forceinline__ void flag_lengths(const int32_t* cu, const int32_t* l
 // than 2^-15 from x/d, so only a remainder close to one half is checked, in
 // exact arithmetic: x - k d is exact in f32 (x has 11 bits or fewer and |x - k
 // d| < d, a multiple of d's last bit).
-__device__ __forceinline__ void quantise16(const float (&x)[16], float d, float inv,
+template <bool BF16>
+__device__ __forceinline__ void quantise16(const uint32_t (&x2)[8], float d, float inv,
                                            uint32_t (&w)[4]) {
   constexpr float kMagic = 12582912.f + kInt8Bias;
-  float t[16], worst = 0.f;
+  const float2 inv2 = make_float2(inv, inv), up2 = make_float2(kMagic, kMagic);
+  const float2 down2 = make_float2(-kMagic, -kMagic), minus2 = make_float2(-1.f, -1.f);
+  float2 t[8];
+  float worst = 0.f;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    t[e] = __fmaf_rn(x[e], inv, kMagic);
-    const float k = __fsub_rn(t[e], kMagic);
-    worst = fmaxf(worst, fabsf(__fmaf_rn(x[e], inv, -k)));
+  for (int e = 0; e < 8; ++e) {
+    const float2 x = unpack2<BF16>(x2[e]);
+    t[e] = ffma2(x, inv2, up2);
+    const float2 k = fadd2(t[e], down2);
+    const float2 r = ffma2(x, inv2, ffma2(k, minus2, make_float2(0.f, 0.f)));
+    worst = fmaxf(worst, fmaxf(fabsf(r.x), fabsf(r.y)));
   }
   if (worst > 0.4999f) {
     const float h = 0.5f * d;
+    auto fix = [&](float x, float& v) {
+      const float k = __fsub_rn(v, kMagic);
+      const float r = __fmaf_rn(-k, d, x);
+      const bool odd = __float_as_uint(v) & 1u;
+      if (r > h || (r == h && odd)) v += 1.f;
+      if (r < -h || (r == -h && odd)) v -= 1.f;
+    };
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const float k = __fsub_rn(t[e], kMagic);
-      const float r = __fmaf_rn(-k, d, x[e]);
-      const bool odd = __float_as_uint(t[e]) & 1u;
-      if (r > h || (r == h && odd)) t[e] += 1.f;
-      if (r < -h || (r == -h && odd)) t[e] -= 1.f;
+    for (int e = 0; e < 8; ++e) {
+      const float2 x = unpack2<BF16>(x2[e]);
+      fix(x.x, t[e].x);
+      fix(x.y, t[e].y);
     }
   }
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
-    const uint32_t lo = __byte_perm(__float_as_uint(t[4 * a]), __float_as_uint(t[4 * a + 1]), 0x0040);
+    const uint32_t lo = __byte_perm(__float_as_uint(t[2 * a].x), __float_as_uint(t[2 * a].y), 0x0040);
     const uint32_t hi =
-        __byte_perm(__float_as_uint(t[4 * a + 2]), __float_as_uint(t[4 * a + 3]), 0x0040);
+        __byte_perm(__float_as_uint(t[2 * a + 1].x), __float_as_uint(t[2 * a + 1].y), 0x0040);
     w[a] = __byte_perm(lo, hi, 0x5410);
   }
 }
@@ -127,84 +164,100 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(2 * D) int8_append_kernel(Int8AppendArgs a) {
+__global__ void __launch_bounds__(2 * D) int8_append_kernel(Int8AppendArgs a, Plan plan) {
   using F = Int8Fmt<D>;
   constexpr int CH = D / 16, HALF = kPage * CH;  // threads per tensor
-  const long long u = blockIdx.x / a.n_kv_heads;
-  const int h = blockIdx.x % a.n_kv_heads;
+  const int parts = (a.n_kv_heads + plan.heads - 1) / plan.heads;
+  const int u = blockIdx.x / parts, h0 = (blockIdx.x - u * parts) * plan.heads;
+  const int h1 = min(h0 + plan.heads, a.n_kv_heads);
   if (blockIdx.x == 0)
     flag_lengths(a.cu, a.lens_old, a.num_seqs, a.total, a.max_new, a.max_blocks, a.err);
   PageUnit p;
-  if (!page_unit(a.cu, a.lens_old, a.num_seqs, a.total, a.max_new, a.max_blocks, u, p)) return;
+  if (!page_unit(a.cu, a.lens_old, a.num_seqs, a.total, a.max_new, a.max_blocks, u, plan.per_token, p)) return;
   const int tid = threadIdx.x;
   const bool is_v = tid >= HALF;
   const int r = is_v ? tid - HALF : tid;
   const int i = r & 3, c = (r >> 2) % CH, t4 = r / (4 * CH), tok = 4 * t4 + i;
+  const int pos = p.page * kPage + tok;
+  const bool valid = pos >= p.t_lo && pos < p.t_hi;
+  const int64_t row = p.row + (pos - p.t_lo);
+  const uint16_t* src = (is_v ? a.v + row * a.v_t : a.k + row * a.k_t) + 16 * c;
+  const int64_t step = is_v ? a.v_h : a.k_h;
+  auto load = [&](int h, uint32_t (&x)[8]) {
+    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+    if (valid) {
+      const uint4* s4 = reinterpret_cast<const uint4*>(src + h * step);
+      if (plan.wide) {
+        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]),
+                       "=r"(x[6]), "=r"(x[7])
+                     : "l"(s4));
+        return;
+      }
+      lo = __ldcs(s4);
+      hi = __ldcs(s4 + 1);
+    }
+    x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
+    x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+  };
+  uint32_t next[8];
+  load(h0, next);
   const int pid = __ldg(a.block_tables + static_cast<int64_t>(p.s) * a.max_blocks + p.page);
   if (pid < 0 || pid >= a.num_pages) {
     if (tid == 0) set_err(a.err, TKV_ERR_BAD_PAGE);
     return;
   }
-  const int pos = p.page * kPage + tok;
-  const bool valid = pos >= p.t_lo && pos < p.t_hi;
-  uint32_t x2[8];
+  uint8_t* blk = a.pool + (static_cast<int64_t>(pid) * a.n_kv_heads + h0) * F::BYTES;
+  for (int h = h0; h < h1; ++h, blk += F::BYTES) {
+    uint32_t x2[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) x2[e] = 0u;
-  if (valid) {
-    const int64_t row = p.row + (pos - p.t_lo);
-    const uint16_t* src = is_v ? a.v + row * a.v_t + h * a.v_h : a.k + row * a.k_t + h * a.k_h;
-    const uint4* s4 = reinterpret_cast<const uint4*>(src + 16 * c);
-    const uint4 lo = __ldg(s4), hi = __ldg(s4 + 1);
-    x2[0] = lo.x, x2[1] = lo.y, x2[2] = lo.z, x2[3] = lo.w;
-    x2[4] = hi.x, x2[5] = hi.y, x2[6] = hi.z, x2[7] = hi.w;
-  }
-  // the row's largest magnitude: its CH chunks are lanes 4 c + i
-  float m = amax16<BF16>(x2);
+    for (int e = 0; e < 8; ++e) x2[e] = next[e];
+    if (h + 1 < h1) load(h + 1, next);
+    // the row's largest magnitude: its CH chunks are lanes 4 c + i
+    float m = amax16<BF16>(x2);
 #pragma unroll
-  for (int o = 4; o < 4 * CH; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float d = __fdiv_rn(m, 127.f);
-  const bool finite = m <= FLT_MAX;  // false for NaN too
-  const bool some = finite && d >= FLT_MIN;
-  const float inv = some ? __fdiv_rn(1.f, d) : 0.f;
-  if (!some) d = finite ? 0.f : __uint_as_float(0x7fffffffu);
-  float x[16];
+    for (int o = 4; o < 4 * CH; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float d = __fdiv_rn(m, 127.f);
+    const bool finite = m <= FLT_MAX;  // false for NaN too
+    const bool some = finite && d >= FLT_MIN;
+    const float inv = some ? __fdiv_rn(1.f, d) : 0.f;
+    if (!some) {
+      d = finite ? 0.f : __uint_as_float(0x7fffffffu);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float2 f = unpack2<BF16>(some ? x2[e] : 0u);
-    x[2 * e] = f.x;
-    x[2 * e + 1] = f.y;
-  }
-  uint32_t w[4];
-  quantise16(x, d, inv, w);
-  uint8_t* blk = a.pool + (static_cast<int64_t>(pid) * a.n_kv_heads + h) * F::BYTES;
-  if (valid && c == 0)
-    reinterpret_cast<float*>(blk + F::SCALE_OFF)[2 * tok + (is_v ? 1 : 0)] = d;
-  if (!is_v) {
-    if (valid)
-      *reinterpret_cast<uint4*>(blk + int8_k_unit(tok, c)) = make_uint4(w[0], w[1], w[2], w[3]);
-    return;
-  }
-  // words (channels 4 a ..) of four tokens -> this thread's unit: channels 16 c
-  // + 4 i .., tokens 4 t4 ..
-  quad_transpose(w, i);
-  byte_transpose(w);
-  uint8_t* dst = blk + F::V_OFF + int8_v_unit(c / 2, 4 * (c & 1) + i, t4);
-  const int q0 = p.page * kPage + 4 * t4;
-  if (q0 >= p.t_lo && q0 + 4 <= p.t_hi) {
-    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
+      for (int e = 0; e < 8; ++e) x2[e] = 0u;
+    }
+    uint32_t w[4];
+    quantise16<BF16>(x2, d, inv, w);
+    if (valid && c == 0)
+      reinterpret_cast<float*>(blk + F::SCALE_OFF)[2 * tok + (is_v ? 1 : 0)] = d;
+    if (!is_v) {
+      if (valid)
+        *reinterpret_cast<uint4*>(blk + int8_k_unit(tok, c)) = make_uint4(w[0], w[1], w[2], w[3]);
+      continue;
+    }
+    // words (channels 4 a ..) of four tokens -> this thread's unit: channels 16 c
+    // + 4 i .., tokens 4 t4 ..
+    quad_transpose(w, i);
+    byte_transpose(w);
+    uint8_t* dst = blk + F::V_OFF + int8_v_unit(c / 2, 4 * (c & 1) + i, t4);
+    const int q0 = p.page * kPage + 4 * t4;
+    if (q0 >= p.t_lo && q0 + 4 <= p.t_hi) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      if (q0 + b < p.t_lo || q0 + b >= p.t_hi) continue;
+      for (int b = 0; b < 4; ++b) {
+        if (q0 + b < p.t_lo || q0 + b >= p.t_hi) continue;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) dst[4 * j + b] = static_cast<uint8_t>(w[j] >> (8 * b));
+        for (int j = 0; j < 4; ++j) dst[4 * j + b] = static_cast<uint8_t>(w[j] >> (8 * b));
+      }
     }
   }
 }
 
 // OUT: TKV_F32, TKV_F16 or TKV_BF16
 template <int OUT>
-__device__ __forceinline__ void store16(void* out, int64_t at, const uint32_t (&w)[4], float s) {
+__device__ __forceinline__ void store16(void* out, int64_t at, const uint32_t (&w)[4], float s,
+                                        bool wide) {
   float x[16];
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
@@ -224,25 +277,31 @@ __device__ __forceinline__ void store16(void* out, int64_t at, const uint32_t (&
       dst[e] = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
   } else {
     uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at);
+    uint32_t y[8];
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-      dst[e] = make_uint4(pack2<OUT == TKV_BF16>(x[8 * e], x[8 * e + 1]),
-                          pack2<OUT == TKV_BF16>(x[8 * e + 2], x[8 * e + 3]),
-                          pack2<OUT == TKV_BF16>(x[8 * e + 4], x[8 * e + 5]),
-                          pack2<OUT == TKV_BF16>(x[8 * e + 6], x[8 * e + 7]));
+    for (int e = 0; e < 8; ++e) y[e] = pack2<OUT == TKV_BF16>(x[2 * e], x[2 * e + 1]);
+    if (wide) {  // whole 32-byte sectors
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(y[0]),
+                   "r"(y[1]), "r"(y[2]), "r"(y[3]), "r"(y[4]), "r"(y[5]), "r"(y[6]), "r"(y[7])
+                   : "memory");
+    } else {
+      dst[0] = make_uint4(y[0], y[1], y[2], y[3]);
+      dst[1] = make_uint4(y[4], y[5], y[6], y[7]);
+    }
   }
 }
 
 template <int D, int OUT>
-__global__ void __launch_bounds__(2 * D) int8_read_kernel(Int8ReadArgs a) {
+__global__ void __launch_bounds__(2 * D) int8_read_kernel(Int8ReadArgs a, Plan plan) {
   using F = Int8Fmt<D>;
   constexpr int CH = D / 16, HALF = kPage * CH;
-  const long long u = blockIdx.x / a.n_kv_heads;
-  const int h = blockIdx.x % a.n_kv_heads;
+  const int parts = (a.n_kv_heads + plan.heads - 1) / plan.heads;
+  const int u = blockIdx.x / parts, h0 = (blockIdx.x - u * parts) * plan.heads;
+  const int h1 = min(h0 + plan.heads, a.n_kv_heads);
   if (blockIdx.x == 0)
     flag_lengths(a.cu, a.starts, a.num_seqs, a.total, a.max_tokens, a.max_blocks, a.err);
   PageUnit p;
-  if (!page_unit(a.cu, a.starts, a.num_seqs, a.total, a.max_tokens, a.max_blocks, u, p)) return;
+  if (!page_unit(a.cu, a.starts, a.num_seqs, a.total, a.max_tokens, a.max_blocks, u, plan.per_token, p)) return;
   const int tid = threadIdx.x;
   const bool is_v = tid >= HALF;
   void* const out = is_v ? a.v_out : a.k_out;
@@ -252,55 +311,81 @@ __global__ void __launch_bounds__(2 * D) int8_read_kernel(Int8ReadArgs a) {
   const int pid = __ldg(a.block_tables + static_cast<int64_t>(p.s) * a.max_blocks + p.page);
   const bool ok = pid >= 0 && pid < a.num_pages;
   if (!ok && r == 0) set_err(a.err, TKV_ERR_BAD_PAGE);
-  const uint8_t* blk =
-      a.pool + (static_cast<int64_t>(ok ? pid : 0) * a.n_kv_heads + h) * F::BYTES;
-  const uint4 q = __ldg(reinterpret_cast<const uint4*>(
-      is_v ? blk + F::V_OFF + int8_v_unit(c / 2, 4 * (c & 1) + i, t4) : blk + int8_k_unit(tok, c)));
-  float s = __ldg(reinterpret_cast<const float*>(blk + F::SCALE_OFF) + 2 * tok + (is_v ? 1 : 0));
-  uint32_t w[4] = {q.x, q.y, q.z, q.w};
-  if (is_v) {
-    byte_transpose(w);
-    quad_transpose(w, i);
-  }
-  if (!ok) {
-    s = 0.f;
-    w[0] = w[1] = w[2] = w[3] = 0x80808080u;
-  }
+  const uint8_t* const blk =
+      a.pool + (static_cast<int64_t>(ok ? pid : 0) * a.n_kv_heads + h0) * F::BYTES;
+  const uint8_t* src = blk + (is_v ? F::V_OFF + int8_v_unit(c / 2, 4 * (c & 1) + i, t4) : int8_k_unit(tok, c));
+  const uint8_t* scale = blk + F::SCALE_OFF + 8 * tok + (is_v ? 4 : 0);
   const int pos = p.page * kPage + tok;
-  if (pos < p.t_lo || pos >= p.t_hi) return;
-  const int64_t row = p.row + (pos - p.t_lo);
-  store16<OUT>(out, (row * a.n_kv_heads + h) * D + 16 * c, w, s);
+  const bool valid = pos >= p.t_lo && pos < p.t_hi;
+  int64_t at = (static_cast<int64_t>(p.row + (pos - p.t_lo)) * a.n_kv_heads + h0) * D + 16 * c;
+  uint4 q = __ldcs(reinterpret_cast<const uint4*>(src));
+  float s = __ldcs(reinterpret_cast<const float*>(scale));
+  for (int h = h0; h < h1; ++h, at += D) {
+    uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    float sh = s;
+    if (h + 1 < h1) {
+      src += F::BYTES;
+      scale += F::BYTES;
+      q = __ldcs(reinterpret_cast<const uint4*>(src));
+      s = __ldcs(reinterpret_cast<const float*>(scale));
+    }
+    if (is_v) {
+      byte_transpose(w);
+      quad_transpose(w, i);
+    }
+    if (!ok) {
+      sh = 0.f;
+      w[0] = w[1] = w[2] = w[3] = 0x80808080u;
+    }
+    if (valid) store16<OUT>(out, at, w, sh, plan.wide);
+  }
 }
 
-// CTAs of a call over `total` tokens of `num_seqs` sequences; 0: too many
-unsigned int grid_of(int total, int num_seqs, int heads) {
-  const long long n = (static_cast<long long>(total) / kPage + 2ll * num_seqs) * heads;
+// CTAs of a call over `total` tokens; 0: more than a grid has.  A CTA takes one
+// head while that leaves CTAs enough for one round of the GPU's 16 x 148; beyond,
+// up to 8, which spares the later heads their search for the sequence and keeps
+// loads in flight (64 x 2048 tokens of 8 heads, 1, 2, 4 and 8 heads a CTA: append
+// 432, 315, 257 and 228 us, read 224, 156, 138 and 140 us).
+unsigned int plan_grid(int total, int num_seqs, int n_heads, Plan& plan) {
+  const long long pages = static_cast<long long>(total) / kPage + 2ll * num_seqs;
+  plan.per_token = total < pages;
+  const long long units = plan.per_token ? total : pages;
+  plan.heads = static_cast<int>(
+      std::max<long long>(1, std::min<long long>({8ll, n_heads, units * n_heads / 2368})));
+  const long long n = units * ((n_heads + plan.heads - 1) / plan.heads);
   return n > INT_MAX ? 0u : static_cast<unsigned int>(n);
 }
 
 }  // namespace
 
 int launch_int8_append(const Int8AppendArgs& a, int head_dim, bool bf16, cudaStream_t stream) {
-  const unsigned int grid = grid_of(a.total, a.num_seqs, a.n_kv_heads);
+  Plan plan;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
+                       static_cast<uintptr_t>(2 * (a.k_t | a.k_h | a.v_t | a.v_h));
+  plan.wide = (at & 31) == 0;
+  const unsigned int grid = plan_grid(a.total, a.num_seqs, a.n_kv_heads, plan);
   if (grid == 0) return TKV_INVALID_ARGUMENT;
   if (head_dim == 128) {
     if (bf16)
-      int8_append_kernel<128, true><<<grid, 256, 0, stream>>>(a);
+      int8_append_kernel<128, true><<<grid, 256, 0, stream>>>(a, plan);
     else
-      int8_append_kernel<128, false><<<grid, 256, 0, stream>>>(a);
+      int8_append_kernel<128, false><<<grid, 256, 0, stream>>>(a, plan);
   } else {
     if (bf16)
-      int8_append_kernel<64, true><<<grid, 128, 0, stream>>>(a);
+      int8_append_kernel<64, true><<<grid, 128, 0, stream>>>(a, plan);
     else
-      int8_append_kernel<64, false><<<grid, 128, 0, stream>>>(a);
+      int8_append_kernel<64, false><<<grid, 128, 0, stream>>>(a, plan);
   }
   return cudaGetLastError() == cudaSuccess ? TKV_OK : TKV_BACKEND_ERROR;
 }
 
 int launch_int8_read(const Int8ReadArgs& a, int head_dim, int out_dtype, cudaStream_t stream) {
-  const unsigned int grid = grid_of(a.total, a.num_seqs, a.n_kv_heads);
+  Plan plan;
+  plan.wide =
+      ((reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.v_out)) & 31) == 0;
+  const unsigned int grid = plan_grid(a.total, a.num_seqs, a.n_kv_heads, plan);
   if (grid == 0) return TKV_INVALID_ARGUMENT;
-#define TKV_READ(D, OUT) int8_read_kernel<D, OUT><<<grid, 2 * D, 0, stream>>>(a)
+#define TKV_READ(D, OUT) int8_read_kernel<D, OUT><<<grid, 2 * D, 0, stream>>>(a, plan)
   if (head_dim == 128) {
     if (out_dtype == TKV_F32) TKV_READ(128, TKV_F32);
     else if (out_dtype == TKV_F16) TKV_READ(128, TKV_F16);
