@@ -15,11 +15,11 @@
 // whatever its longest sequence; a CTA finds its sequence by a 32-way search.
 // Where that is more than the tokens there are (a decode step), sequence s owns
 // the units from cu[s] on: a page that is touched holds a token of the range.
-// 256 sequences of one token, 8 heads: @TOKENUNIT us against 19.9.
+// 256 sequences of one token, 8 heads: append 14.5 us against 19.9.
 //
 // Both kernels are bound by memory: 2 bytes a channel on the dense side, 1 and a
 // scale on the paged one.  64 x 2048 tokens of 8 heads of 128 channels: append
-// @APP us, read @READ us.
+// 167 us (4.9 TB/s), read 139 us (5.9 TB/s).
 #include <limits.h>
 
 #include <algorithm>
@@ -53,10 +53,12 @@ __device__ __forceinline__ int find_seq(const int32_t* cu, int num_seqs, long lo
   return lo;
 }
 
+constexpr int kAhead = 3;  // heads of the append kernel's rows in shared memory
+
 // How a launch is cut up.  heads: kv heads a CTA takes one after another;
 // per_token: the numbering of page units; wide: the dense rows and their strides
 // are multiples of 32 bytes, so 16 channels are one access of a whole sector
-// (64 x 2048 tokens of 8 heads: read @WIDE).
+// (ragged prefixes of 16 sequences read: 98 -> 88 us).
 struct Plan {
   int heads;
   bool per_token, wide;
@@ -96,40 +98,45 @@ __device__ __forceinline__ void flag_lengths(const int32_t* cu, const int32_t* l
 
 // Codes (+ 128) of x[0..15] for scale d, packed four to a word.  The sum x/d +
 // 1.5 2^23 + 128 rounds to a whole number, halves to even (its bias is even),
-// and the low byte of its bits is the stored byte.  x * (1/d) is off by less
-// than 2^-15 from x/d, so only a remainder close to one half is checked, in
-// exact arithmetic: x - k d is exact in f32 (x has 11 bits or fewer and |x - k
-// d| < d, a multiple of d's last bit).
+// and the low byte of its bits is the stored byte.  inv_lo <= 1/d <= inv_hi, so
+// where the sums with both agree (each a multiply-add, rounded once), the sum with
+// x/d itself, which lies between them, rounds to the same.  The others (x/d within
+// 2^-15 of a half; with bf16 values, half of a row's largest is such) are
+// corrected in exact arithmetic: x - k d is exact in f32 (x has 11 bits or fewer
+// and |x - k d| < 2 d, a multiple of d's last bit).  The correction is right for
+// every value, so a warp makes it for the pairs where any of its lanes needs it.
 template <bool BF16>
-__device__ __forceinline__ void quantise16(const uint32_t (&x2)[8], float d, float inv,
-                                           uint32_t (&w)[4]) {
+__device__ __forceinline__ void quantise16(const uint32_t (&x2)[8], float d, float inv_lo,
+                                           float inv_hi, uint32_t (&w)[4]) {
   constexpr float kMagic = 12582912.f + kInt8Bias;
-  const float2 inv2 = make_float2(inv, inv), up2 = make_float2(kMagic, kMagic);
-  const float2 down2 = make_float2(-kMagic, -kMagic), minus2 = make_float2(-1.f, -1.f);
-  float2 t[8];
-  float worst = 0.f;
+  const float2 lo2 = make_float2(inv_lo, inv_lo), hi2 = make_float2(inv_hi, inv_hi);
+  const float2 up2 = make_float2(kMagic, kMagic), minus2 = make_float2(-1.f, -1.f);
+  float2 t[8], differ = make_float2(0.f, 0.f);  // a bit for each pair
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float2 x = unpack2<BF16>(x2[e]);
-    t[e] = ffma2(x, inv2, up2);
-    const float2 k = fadd2(t[e], down2);
-    const float2 r = ffma2(x, inv2, ffma2(k, minus2, make_float2(0.f, 0.f)));
-    worst = fmaxf(worst, fmaxf(fabsf(r.x), fabsf(r.y)));
+    t[e] = ffma2(x, lo2, up2);
+    const float2 gap = ffma2(t[e], minus2, ffma2(x, hi2, up2));  // exact: 0, 1 or -1
+    const float2 bit = make_float2(1 << e, 1 << e);
+    differ = ffma2(ffma2(gap, gap, make_float2(0.f, 0.f)), bit, differ);
   }
-  if (worst > 0.4999f) {
-    const float h = 0.5f * d;
+  const uint32_t near_half = __reduce_or_sync(
+      0xffffffffu, static_cast<uint32_t>(differ.x) | static_cast<uint32_t>(differ.y));
+  if (near_half) {
+    const uint32_t h = __float_as_uint(0.5f * d);
     auto fix = [&](float x, float& v) {
-      const float k = __fsub_rn(v, kMagic);
-      const float r = __fmaf_rn(-k, d, x);
-      const bool odd = __float_as_uint(v) & 1u;
-      if (r > h || (r == h && odd)) v += 1.f;
-      if (r < -h || (r == -h && odd)) v -= 1.f;
+      const float r = __fmaf_rn(__fsub_rn(kMagic, v), d, x);
+      // at a remainder of exactly d/2 an odd code gives way
+      const float most = __uint_as_float(h - (__float_as_uint(v) & 1u));
+      if (fabsf(r) > most) v += copysignf(1.f, r);
     };
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float2 x = unpack2<BF16>(x2[e]);
-      fix(x.x, t[e].x);
-      fix(x.y, t[e].y);
+      if (near_half >> e & 1) {
+        const float2 x = unpack2<BF16>(x2[e]);
+        fix(x.x, t[e].x);
+        fix(x.y, t[e].y);
+      }
     }
   }
 #pragma unroll
@@ -141,30 +148,25 @@ __device__ __forceinline__ void quantise16(const uint32_t (&x2)[8], float d, flo
   }
 }
 
-// max |x| of 16 packed values; a NaN among them gives NaN
+// bits of max |x| of 16 packed values as f32; a NaN among them gives a NaN's,
+// which as whole numbers are above infinity's
 template <bool BF16>
-__device__ __forceinline__ float amax16(const uint32_t (&p)[8]) {
-  if constexpr (BF16) {
-    __nv_bfloat162 m = __habs2(*reinterpret_cast<const __nv_bfloat162*>(&p[0]));
+__device__ __forceinline__ uint32_t amax16(const uint32_t (&p)[8]) {
+  uint32_t m = p[0];  // signs are left to the last step
 #pragma unroll
-    for (int i = 1; i < 8; ++i)
-      m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&p[i])));
-    return __bfloat162float(__hmax_nan(m.x, m.y));
-  } else {
-    __half2 m = __habs2(*reinterpret_cast<const __half2*>(&p[0]));
-#pragma unroll
-    for (int i = 1; i < 8; ++i)
-      m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&p[i])));
-    return __half2float(__hmax_nan(m.x, m.y));
+  for (int i = 1; i < 8; ++i) {
+    if constexpr (BF16)
+      asm("max.NaN.xorsign.abs.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(p[i]));
+    else
+      asm("max.NaN.xorsign.abs.f16x2 %0, %0, %1;" : "+r"(m) : "r"(p[i]));
   }
-}
-
-__device__ __forceinline__ float max_nan(float a, float b) {
-  return a != a ? a : (b != b ? b : fmaxf(a, b));
+  const float2 f = unpack2<BF16>(m & 0x7fff7fffu);
+  return max(__float_as_uint(f.x), __float_as_uint(f.y));
 }
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(2 * D) int8_append_kernel(Int8AppendArgs a, Plan plan) {
+__global__ void __launch_bounds__(2 * D, 1024 / (2 * D))
+    int8_append_kernel(Int8AppendArgs a, Plan plan) {
   using F = Int8Fmt<D>;
   constexpr int CH = D / 16, HALF = kPage * CH;  // threads per tensor
   const int parts = (a.n_kv_heads + plan.heads - 1) / plan.heads;
@@ -180,54 +182,75 @@ __global__ void __launch_bounds__(2 * D) int8_append_kernel(Int8AppendArgs a, Pl
   const int i = r & 3, c = (r >> 2) % CH, t4 = r / (4 * CH), tok = 4 * t4 + i;
   const int pos = p.page * kPage + tok;
   const bool valid = pos >= p.t_lo && pos < p.t_hi;
-  const int64_t row = p.row + (pos - p.t_lo);
-  const uint16_t* src = (is_v ? a.v + row * a.v_t : a.k + row * a.k_t) + 16 * c;
+  if (!__any_sync(0xffffffffu, valid)) return;  // a warp whose tokens are others'
+  // A warp brings the rows of its 128 / CH tokens to shared memory itself, kAhead
+  // heads ahead: 64 pieces of 16 bytes a head, lane l copies pieces l and l + 32.
+  // Piece q of token 4 t + i lies at q ^ (i & 1 | (i & 2) << 1), so the eight
+  // lanes that read at once are in different banks.
+  __shared__ __align__(16) uint4 stage[kAhead][2 * D / 32][64];
+  const int warp = tid / 32, lane = tid & 31;
+  const uint16_t* src[2];
+  uint32_t to[2], bytes[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int piece = lane + 32 * e, t = piece / (2 * CH), q = piece % (2 * CH);
+    const int at = p.page * kPage + (r & ~31) / CH + t;
+    const bool in = at >= p.t_lo && at < p.t_hi;
+    const int64_t row = in ? p.row + (at - p.t_lo) : p.row;
+    src[e] = (is_v ? a.v + row * a.v_t + h0 * a.v_h : a.k + row * a.k_t + h0 * a.k_h) + 8 * q;
+    to[e] = smem_u32(&stage[0][warp][2 * CH * t + (q ^ ((t & 1) | (t & 2) << 1))]);
+    bytes[e] = in ? 16u : 0u;  // the rest is filled with zeros
+  }
   const int64_t step = is_v ? a.v_h : a.k_h;
-  auto load = [&](int h, uint32_t (&x)[8]) {
-    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-    if (valid) {
-      const uint4* s4 = reinterpret_cast<const uint4*>(src + h * step);
-      if (plan.wide) {
-        asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]),
-                       "=r"(x[6]), "=r"(x[7])
-                     : "l"(s4));
-        return;
-      }
-      lo = __ldcs(s4);
-      hi = __ldcs(s4 + 1);
+  auto fetch = [&](int h) {  // h heads from the first one
+    if (h0 + h < h1) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                         to[e] + (h % kAhead) * static_cast<uint32_t>(sizeof(stage[0]))),
+                     "l"(src[e] + h * step), "r"(bytes[e])
+                     : "memory");
     }
-    x[0] = lo.x, x[1] = lo.y, x[2] = lo.z, x[3] = lo.w;
-    x[4] = hi.x, x[5] = hi.y, x[6] = hi.z, x[7] = hi.w;
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  uint32_t next[8];
-  load(h0, next);
+#pragma unroll
+  for (int h = 0; h < kAhead - 1; ++h) fetch(h);
   const int pid = __ldg(a.block_tables + static_cast<int64_t>(p.s) * a.max_blocks + p.page);
   if (pid < 0 || pid >= a.num_pages) {
-    if (tid == 0) set_err(a.err, TKV_ERR_BAD_PAGE);
+    if (valid) set_err(a.err, TKV_ERR_BAD_PAGE);
+    asm volatile("cp.async.wait_all;" ::: "memory");
     return;
   }
   uint8_t* blk = a.pool + (static_cast<int64_t>(pid) * a.n_kv_heads + h0) * F::BYTES;
-  for (int h = h0; h < h1; ++h, blk += F::BYTES) {
-    uint32_t x2[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x2[e] = next[e];
-    if (h + 1 < h1) load(h + 1, next);
+  const int mine = 2 * CH * ((r & 31) / (4 * CH) * 4 + i), turn = (i & 1) | (i & 2) << 1;
+  for (int h = 0; h < h1 - h0; ++h, blk += F::BYTES) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory");
+    __syncwarp();  // every lane's pieces are there, and the stage before is read
+    fetch(h + kAhead - 1);
+    const uint4* from = stage[h % kAhead][warp] + mine;
+    const uint4 lo = from[(2 * c) ^ turn], hi = from[(2 * c + 1) ^ turn];
+    uint32_t x2[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     // the row's largest magnitude: its CH chunks are lanes 4 c + i
-    float m = amax16<BF16>(x2);
+    uint32_t bits = amax16<BF16>(x2);
 #pragma unroll
-    for (int o = 4; o < 4 * CH; o <<= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    for (int o = 4; o < 4 * CH; o <<= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+    const float m = __uint_as_float(bits);
     float d = __fdiv_rn(m, 127.f);
     const bool finite = m <= FLT_MAX;  // false for NaN too
     const bool some = finite && d >= FLT_MIN;
-    const float inv = some ? __fdiv_rn(1.f, d) : 0.f;
+    // the approximation of 1/d (normal, as d is) is off by one unit in the last
+    // place at most, so two either way enclose it
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(some ? d : 1.f));
+    const float inv_lo = __uint_as_float(__float_as_uint(inv) - 2u);
+    const float inv_hi = __uint_as_float(__float_as_uint(inv) + 2u);
     if (!some) {
       d = finite ? 0.f : __uint_as_float(0x7fffffffu);
 #pragma unroll
       for (int e = 0; e < 8; ++e) x2[e] = 0u;
     }
     uint32_t w[4];
-    quantise16<BF16>(x2, d, inv, w);
+    quantise16<BF16>(x2, d, inv_lo, inv_hi, w);
     if (valid && c == 0)
       reinterpret_cast<float*>(blk + F::SCALE_OFF)[2 * tok + (is_v ? 1 : 0)] = d;
     if (!is_v) {
@@ -308,15 +331,17 @@ __global__ void __launch_bounds__(2 * D) int8_read_kernel(Int8ReadArgs a, Plan p
   if (out == nullptr) return;  // whole warps: HALF is a multiple of 32
   const int r = is_v ? tid - HALF : tid;
   const int i = r & 3, c = (r >> 2) % CH, t4 = r / (4 * CH), tok = 4 * t4 + i;
-  const int pid = __ldg(a.block_tables + static_cast<int64_t>(p.s) * a.max_blocks + p.page);
-  const bool ok = pid >= 0 && pid < a.num_pages;
-  if (!ok && r == 0) set_err(a.err, TKV_ERR_BAD_PAGE);
-  const uint8_t* const blk =
-      a.pool + (static_cast<int64_t>(ok ? pid : 0) * a.n_kv_heads + h0) * F::BYTES;
-  const uint8_t* src = blk + (is_v ? F::V_OFF + int8_v_unit(c / 2, 4 * (c & 1) + i, t4) : int8_k_unit(tok, c));
-  const uint8_t* scale = blk + F::SCALE_OFF + 8 * tok + (is_v ? 4 : 0);
   const int pos = p.page * kPage + tok;
   const bool valid = pos >= p.t_lo && pos < p.t_hi;
+  if (!__any_sync(0xffffffffu, valid)) return;  // a warp whose tokens are others'
+  const int pid = __ldg(a.block_tables + static_cast<int64_t>(p.s) * a.max_blocks + p.page);
+  const bool ok = pid >= 0 && pid < a.num_pages;
+  if (!ok && valid) set_err(a.err, TKV_ERR_BAD_PAGE);
+  const uint8_t* const blk =
+      a.pool + (static_cast<int64_t>(ok ? pid : 0) * a.n_kv_heads + h0) * F::BYTES;
+  const uint8_t* src =
+      blk + (is_v ? F::V_OFF + int8_v_unit(c / 2, 4 * (c & 1) + i, t4) : int8_k_unit(tok, c));
+  const uint8_t* scale = blk + F::SCALE_OFF + 8 * tok + (is_v ? 4 : 0);
   int64_t at = (static_cast<int64_t>(p.row + (pos - p.t_lo)) * a.n_kv_heads + h0) * D + 16 * c;
   uint4 q = __ldcs(reinterpret_cast<const uint4*>(src));
   float s = __ldcs(reinterpret_cast<const float*>(scale));
@@ -342,16 +367,18 @@ __global__ void __launch_bounds__(2 * D) int8_read_kernel(Int8ReadArgs a, Plan p
 }
 
 // CTAs of a call over `total` tokens; 0: more than a grid has.  A CTA takes one
-// head while that leaves CTAs enough for one round of the GPU's 16 x 148; beyond,
-// up to 8, which spares the later heads their search for the sequence and keeps
-// loads in flight (64 x 2048 tokens of 8 heads, 1, 2, 4 and 8 heads a CTA: append
-// 432, 315, 257 and 228 us, read 224, 156, 138 and 140 us).
+// head while that leaves no more than one round of the append kernel's 4 x 148
+// CTAs; beyond, up to 8, which spares the later heads their search for the
+// sequence and keeps loads in flight.  64 x 2048 tokens of 8 heads with 1, 2, 4
+// and 8 heads a CTA: append 432, 315, 257 and 228 us, read 224, 156, 138 and 140
+// us (the loads then went through registers); 8 x 512 tokens with one head and
+// with 4: append 13.7 and 10.7 us, read 9.2 and 7.5 us.
 unsigned int plan_grid(int total, int num_seqs, int n_heads, Plan& plan) {
   const long long pages = static_cast<long long>(total) / kPage + 2ll * num_seqs;
   plan.per_token = total < pages;
   const long long units = plan.per_token ? total : pages;
   plan.heads = static_cast<int>(
-      std::max<long long>(1, std::min<long long>({8ll, n_heads, units * n_heads / 2368})));
+      std::max<long long>(1, std::min<long long>({8ll, n_heads, units * n_heads / 592})));
   const long long n = units * ((n_heads + plan.heads - 1) / plan.heads);
   return n > INT_MAX ? 0u : static_cast<unsigned int>(n);
 }
@@ -360,9 +387,7 @@ unsigned int plan_grid(int total, int num_seqs, int n_heads, Plan& plan) {
 
 int launch_int8_append(const Int8AppendArgs& a, int head_dim, bool bf16, cudaStream_t stream) {
   Plan plan;
-  const uintptr_t at = reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) |
-                       static_cast<uintptr_t>(2 * (a.k_t | a.k_h | a.v_t | a.v_h));
-  plan.wide = (at & 31) == 0;
+  plan.wide = false;
   const unsigned int grid = plan_grid(a.total, a.num_seqs, a.n_kv_heads, plan);
   if (grid == 0) return TKV_INVALID_ARGUMENT;
   if (head_dim == 128) {
