@@ -15,37 +15,35 @@ namespace tkv {
 namespace {
 
 constexpr int kSlots = 148 * 3;  // resident CTAs of the decode kernel
-constexpr int kMinRun = 8;       // pages: one step of each of a CTA's warps
-constexpr int kMaxRun = 64;
-constexpr int kMaxRuns = 512;
-// The workspace starts with the counters of this many (sequence, kv head) pairs,
-// whatever the call's sizes, so calls of different sizes that take turns with one
-// workspace never write partials over each other's counters.  Calls with more
-// pairs have no need to split.
-constexpr int kMaxPairs = 65536;
-constexpr size_t kCounterBytes = kMaxPairs * sizeof(unsigned int);
+// The workspace starts with the decode kernel's counters, in a place that does not
+// depend on the call's sizes, so calls of different sizes that take turns with one
+// workspace never write partials over each other's counters.
+constexpr size_t kCounterBytes = 2048;
+static_assert(kCounterBytes >= kSlots * sizeof(unsigned int), "");
 
 size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
-// How decode contexts of up to these sizes are cut: runs of equal length that
-// give every resident CTA one, but not shorter than a step of each warp nor
-// longer than kMaxRun pages.
+// one CTA for every place on the GPU, or for every step where there are fewer
 void decode_splits(Int8Splits& sp, int num_seqs, int num_kv_heads, int grp, int max_q, int max_len) {
-  const long long pages = (static_cast<long long>(max_len) + kPage - 1) / kPage;
-  const long long pairs = static_cast<long long>(num_seqs) * num_kv_heads, total = pages * pairs;
-  long long run = (total + kSlots - 1) / kSlots;
-  run = std::min<long long>(kMaxRun, std::max<long long>(kMinRun, (run + kMinRun - 1) / kMinRun * kMinRun));
-  run = std::max(run, pairs > kMaxPairs ? pages : (pages + kMaxRuns - 1) / kMaxRuns);
-  sp.pages = static_cast<int>(run);
-  sp.n = static_cast<int>(std::max<long long>(1, (pages + run - 1) / run));
+  const long long steps = (static_cast<long long>(max_len) + kInt8StepPages * kPage - 1) / (kInt8StepPages * kPage);
+  const long long pairs = static_cast<long long>(num_seqs) * num_kv_heads;
+  sp.ctas = static_cast<int>(std::max<long long>(1, pairs >= kSlots ? kSlots : std::min<long long>(kSlots, pairs * steps)));
+  // contexts of 4 steps or less are not cut: 8 heads of 64 channels, 512 tokens: 7.5
+  // us whole, 9.0 us in 4 parts; 8 heads of 128, 2048 tokens in parts of one
+  // step 9.2 us, of four 11.8 us
+  sp.least = steps <= 4 ? static_cast<int>(std::max<long long>(1, steps)) : 1;
   sp.rows = static_cast<int>(std::min<long long>(kInt8DecodeRows, static_cast<long long>(max_q) * grp));
 }
 
+int row_block(const Int8Splits& sp) { return sp.rows <= 8 ? 8 : 16; }
+
+size_t decode_ml_bytes(const Int8Splits& sp) {
+  return round256(static_cast<size_t>(2 * sp.ctas) * row_block(sp) * 8);
+}
+
 // bytes of the decode kernel's partials
-size_t decode_bytes(const Int8Splits& sp, int num_seqs, int num_kv_heads, int head_dim) {
-  const size_t pairs = static_cast<size_t>(num_seqs) * num_kv_heads;
-  const size_t rb = sp.rows <= 8 ? 8 : 16;
-  return sp.n > 1 ? round256(pairs * sp.n * rb * 8) + pairs * sp.n * rb * head_dim * 4 : 0;
+size_t decode_bytes(const Int8Splits& sp, int head_dim) {
+  return decode_ml_bytes(sp) + round256(static_cast<size_t>(2 * sp.ctas) * row_block(sp) * head_dim * 4);
 }
 
 constexpr int kMinTiles = 8;    // 64-token tiles of a run
@@ -80,7 +78,7 @@ size_t int8_attend_workspace(int num_seqs, int num_q_heads, int num_kv_heads, in
                              int max_q, int max_len) {
   Int8Splits sp;
   decode_splits(sp, num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_q, max_len);
-  size_t n = kCounterBytes + round256(decode_bytes(sp, num_seqs, num_kv_heads, head_dim));
+  size_t n = kCounterBytes + decode_bytes(sp, head_dim);
   if (has_chunks(num_q_heads / num_kv_heads, max_q)) {
     Int8ChunkSplits cs;
     chunk_splits(cs, num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_q, max_len);
@@ -96,9 +94,9 @@ int launch_int8_attend(const Int8AttendArgs& a, int head_dim, void* workspace, s
   const size_t pairs = static_cast<size_t>(a.num_seqs) * a.n_kv_heads;
   sp.count = static_cast<unsigned int*>(workspace);
   uint8_t* ws = static_cast<uint8_t*>(workspace) + kCounterBytes;
-  uint8_t* chunk_ws = ws + round256(decode_bytes(sp, a.num_seqs, a.n_kv_heads, head_dim));
+  uint8_t* chunk_ws = ws + decode_bytes(sp, head_dim);
   sp.part_ml = reinterpret_cast<float*>(ws);
-  sp.part_o = reinterpret_cast<float*>(ws + round256(pairs * sp.n * (sp.rows <= 8 ? 8 : 16) * 8));
+  sp.part_o = reinterpret_cast<float*>(ws + decode_ml_bytes(sp));
   const int st = launch_int8_decode(a, sp, head_dim, stream);
   if (st != TKV_OK || !has_chunks(a.grp, a.max_q)) return st;
   Int8ChunkSplits cs;

@@ -16,14 +16,17 @@ constexpr float kInt8LazyWeight = 1024.f;  // 2^kInt8Lazy
 constexpr float kInt8WeightUp = 32.f;
 constexpr int kInt8DecodeRows = 16;     // most rows of the decode kernel
 
-// Runs of a context.  Decode: `n` runs at most per (sequence, kv head), each of
-// `pages` pages or less (ns = min(n, ceil(pages of the sequence / pages)) are
-// used); `rows` is the largest row count the launch may meet.
+// Decode kernel: the steps (8 pages of a (sequence, kv head)) of all its sequences
+// in one row, cut into ranges of equal length, one CTA each.  A pair whose steps
+// lie in several CTAs' ranges is joined by the last of them to finish: partial
+// 2 i + 1 is CTA i's last pair, begun there, 2 i its first, begun earlier.
+constexpr int kInt8StepPages = 8;
 struct Int8Splits {
-  int n, pages, rows;
-  unsigned int* count;  // [pairs], zero between launches
-  float* part_ml;       // [pair][run][row block][2]  (m in log2 units, l)
-  float* part_o;        // [pair][run][row block][D]  normalised
+  int ctas, least;      // CTAs at most; steps of a CTA at least
+  int rows;             // the largest row count the launch may meet
+  unsigned int* count;  // [ctas], zero between launches: of the pair begun there
+  float* part_ml;       // [2 ctas][row block][2]  (m in log2 units, l)
+  float* part_o;        // [2 ctas][row block][D]  normalised
 };
 
 // Chunk kernel: an item is a 256-row tile of a (sequence, kv head).  CTA i < whole
