@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem[];
   // Barriers (tile i counted from the CTA's first), of stage i % 4:
   //   kready          K stored (128 producer arrivals)
-  //   vready          V and the scales stored (128 producer arrivals)
+  //   vready          V and the scales stored (128 and 32 arrivals)
   //   kfree, vfree    S, O += P V of the tile done (a commit per warpgroup)
   // and of warpgroup w, [2 w + i % 2]:
   //   sdone           S done (commit)
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   if (ctid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&kready[i], kProducers);
-      mbar_init(&vready[i], kProducers);
+      mbar_init(&vready[i], kProducers + 32);
       mbar_init(&kfree[i], wgs);
       mbar_init(&vfree[i], wgs);
     }
@@ -335,28 +335,27 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   constexpr uint32_t idS = umma::idesc_f16(kRows, kTN, false);
   constexpr uint32_t idO = umma::idesc_f16(kRows, D, false);
 
+  // Of the warps that read pages, lane l holds the id of page 32 w + l of the run
+  // (window w: 8 tiles), checked against the pool, and of the next window as loaded:
+  // no load of codes waits for a load of the table
+  const int32_t* const bt = a.block_tables + static_cast<int64_t>(s) * a.max_blocks;
+  const uint8_t* const pool_h = a.pool + static_cast<int64_t>(h) * F::BYTES;
+  const int64_t page_stride = static_cast<int64_t>(a.n_kv_heads) * F::BYTES;
+  auto load_ids = [&](int w) {
+    // the table may have dropped what the window passed
+    const int p = j_lo * kTP + 32 * w + lane, n_pages = (kv_end + kPage - 1) / kPage;
+    return p >= kv_lo / kPage && p < n_pages ? __ldg(bt + p) : 0;
+  };
+  auto checked = [&](int id) {
+    if (id >= 0 && id < a.num_pages) return id;
+    set_err(a.err, TKV_ERR_BAD_PAGE);
+    return 0;  // read in bounds; the sequence's output is not meaningful
+  };
+
   if (ctid >= kSoftmax && ctid < kSoftmax + kProducers) {
     // ============================ producers ============================
     regs_down<kRegsProducer>();
     const int tid = ctid - kSoftmax;
-    const bool scales = tid < 32;  // this warp brings the scales: lane l tokens 2 l, 2 l + 1
-    const int32_t* bt = a.block_tables + static_cast<int64_t>(s) * a.max_blocks;
-    const int n_pages = (kv_end + kPage - 1) / kPage;
-    const uint8_t* const pool_h = a.pool + static_cast<int64_t>(h) * F::BYTES;
-    const int64_t page_stride = static_cast<int64_t>(a.n_kv_heads) * F::BYTES;
-    const int first_page = kv_lo / kPage;  // the table may have dropped what the window passed
-    // lane l holds the id of page 32 w + l of the run (window w: 8 tiles), checked
-    // against the pool, and of the next window as loaded: no load of codes waits
-    // for a load of the table
-    auto load_ids = [&](int w) {
-      const int p = j_lo * kTP + 32 * w + lane;
-      return p >= first_page && p < n_pages ? __ldg(bt + p) : 0;
-    };
-    auto checked = [&](int id) {
-      if (id >= 0 && id < a.num_pages) return id;
-      set_err(a.err, TKV_ERR_BAD_PAGE);
-      return 0;  // read in bounds; the sequence's output is not meaningful
-    };
     int ids = checked(load_ids(0)), ids_next = load_ids(1);
     // K unit of this thread in page PSTEP i + tid / UNITS: slot x % 16 of chunk
     // x / 16 (x = tid % UNITS): 8 lanes read 128 bytes and fill one core matrix.
@@ -368,9 +367,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     const int vu = x >> 5, vg = (lane >> 1) & 7, vt = (lane & 1) + 2 * (lane >> 4);
     const uint32_t v_src = F::V_OFF + int8_v_unit(vu, vg, vt);
     const uint32_t v_dst = 4 * vu * (16 * kTN) + (vt >> 1) * 128 + vg * 16 + (vt & 1) * 8;
-    int pid[UPT], spid = 0;
+    int pid[UPT];
     uint4 kr[UPT], vr[UPT];
-    float4 sr = make_float4(0.f, 0.f, 0.f, 0.f);  // key, value scale of two tokens
     auto fetch_ids = [&](int i) {  // the pages of tile i of the run, in order of i
       if (i > 0 && (i & 7) == 0) {
         ids = checked(ids_next);
@@ -379,7 +377,6 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
 #pragma unroll
       for (int k = 0; k < UPT; ++k)
         pid[k] = __shfl_sync(0xffffffffu, ids, (i & 7) * kTP + PSTEP * k + pg0);
-      if (scales) spid = __shfl_sync(0xffffffffu, ids, (i & 7) * kTP + (lane >> 3));
     };
     auto load_k = [&]() {
 #pragma unroll
@@ -390,10 +387,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
 #pragma unroll
       for (int i = 0; i < UPT; ++i)
         vr[i] = __ldg(reinterpret_cast<const uint4*>(pool_h + pid[i] * page_stride + v_src));
-      if (scales)
-        sr = __ldg(reinterpret_cast<const float4*>(pool_h + spid * page_stride + F::SCALE_OFF) + (lane & 7));
     };
-    float vinv = 0x1p126f;  // 2^-E
     if (nj > 0) {
       fetch_ids(0);
       load_k();
@@ -431,20 +425,6 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
           *reinterpret_cast<uint2*>(vd + e * (16 * kTN) + (PSTEP * k + pg0) * 256) = make_uint2(lo, hi);
         }
       }
-      if (scales) {
-        // tokens that no row of the CTA sees count for nothing
-        const int t0 = (j_lo + i) * kTN + 2 * lane;
-        const float v0 = t0 < kv_end && t0 >= kv_lo ? sr.y : 0.f;
-        const float v1 = t0 + 1 < kv_end && t0 + 1 >= kv_lo ? sr.w : 0.f;
-        float top = fmaxf(fmaxf(v0, v1), 0.f);
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-        if (top * vinv > 1.f) vinv = int8_scale_inverse(top);
-        *reinterpret_cast<float2*>(ks_s + st * kTN + 2 * lane) = make_float2(sr.x, sr.z);
-        *reinterpret_cast<float2*>(vs_s + st * kTN + 2 * lane) =
-            make_float2(v0 * vinv * kInt8WeightUp, v1 * vinv * kInt8WeightUp);
-        if (lane == 0) vi_s[st] = vinv;
-      }
       umma::fence_smem_to_async();
       mbar_arrive(&vready[st]);
       if (more) load_v();
@@ -453,6 +433,39 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     // ============================ an MMA warp ============================
     regs_down<kRegsMma>();
     const int w = warp - (kSoftmax + kProducers) / 32;  // its softmax warpgroup
+    if (w == 2 && nj > 0) {
+      // ---- the scales: lane l those of tokens 2 l, 2 l + 1 of a tile ----
+      int ids = checked(load_ids(0)), ids_next = load_ids(1);
+      auto load = [&](int i) {  // in order of i
+        if (i > 0 && (i & 7) == 0) {
+          ids = checked(ids_next);
+          ids_next = load_ids((i >> 3) + 1);
+        }
+        const int id = __shfl_sync(0xffffffffu, ids, (i & 7) * kTP + (lane >> 3));
+        return __ldg(reinterpret_cast<const float4*>(pool_h + id * page_stride + F::SCALE_OFF) + (lane & 7));
+      };
+      float vinv = 0x1p126f;  // 2^-E
+      float4 next = load(0);
+      for (int i = 0; i < nj; ++i) {
+        const int st = i % kStages;
+        const float4 sr = next;  // key, value scale of two tokens
+        if (i + 1 < nj) next = load(i + 1);
+        // tokens that no row of the CTA sees count for nothing
+        const int t0 = (j_lo + i) * kTN + 2 * lane;
+        const float v0 = t0 < kv_end && t0 >= kv_lo ? sr.y : 0.f;
+        const float v1 = t0 + 1 < kv_end && t0 + 1 >= kv_lo ? sr.w : 0.f;
+        float top = fmaxf(fmaxf(v0, v1), 0.f);
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        if (top * vinv > 1.f) vinv = int8_scale_inverse(top);
+        if (i >= kStages && !mbar_wait_near(&vfree[st], ((i / kStages) & 1) ^ 1, a.err)) break;
+        *reinterpret_cast<float2*>(ks_s + st * kTN + 2 * lane) = make_float2(sr.x, sr.z);
+        *reinterpret_cast<float2*>(vs_s + st * kTN + 2 * lane) =
+            make_float2(v0 * vinv * kInt8WeightUp, v1 * vinv * kInt8WeightUp);
+        if (lane == 0) vi_s[st] = vinv;
+        mbar_arrive(&vready[st]);
+      }
+    }
     if (w == 3) prefetch_q<D>(a, sp, blockIdx.x + kInt8ChunkSMs, lane);
     if (lane == 0 && w < wgs && nj > 0) {
       bool ok = true;
