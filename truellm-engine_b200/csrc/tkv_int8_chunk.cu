@@ -39,6 +39,7 @@ namespace {
 constexpr int kRows = 128;       // rows of a softmax warpgroup (the MMA's M)
 constexpr int kTN = 64;          // tokens per tile
 constexpr int kStages = 4;       // K and V buffers
+constexpr int kPrefetch = 3;     // tiles that L2 is ahead of the producers
 constexpr int kTP = kTN / kPage; // pages per tile
 constexpr int kSoftmax = 256, kProducers = 128;
 constexpr int kCtaThreads = kSoftmax + kProducers + 128;  // the MMA warps' warpgroup: two idle
@@ -444,12 +445,22 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         const int id = __shfl_sync(0xffffffffu, ids, (i & 7) * kTP + (lane >> 3));
         return __ldg(reinterpret_cast<const float4*>(pool_h + id * page_stride + F::SCALE_OFF) + (lane & 7));
       };
+      // tile j (later than i, not by a window or more) into L2, a page a lane
+      auto prefetch_tile = [&](int i, int j) {
+        const int id = __shfl_sync(0xffffffffu, (j >> 3) == (i >> 3) ? ids : ids_next,
+                                   (j & 7) * kTP + (lane & 3));
+        if (lane < kTP && j < nj && id >= 0 && id < a.num_pages)
+          asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" ::"l"(pool_h + id * page_stride),
+                       "r"(F::BYTES));
+      };
+      for (int j = 1; j < kPrefetch; ++j) prefetch_tile(0, j);
       float vinv = 0x1p126f;  // 2^-E
       float4 next = load(0);
       for (int i = 0; i < nj; ++i) {
         const int st = i % kStages;
         const float4 sr = next;  // key, value scale of two tokens
         if (i + 1 < nj) next = load(i + 1);
+        prefetch_tile(i + 1, i + kPrefetch);
         // tokens that no row of the CTA sees count for nothing
         const int t0 = (j_lo + i) * kTN + 2 * lane;
         const float v0 = t0 < kv_end && t0 >= kv_lo ? sr.y : 0.f;
