@@ -26,6 +26,9 @@
 //     buffers, like the reference's TrueBuffer): append (the reshape_and_cache
 //     slot) and decode (the paged_attention_v1/v2 slot), throwing
 //     std::invalid_argument / std::runtime_error on a non-OK status.
+//   * PagedInt8Cache -- the paged int8 cache (a view over a caller-owned pool):
+//     append, read and attend (decode steps, draft tokens and prefill chunks in one
+//     call); RopeAxes -- rotary positions with several axes.  The same exceptions.
 #pragma once
 
 #include <cstddef>
@@ -234,6 +237,85 @@ class PagedKiviCache {
       throw_on(TKV_INVALID_ARGUMENT, what);
   }
   tkv_cache_t c_{};
+};
+
+// ---------------------------------------------------------------- paged int8 cache
+// A view over the caller's pool (num_pages x n_kv_heads x page_bytes, zeroed once);
+// block tables, lengths and offsets as the C entry points take them.
+class PagedInt8Cache {
+ public:
+  PagedInt8Cache(void* pool, int num_pages, int n_kv_heads, int head_dim) {
+    if (page_bytes(head_dim) == 0) throw_on(TKV_INVALID_ARGUMENT, "PagedInt8Cache: head_dim");
+    c_.pool = static_cast<uint8_t*>(pool);
+    c_.num_pages = num_pages;
+    c_.n_kv_heads = n_kv_heads;
+    c_.head_dim = head_dim;
+  }
+  // Bytes of one page of one kv head; 0 for a head_dim that has no layout.
+  static size_t page_bytes(int head_dim) { return tkv_int8_page_bytes(head_dim); }
+  const tkv_int8_cache_t& c() const { return c_; }
+
+  // strides: token and head stride of k, then of v, in elements
+  void append(const void* k, const void* v, int dtype, const int64_t strides[4],
+              const int32_t* cu_new, const int32_t* seq_lens_old, const int32_t* block_tables,
+              int max_blocks_per_seq, int num_seqs, int total_new_tokens, int max_new_tokens,
+              int* err_flag, cudaStream_t stream) const {
+    throw_on(tkv_int8_append(&c_, k, v, dtype, strides, cu_new, seq_lens_old, block_tables,
+                             max_blocks_per_seq, num_seqs, total_new_tokens, max_new_tokens,
+                             err_flag, stream),
+             "PagedInt8Cache::append");
+  }
+  void read(void* k_out, void* v_out, int out_dtype, const int32_t* block_tables,
+            int max_blocks_per_seq, const int32_t* starts, const int32_t* cu, int num_seqs,
+            int total_tokens, int max_tokens, int* err_flag, cudaStream_t stream) const {
+    throw_on(tkv_int8_read(&c_, k_out, v_out, out_dtype, block_tables, max_blocks_per_seq, starts,
+                           cu, num_seqs, total_tokens, max_tokens, err_flag, stream),
+             "PagedInt8Cache::read");
+  }
+  size_t workspace_bytes(int num_seqs, int num_q_heads, int max_q_tokens,
+                         int max_context_len) const {
+    return tkv_int8_attend_workspace_bytes(num_seqs, num_q_heads, c_.n_kv_heads, c_.head_dim,
+                                           max_q_tokens, max_context_len);
+  }
+  // q_stride: token and head stride of q in elements
+  void attend(const void* q, int q_dtype, const int64_t q_stride[2], void* out, int out_dtype,
+              const int32_t* cu_q, const int32_t* block_tables, int max_blocks_per_seq,
+              const int32_t* seq_lens, int num_seqs, int num_q_heads, int total_q_tokens,
+              int max_q_tokens, int max_context_len, int window, float scale, void* workspace,
+              size_t workspace_bytes, int* err_flag, cudaStream_t stream) const {
+    throw_on(tkv_int8_attend(&c_, q, q_dtype, q_stride, out, out_dtype, cu_q, block_tables,
+                             max_blocks_per_seq, seq_lens, num_seqs, num_q_heads, total_q_tokens,
+                             max_q_tokens, max_context_len, window, scale, workspace,
+                             workspace_bytes, err_flag, stream),
+             "PagedInt8Cache::attend");
+  }
+
+ private:
+  tkv_int8_cache_t c_{};
+};
+
+// ---------------------------------------------------------------- rotary positions
+// sections[a]: frequency pairs of axis a; rotary_dim = twice their sum.
+class RopeAxes {
+ public:
+  RopeAxes(int rotary_dim, double theta, const int32_t* sections, int n_axes, int order,
+           int pairing) {
+    throw_on(tkv_rope_plan_init(&p_, rotary_dim, theta, sections, n_axes, order, pairing),
+             "RopeAxes");
+  }
+  // strides: token and head stride of q, k, q_out, k_out in elements; k may be null
+  void apply(const void* q, const void* k, void* q_out, void* k_out, int dtype, int num_q_heads,
+             int num_k_heads, int head_dim, int n_tokens, const int64_t strides[8],
+             const int32_t* positions, int64_t axis_stride, bool inverse,
+             cudaStream_t stream) const {
+    throw_on(tkv_rope_axes(&p_, q, k, q_out, k_out, dtype, num_q_heads, num_k_heads, head_dim,
+                           n_tokens, strides, positions, axis_stride, inverse ? 1 : 0, stream),
+             "RopeAxes::apply");
+  }
+  const tkv_rope_plan_t& plan() const { return p_; }
+
+ private:
+  tkv_rope_plan_t p_{};
 };
 
 // ---------------------------------------------------------------- page allocator

@@ -674,3 +674,82 @@ def test_a_pool_past_4_gib(ops, cuda):
         a = ops.int8_attend(cache, q[r], t32([0, m], cuda), bt_t, t32([n], cuda))
         c = ops.int8_attend(small, q[r], t32([0, m], cuda), t32([[0, 1, 2]], cuda), t32([n], cuda))
         assert torch.equal(a, c)
+
+
+# --------------------------------------------------------------------------
+# how work is shared out
+# --------------------------------------------------------------------------
+@pytest.mark.parametrize("H", [5, 8, 20])
+@pytest.mark.parametrize("D,dt", [(64, "f16"), (128, "bf16")])
+def test_several_heads_a_cta(ops, cuda, H, D, dt):
+    """Long calls, in which a CTA takes several kv heads one after another (and a
+    last CTA fewer), leave the bytes and values of short ones."""
+    lens = [0, 4093, 1, 2500, 16, 31]
+    b = Batch(ops, cuda, [0] * len(lens), lens, H, D, DT[dt], seed=H)
+    b.fill()
+    whole = b.pool.clone()
+    b.pool.fill_(255)
+    for i, n in enumerate(lens):
+        for at in range(0, n, 60):
+            m = min(60, n - at)
+            rows = slice(int(b.cu_all[i]) + at, int(b.cu_all[i]) + at + m)
+            ops.int8_append(b.cache, b.k[rows], b.v[rows], t32([0, m], cuda), t32([at], cuda),
+                            b.bt_t[i:i + 1])
+    assert torch.equal(whole, b.pool)
+    T, z = sum(lens), t32([0] * len(lens), cuda)
+    ko, vo = ops.int8_read(b.cache, b.bt_t, z, t32(b.cu_all, cuda), T, dtype=BF16)
+    # outputs that start 16 bytes off a sector
+    raw = [torch.zeros(T * H * D + 8, dtype=BF16, device=cuda) for _ in range(2)]
+    k1, v1 = (x[8:].view(T, H, D) for x in raw)
+    ops.int8_read(b.cache, b.bt_t, z, t32(b.cu_all, cuda), T, k_out=k1, v_out=v1)
+    assert torch.equal(k1, ko) and torch.equal(v1, vo)
+    for i, n in enumerate(lens):
+        for at in range(0, n, 999):
+            m = min(60, n - at)
+            rows = slice(int(b.cu_all[i]) + at, int(b.cu_all[i]) + at + m)
+            kk, vv = ops.int8_read(b.cache, b.bt_t[i:i + 1], t32([at], cuda), t32([0, m], cuda), m,
+                                   dtype=BF16)
+            assert torch.equal(kk, ko[rows]) and torch.equal(vv, vo[rows])
+
+
+def test_one_token_of_many_sequences(ops, cuda):
+    """A decode step's append and read-back: more sequences than tokens / 16."""
+    B, H, D = 700, 2, 64
+    rng = np.random.default_rng(5)
+    old = rng.integers(0, 40, B)
+    new = (rng.random(B) < 0.8).astype(int)
+    b = Batch(ops, cuda, old, new, H, D, BF16, seed=5)
+    b.fill()
+    want = b.pool.clone()
+    last = torch.tensor(b.cu_all[1:][new > 0] - 1, device=cuda, dtype=torch.long)
+    pages, slots = b.bt[np.arange(B), np.maximum(b.lens - 1, 0) // PAGE], (b.lens - 1) % PAGE
+    kc, vc, s = unpack(want.cpu().numpy(), D)
+    for other in (True, False):  # another token's rows first
+        k, v = (x[last].flip(-1) * 3 if other else x[last] for x in (b.k, b.v))
+        ops.int8_append(b.cache, k, v, t32(b.cu, cuda), t32(old, cuda), b.bt_t, max_new_tokens=1)
+        assert torch.equal(b.pool, want) != other
+    ko, vo = ops.int8_read(b.cache, b.bt_t, t32(old, cuda), t32(b.cu, cuda), int(new.sum()),
+                           max_tokens=1, dtype=F32)
+    for j, i in enumerate(np.flatnonzero(new)):
+        p, t = pages[i], slots[i]
+        for h in range(H):
+            assert np.array_equal(f64(ko[j, h]), np.float64(np.float32(kc[p, h, t]) * s[p, h, t, 0]))
+            assert np.array_equal(f64(vo[j, h]), np.float64(np.float32(vc[p, h, t]) * s[p, h, t, 1]))
+
+
+@pytest.mark.parametrize("D,dt", [(128, "bf16"), (64, "f16")])
+@pytest.mark.parametrize("window", [0, 200])
+def test_decode_ranges_across_sequences(ops, cuda, D, dt, window):
+    """CTAs whose range of the steps begins and ends inside contexts and spans short
+    ones, sequences without tokens and, more than 32 in a row, chunks."""
+    rng = np.random.default_rng(11)
+    old = np.r_[rng.integers(0, 700, 60), [0] * 40, [9000, 1, 0, 2500], rng.integers(0, 300, 100)]
+    new = np.r_[np.ones(60, int), [17] * 40, [1, 0, 1, 1], rng.integers(0, 2, 100)]
+    b = Batch(ops, cuda, old, new, 2, D, DT[dt], seed=9)
+    b.fill()
+    q = b.query(8)
+    err = err_word(cuda)
+    out = b.attend(q, window=window, err=err)
+    b.check(q, out, window=window, rows=3)
+    assert err.item() == 0
+    assert torch.equal(out, b.attend(q, window=window))

@@ -158,3 +158,17 @@ def test_captured_and_on_another_stream(ops, cuda):
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(out[0], ops.rope_axes(q, k, pos, (16, 24, 24))[0])
+
+
+@pytest.mark.parametrize("T", [1023, 1024, 1025, 4099])
+def test_long_calls_turn_as_short_ones_do(ops, cuda, T):
+    """Calls long enough for several tokens a CTA, against calls of 100 tokens."""
+    rng = np.random.default_rng(T)
+    q = torch.randn(T, 5, 72, device=cuda, dtype=torch.bfloat16)
+    k = torch.randn(T, 2, 72, device=cuda, dtype=torch.bfloat16)
+    pos = positions(rng, 2, T, 1 << 20, cuda)
+    got = ops.rope_axes(q, k, pos, (20, 12))
+    for at in range(0, T, 100):
+        s = slice(at, min(T, at + 100))
+        want = ops.rope_axes(q[s], k[s], pos[:, s].contiguous(), (20, 12))
+        assert torch.equal(got[0][s], want[0]) and torch.equal(got[1][s], want[1])

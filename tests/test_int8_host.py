@@ -103,7 +103,7 @@ def test_append_refusals():
                dict(st=(-256, 128, 256, 128))):
         assert call(t=4, **kw) == BAD, kw
     # more CTAs than one grid has
-    assert call(t=2 ** 31 - 1, c=_cache(n_kv_heads=64)) == BAD
+    assert call(t=2 ** 31 - 1, c=_cache(n_kv_heads=256)) == BAD
 
 
 def test_read_refusals():

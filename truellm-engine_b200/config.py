@@ -6,7 +6,7 @@ defaults from include/truellm/config_schema.h:46-50, 66-84, 121-129, 204).
     [inference]                       backend: "cpu" | "ggml" | "cuda"
     [inference.compression.kv_kivi]   enabled, bits, residual_length, (group_size)
     [inference.kv_cache]              type_k / type_v: "f16" | "q8_0" | "q4_0" and,
-                                      for this path, "kivi4" | "kivi2"
+                                      for this path, "kivi4" | "kivi2" | "int8"
     [inference.cuda_engine]           paged_kv_block_size, max_num_blocks,
                                       max_num_seqs, use_megakernel
 
@@ -18,12 +18,13 @@ in the reference a config that enables both (configs/cuda-kivi-compression.toml
 sets use_megakernel = true at :55) builds the pass and never runs it;
 `PathConfig.pass_runs` reports what the config asks for.
 
-Two consumers:
+Three consumers:
 * the per-vector fake-quant pass (KvCompressionPass, kv_compression_pass.cpp
   :29-67): outliers = residual_length, group = 16 when bits == 4 else 8;
 * the paged KIVI cache: selected by type_k/type_v = "kivi4"/"kivi2" (the same
   bit width on both), with G = group_size (default 128) and R =
-  residual_length.
+  residual_length;
+* the paged int8 cache (ops.Int8PagedCache): type_k = type_v = "int8".
 
 `KvCompressionPass` mirrors the reference class over the C ABI: the same
 constructor arguments, `init`, `run`, `enabled`; unsupported parameters
@@ -38,7 +39,7 @@ from dataclasses import dataclass, field
 from pathlib import Path
 from typing import Any, Mapping, Optional, Union
 
-KV_CACHE_TYPES = ("f16", "q8_0", "q4_0", "kivi4", "kivi2")
+KV_CACHE_TYPES = ("f16", "q8_0", "q4_0", "kivi4", "kivi2", "int8")
 
 
 @dataclass
@@ -89,6 +90,8 @@ class PathConfig:
             return None
         if self.paged_kivi:
             return "paged"
+        if self.paged_int8:
+            return None
         return "pass" if self.compression_pass else None
 
     @property
@@ -97,13 +100,18 @@ class PathConfig:
         return self.kv_cache.type_k.startswith("kivi")
 
     @property
+    def paged_int8(self) -> bool:
+        """True when the KV cache is the paged int8 cache."""
+        return self.kv_cache.type_k == "int8"
+
+    @property
     def paged_bits(self) -> int:
         return 4 if self.kv_cache.type_k == "kivi4" else 2
 
     @property
     def compression_pass(self) -> bool:
         """True when the per-vector KIVI pass is built over an fp16 cache."""
-        return self.kv_kivi.enabled and not self.paged_kivi
+        return self.kv_kivi.enabled and not self.paged_kivi and not self.paged_int8
 
     @property
     def pass_runs(self) -> bool:
@@ -170,6 +178,20 @@ def validate(cfg: PathConfig) -> Optional[str]:
     if cfg.paged_kivi != cfg.kv_cache.type_v.startswith("kivi") or (
             cfg.paged_kivi and cfg.kv_cache.type_k != cfg.kv_cache.type_v):
         return "inference.kv_cache: kivi4/kivi2 must be set on both type_k and type_v"
+    if cfg.paged_int8 or cfg.kv_cache.type_v == "int8":
+        if cfg.kv_cache.type_k != cfg.kv_cache.type_v:
+            return "inference.kv_cache: int8 must be set on both type_k and type_v"
+        if cfg.backend != "cuda":
+            return 'inference.kv_cache: int8 needs inference.backend = "cuda"'
+        if cfg.cuda_engine.paged_kv_block_size != 16:
+            return ("inference.cuda_engine.paged_kv_block_size must be 16 with int8 "
+                    "(16-token pages)")
+        if cfg.cuda_engine.use_megakernel:
+            return ("inference.kv_cache: int8 replaces the per-layer cache and attention "
+                    "calls; inference.cuda_engine.use_megakernel must be false")
+        if cfg.kv_kivi.enabled:
+            return ("inference.kv_cache: int8 pages hold codes of their own; "
+                    "inference.compression.kv_kivi must not be enabled")
     if cfg.paged_kivi:
         if cfg.kv_kivi.group_size not in (16, 32, 64, 128):
             return "inference.compression.kv_kivi.group_size must be 16, 32, 64 or 128"

@@ -643,17 +643,17 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
         if (positions.dtype is not torch.int32 or positions.shape != (len(sections), T) or
                 (T > 1 and positions.stride(1) != 1)):
             raise ValueError(f"positions must be an int32 [{len(sections)}, {T}] tensor")
+        if kx is None and k_out is not None:
+            raise ValueError("k_out without k")
+        for o, x in ((q_out, qx), (k_out, kx)):
+            if o is not None and (o.shape != x.shape or o.dtype is not x.dtype or
+                                  _heads("output", o) is not o):
+                raise ValueError("an output must have its input's shape and type, contiguous "
+                                 "channels and strides that are multiples of 8")
         if q_out is None:
             q_out = torch.empty((T, Hq, D), dtype=qx.dtype, device=qx.device)
         if kx is not None and k_out is None:
             k_out = torch.empty(kx.shape, dtype=kx.dtype, device=kx.device)
-        if kx is None and k_out is not None:
-            raise ValueError("k_out without k")
-        for o, x in ((q_out, qx), (k_out, kx)):
-            if x is not None and (o.shape != x.shape or o.dtype is not x.dtype or
-                                  _heads("output", o) is not o):
-                raise ValueError("an output must have its input's shape and type, contiguous "
-                                 "channels and strides that are multiples of 8")
         qst, qos = qx.stride(), q_out.stride()
         Hk, kst, kos = 0, (0, 0), (0, 0)
         if kx is not None:
