@@ -585,6 +585,13 @@ def _heads(name: str, t: torch.Tensor) -> torch.Tensor:
     return t
 
 
+def _like(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A new contiguous tensor of x's shape."""
+    if x.dtype is dtype and x.is_contiguous():
+        return torch.empty_like(x)  # half the host's time of torch.empty
+    return torch.empty(x.shape, dtype=dtype, device=x.device)
+
+
 _I64x2, _I64x4, _I64x8 = C.c_int64 * 2, C.c_int64 * 4, C.c_int64 * 8
 
 
@@ -651,9 +658,9 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
                 raise ValueError("an output must have its input's shape and type, contiguous "
                                  "channels and strides that are multiples of 8")
         if q_out is None:
-            q_out = torch.empty((T, Hq, D), dtype=qx.dtype, device=qx.device)
+            q_out = _like(qx, qx.dtype)
         if kx is not None and k_out is None:
-            k_out = torch.empty(kx.shape, dtype=kx.dtype, device=kx.device)
+            k_out = _like(kx, kx.dtype)
         qst, qos = qx.stride(), q_out.stride()
         Hk, kst, kos = 0, (0, 0), (0, 0)
         if kx is not None:
@@ -772,7 +779,7 @@ def int8_read(cache: Int8PagedCache, block_tables: torch.Tensor, starts: torch.T
         if k_out is None:
             k_out = torch.empty(shape, dtype=dtype, device=cache.pool.device)
         if v_out is None:
-            v_out = torch.empty(shape, dtype=dtype, device=cache.pool.device)
+            v_out = _like(k_out, dtype)
         bt, mb = _table(block_tables, B)
         L.check("tkv_int8_read", L.lib().tkv_int8_read(
             cache._ref, k_out.data_ptr(), v_out.data_ptr(), _DT[dtype], bt, mb,
@@ -826,7 +833,7 @@ def int8_attend(cache: Int8PagedCache, q: torch.Tensor, cu_q: torch.Tensor,
         mq = T if max_q_tokens is None else int(max_q_tokens)
         ml = mb * L.TKV_PAGE_SIZE if max_context_len is None else int(max_context_len)
         if out is None:
-            out = torch.empty((T, Hq, D), dtype=out_dtype or x.dtype, device=x.device)
+            out = _like(x, out_dtype or x.dtype)
         elif out.shape != (T, Hq, D) or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {[T, Hq, D]} tensor")
         if out.dtype not in _HALF:
