@@ -7,7 +7,7 @@
 //                        become exact f16 integers in the K-major operands K
 //                        [64 tokens][D] and V^T [D][64 tokens] (four buffers);
 //                        one of the warps also brings the scales
-//   MMA (2 warps, 1 lane each, one per softmax warpgroup)  S = Q K^T into tensor
+//   MMA (2 warps, one per softmax warpgroup)  S = Q K^T into tensor
 //                        memory (two buffers), O += P V with P read from there
 //   softmax (2 x 4 warps) one thread per query row: score x key scale, online
 //                        softmax, weight x value scale rounded once to f16 and
@@ -433,7 +433,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   } else if (ctid >= kSoftmax + kProducers) {
     // ============================ an MMA warp ============================
     regs_down<kRegsMma>();
-    const int w = warp - (kSoftmax + kProducers) / 32;  // its softmax warpgroup
+    // its softmax warpgroup, known to be one number for the warp
+    const int w = __shfl_sync(0xffffffffu, warp, 0) - (kSoftmax + kProducers) / 32;
     if (w == 2 && nj > 0) {
       // ---- the scales: lane l those of tokens 2 l, 2 l + 1 of a tile ----
       int ids = checked(load_ids(0)), ids_next = load_ids(1);
@@ -478,43 +479,55 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       }
     }
     if (w == 3) prefetch_q<D>(a, sp, blockIdx.x + kInt8ChunkSMs, lane);
-    if (lane == 0 && w < wgs && nj > 0) {
+    if (w < wgs && nj > 0) {
+      // The whole warp runs the loop and one lane issues: what the instructions take
+      // is then known to be the same for the warp and stays in uniform registers
+      // (issued from a loop of one lane, a tile's products took this warp 1300 cycles).
       bool ok = true;
       int last_s = -1, last_o = -1;
       const uint64_t dq = umma::smem_desc(smem_u32(smem + SM::Q_OFF + w * SM::Q_BYTES), 128, 16 * D);
       const uint64_t dk = umma::smem_desc(smem_u32(smem + SM::K_OFF), 128, 16 * D);
       const uint64_t dv = umma::smem_desc(smem_u32(smem + SM::V_OFF), 128, 16 * kTN);
-      const uint32_t tS = tmem + w * SM::TWG, tO = tS + SM::TO;
+      const uint32_t tS = __shfl_sync(0xffffffffu, tmem, 0) + w * SM::TWG, tO = tS + SM::TO;
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait_near(bar, parity, a.err));
+      };
       auto issue_s = [&](int i) {
-        ok = mbar_wait_near(&kready[i % kStages], (i / kStages) & 1, a.err);
+        ok = wait(&kready[i % kStages], (i / kStages) & 1);
         if (!ok) return;
         umma::fence_after_sync();
         const uint64_t d = dk + (i % kStages) * (SM::K_BYTES >> 4);
+        if (umma::elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk)
-          umma::mma_f16(tS + (i & 1) * kTN, dq + 16 * kk, d + 16 * kk, idS, kk > 0);
-        umma::commit(&sdone[2 * w + (i & 1)]);
-        umma::commit(&kfree[i % kStages]);
+          for (int kk = 0; kk < D / 16; ++kk)
+            umma::mma_f16(tS + (i & 1) * kTN, dq + 16 * kk, d + 16 * kk, idS, kk > 0);
+          umma::commit(&sdone[2 * w + (i & 1)]);
+          umma::commit(&kfree[i % kStages]);
+        }
+        __syncwarp();
         last_s = i;
       };
-      ok = mbar_wait_near(qready, 0, a.err);
+      ok = wait(qready, 0);
       if (ok) issue_s(0);
       if (ok && nj > 1) issue_s(1);
       for (int i = 0; ok && i < nj; ++i) {
-        ok = mbar_wait_near(&vready[i % kStages], (i / kStages) & 1, a.err) &&
-             mbar_wait_near(&pready[2 * w + (i & 1)], (i >> 1) & 1, a.err);
+        ok = wait(&vready[i % kStages], (i / kStages) & 1) &&
+             wait(&pready[2 * w + (i & 1)], (i >> 1) & 1);
         if (!ok) break;
         umma::fence_after_sync();
         const uint64_t d = dv + (i % kStages) * (SM::V_BYTES >> 4);
+        if (umma::elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < kTN / 16; ++kk)
-          umma::mma_f16_ta(tO, tS + (i & 1) * kTN + 8 * kk, d + 16 * kk, idO, i > 0 || kk > 0);
-        umma::commit(&odone[2 * w + (i & 1)]);
-        umma::commit(&vfree[i % kStages]);
+          for (int kk = 0; kk < kTN / 16; ++kk)
+            umma::mma_f16_ta(tO, tS + (i & 1) * kTN + 8 * kk, d + 16 * kk, idO, i > 0 || kk > 0);
+          umma::commit(&odone[2 * w + (i & 1)]);
+          umma::commit(&vfree[i % kStages]);
+        }
+        __syncwarp();
         last_o = i;
         if (i + 2 < nj) {
           // S of tile i + 2 overwrites the scores and weights of this one
-          ok = mbar_wait_near(&odone[2 * w + (i & 1)], (i >> 1) & 1, a.err);
+          ok = wait(&odone[2 * w + (i & 1)], (i >> 1) & 1);
           if (ok) issue_s(i + 2);
         }
       }
