@@ -155,19 +155,21 @@ __device__ __forceinline__ void scale_scores(float (&x)[16], const float4* ks4, 
   }
 }
 
-// The weights of a tile's 64 tokens (scores at tensor-memory column ts), every one
-// of which the row sees: 2^(x ra + nm), added to sum, and times the value scales
-// (2^-E 2^5 included) as f16 pairs.  Sixteen tokens at a time, one group's
-// exponentials while the next one's scores are scaled.
+// The weights of a tile's 64 tokens (scores at tensor-memory column ts, positions
+// t ..): 2^(x ra + nm), added to sum, and times the value scales (2^-E 2^5 included)
+// as f16 pairs; MASKED: 0 for tokens outside [pmin, plim].  Sixteen tokens at a
+// time, one group's exponentials while the next one's scores are scaled.
+template <bool MASKED>
 __device__ __forceinline__ void tile_weights(uint32_t ts, const float4* ks4, const float4* vs4,
-                                             float2 ra2, float nm, float2& sum, uint32_t (&pk)[32]) {
+                                             float2 ra2, float nm, int t, int pmin, int plim,
+                                             float2& sum, uint32_t (&pk)[32]) {
   const float2 nm2 = make_float2(nm, nm);
   float x[2][16];
   float2 s1 = make_float2(0.f, 0.f);
   ld16_issue(ts, x[0]);
   wait_ld_of(x[0]);
   ld16_issue(ts + 16, x[1]);
-  scale_scores<false>(x[0], ks4, 0, 0, 0);
+  scale_scores<MASKED>(x[0], ks4, t, pmin, plim);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     float(&y)[16] = x[q & 1];
@@ -179,15 +181,21 @@ __device__ __forceinline__ void tile_weights(uint32_t ts, const float4* ks4, con
     }
     if (q < 3) {
       wait_ld_of(x[(q + 1) & 1]);
-      scale_scores<false>(x[(q + 1) & 1], ks4 + 4 * (q + 1), 0, 0, 0);
+      scale_scores<MASKED>(x[(q + 1) & 1], ks4 + 4 * (q + 1), t + 16 * (q + 1), pmin, plim);
     }
 #pragma unroll
     for (int c = 0; c < 16; c += 4) {
       const float4 v4 = vs4[4 * q + c / 4];
       sum = fadd2(sum, w[c / 2]);
       s1 = fadd2(s1, w[c / 2 + 1]);
-      const float2 w0 = fmul2(w[c / 2], make_float2(v4.x, v4.y));
-      const float2 w1 = fmul2(w[c / 2 + 1], make_float2(v4.z, v4.w));
+      float2 w0 = fmul2(w[c / 2], make_float2(v4.x, v4.y));
+      float2 w1 = fmul2(w[c / 2 + 1], make_float2(v4.z, v4.w));
+      if constexpr (MASKED) {  // whatever the scale holds
+        if (y[c] == -INFINITY) w0.x = 0.f;
+        if (y[c + 1] == -INFINITY) w0.y = 0.f;
+        if (y[c + 2] == -INFINITY) w1.x = 0.f;
+        if (y[c + 3] == -INFINITY) w1.y = 0.f;
+      }
       pk[8 * q + c / 2] = pack_h2(w0.x, w0.y);
       pk[8 * q + c / 2 + 1] = pack_h2(w1.x, w1.y);
     }
@@ -607,13 +615,16 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       const uint32_t tSi = tS + (i & 1) * kTN;
       const float4* ks4 = reinterpret_cast<const float4*>(ks_s + st * kTN);
       const float4* vs4 = reinterpret_cast<const float4*>(vs_s + st * kTN);
-      bool plain = !masked && !fresh && fv == 1.f;
+      bool plain = !fresh && fv == 1.f;
       if (plain) {
         // A pass with the reference as it is: no maximum is taken.  A sum of
         // 2^kInt8Lazy or less shows that no weight has outgrown it.
         float2 sum = make_float2(0.f, 0.f);
         uint32_t pk[32];
-        tile_weights(tSi, ks4, vs4, ra2, -m, sum, pk);
+        if (masked)
+          tile_weights<true>(tSi, ks4, vs4, ra2, -m, t0, pmin, plim, sum, pk);
+        else
+          tile_weights<false>(tSi, ks4, vs4, ra2, -m, 0, 0, 0, sum, pk);
         plain = !__any_sync(0xffffffffu, sum.x + sum.y > kInt8LazyWeight);
         if (plain) {
           l += sum.x + sum.y;
@@ -621,8 +632,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         }
       }
       if (!plain) {
-        // Masked tokens, a first reference, one that has to move, or the value
-        // scales' power of two has: the tile's maximum, O and l brought to the new
+        // A first reference, one that has to move, or the value scales' power of two
+        // has: the tile's maximum, O and l brought to the new
         // reference, then the weights.  (Compact code: it is rare, and instruction
         // fetches cost the CTA's start and end more than its loops.)
         float mx = -INFINITY;
