@@ -46,7 +46,7 @@ size_t decode_bytes(const Int8Splits& sp, int head_dim) {
   return decode_ml_bytes(sp) + round256(static_cast<size_t>(2 * sp.ctas) * row_block(sp) * head_dim * 4);
 }
 
-constexpr int kMinTiles = 8;    // 64-token tiles of a run
+constexpr int kMinTiles = 4;    // 64-token tiles of a run
 
 // How chunk items are cut: those that fill whole rounds of the SMs not at all; the
 // rest (or all, when there are few) into as many runs as leave no SM idle.
