@@ -6,7 +6,9 @@ include/truellm_kivi.h (library: libtruellm_kivi.so, built by build.py):
   ops          kivi_compress / kivi_decompress / kivi_params_supported /
                kivi_compressed_bytes (kivi_cache.cuh), paged_append (the KIVI
                reshape_and_cache), paged_decode (the paged_attention_v1/v2 slot),
-               split partials + merge, chunked prefill, page / ring-row moves
+               split partials + merge, chunked prefill, page / ring-row moves;
+               rope_axes, and the paged int8 cache: Int8PagedCache, int8_append,
+               int8_read, int8_attend
   allocator    PageAllocator / KiviCacheAllocator: the CudaAllocator page pool,
                block tables, fork, evict / reload
   config       KvCompressionPass mapping + config switches (kv_kivi, kv_cache
