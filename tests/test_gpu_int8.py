@@ -753,3 +753,29 @@ def test_decode_ranges_across_sequences(ops, cuda, D, dt, window):
     b.check(q, out, window=window, rows=3)
     assert err.item() == 0
     assert torch.equal(out, b.attend(q, window=window))
+
+
+@pytest.mark.parametrize("n", [1, 3])
+def test_rows_at_odd_strides_and_addresses(ops, cuda, n):
+    """Rows that 16-byte vectors cannot address are copied, a single token's too."""
+    H, D, old = 2, 64, 20
+    b = Batch(ops, cuda, [old], [n], H, D, F16, seed=n)
+    b.fill()
+    want = b.pool.clone()
+    q = b.query(4)
+    out = b.attend(q)
+    for off in (0, 1):
+        raw = torch.zeros(n, 4 * D + 3, dtype=F16, device=cuda)
+        at = lambda x: raw[:, off:off + x[0].numel()].unflatten(1, x.shape[1:]).copy_(x)  # noqa: E731
+        assert torch.equal(b.attend(at(q)), out)
+        b.pool.copy_(want)
+        k, v = at(b.k[old:]), b.v[old:]
+        b.pool[b.bt[0, old // PAGE]] = 3  # the page of the last tokens, but for its first ones
+        ops.int8_append(b.cache, b.k[16:old], b.v[16:old], t32([0, old - 16], cuda), t32([16], cuda),
+                        b.bt_t)
+        ops.int8_append(b.cache, k, v, t32([0, n], cuda), t32([old], cuda), b.bt_t)
+        kc, vc, s = unpack(b.pool.cpu().numpy(), D)
+        kw, vw, sw = unpack(want.cpu().numpy(), D)
+        p, t = b.bt[0, old // PAGE], slice(0, old - 16 + n)
+        for x, y in ((kc, kw), (vc, vw), (s, sw)):
+            assert np.array_equal(x[p][:, t], y[p][:, t])

@@ -172,3 +172,27 @@ def test_long_calls_turn_as_short_ones_do(ops, cuda, T):
         s = slice(at, min(T, at + 100))
         want = ops.rope_axes(q[s], k[s], pos[:, s].contiguous(), (20, 12))
         assert torch.equal(got[0][s], want[0]) and torch.equal(got[1][s], want[1])
+
+
+def test_second_derivative(ops, cuda):
+    """The gradient is linear in what comes back: its own gradient turns forwards."""
+    rng = np.random.default_rng(8)
+    pos = positions(rng, 2, 21, 5000, cuda)
+    q = torch.randn(21, 3, 64, device=cuda, dtype=torch.float16).requires_grad_()
+    v = torch.randn_like(q).requires_grad_()
+    u = torch.randn_like(q)
+    (g,) = torch.autograd.grad(ops.rope_axes(q, None, pos, (20, 12))[0], q, v, create_graph=True)
+    (h,) = torch.autograd.grad(g, v, u)
+    assert torch.equal(h, ops.rope_axes(u, None, pos, (20, 12))[0])
+
+
+@pytest.mark.parametrize("T", [1, 3])
+def test_rows_at_odd_strides_and_addresses(ops, cuda, T):
+    """Rows that 16-byte vectors cannot address are copied, one token's too (whose
+    token stride counts for nothing)."""
+    raw = torch.randn(T, 2 * 64 + 3, device=cuda, dtype=torch.bfloat16)
+    pos = torch.arange(7, 7 + T, device=cuda, dtype=torch.int32)[None]
+    for off in (0, 1):
+        q = raw[:, off:off + 128].unflatten(1, (2, 64))
+        same = q.new_empty(q.shape).copy_(q)
+        assert torch.equal(ops.rope_axes(q, q, pos, (32,))[1], ops.rope_axes(same, None, pos, (32,))[0])

@@ -581,7 +581,8 @@ def _heads(name: str, t: torch.Tensor) -> torch.Tensor:
         raise ValueError(f"{name} must be an fp16 or bf16 [tokens, heads, channels] tensor")
     st, sh, sd = t.stride()
     if sd != 1 or (st | sh) & 7 or t.data_ptr() & 15:
-        return t.contiguous()
+        # (contiguous() would keep the strides of an axis of one, and the address)
+        return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
@@ -689,9 +690,9 @@ class _RopeAxes(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *grads):
         (positions,) = ctx.saved_tensors
-        with torch.no_grad():
-            gq, gk = rope_axes(grads[0], grads[1] if ctx.has_k else None, positions,
-                               *ctx.how, not ctx.inverse, stream=ctx.stream)
+        # (differentiable itself where a second derivative is asked for)
+        gq, gk = rope_axes(grads[0], grads[1] if ctx.has_k else None, positions,
+                           *ctx.how, not ctx.inverse, stream=ctx.stream)
         return gq, gk, None, None, None, None, None, None, None
 
 
