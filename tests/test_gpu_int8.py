@@ -779,3 +779,41 @@ def test_rows_at_odd_strides_and_addresses(ops, cuda, n):
         p, t = b.bt[0, old // PAGE], slice(0, old - 16 + n)
         for x, y in ((kc, kw), (vc, vw), (s, sw)):
             assert np.array_equal(x[p][:, t], y[p][:, t])
+
+
+@pytest.mark.parametrize("D,dt", [(128, "bf16"), (64, "f16")])
+def test_graphs_that_share_a_workspace_and_change_lengths(ops, cuda, D, dt):
+    """A decode call and a call that mixes chunks and decodes, captured on one
+    workspace, replayed in turn with other lengths and shares of the rows."""
+    B, H, Hq = 5, 2, 8
+    b = Batch(ops, cuda, [900, 300, 2000, 64, 1500], [80] * B, H, D, DT[dt], seed=2)
+    b.fill()
+    ws = ops.int8_workspace(B, Hq, H, D, 80, 2100)
+    q1, q2 = (torch.randn(n, Hq, D, device=cuda).to(DT[dt]) for n in (B, 120))
+    lens, cu1, cu2 = t32(b.lens, cuda), t32(range(B + 1), cuda), t32([0, 80, 81, 85, 118, 120], cuda)
+    call = lambda q, cu, n, w: ops.int8_attend(b.cache, q, cu, b.bt_t, lens, max_q_tokens=n,  # noqa: E731
+                                               max_context_len=2100, workspace=w)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(q1, cu1, 1, ws), call(q2, cu2, 80, ws)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for q, cu, n in ((q1, cu1, 1), (q2, cu2, 80)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call(q, cu, n, ws)
+        graphs.append((g, out, q, cu, n))
+    for length, share in (([980, 380, 2080, 144, 1580], [0, 80, 81, 85, 118, 120]),
+                          ([90, 91, 2080, 100, 82], [0, 1, 2, 79, 80, 120]),
+                          ([980, 17, 1, 144, 700], [0, 80, 97, 98, 119, 120])):
+        lens.copy_(t32(length, cuda))
+        cu2.copy_(t32(share, cuda))
+        for g, out, q, cu, n in graphs * 2:
+            out.fill_(3)
+            g.replay()
+            assert torch.equal(out, call(q, cu, n, None))
+        b.lens, b.cu = np.array(length), np.array(share)
+        b.new = np.diff(b.cu)
+        b.old = b.lens - b.new
+        b.check(q2, graphs[1][1], rows=5)

@@ -149,6 +149,9 @@ def test_attend_refusals():
                dict(lens=None), dict(ws=None), dict(q=P + 2), dict(o=P + 8), dict(ws=P + 4),
                dict(st=(1024, 4)), dict(st=(-1024, 128)), dict(wb=need - 1), dict(wb=0)):
         assert call(t=4, **kw) == BAD, kw
+    # more CTAs than one grid has, refused before anything is launched
+    for hq in (2, 8):
+        assert call(t=4, b=65535, hq=hq, mq=1 << 27, mb=1 << 27, ml=1 << 27, wb=1 << 62) == BAD, hq
 
 
 def test_workspace_sizes():

@@ -101,10 +101,14 @@ int launch_int8_attend(const Int8AttendArgs& a, int head_dim, void* workspace, s
   uint8_t* chunk_ws = ws + decode_bytes(sp, head_dim);
   sp.part_ml = reinterpret_cast<float*>(ws);
   sp.part_o = reinterpret_cast<float*>(ws + decode_ml_bytes(sp));
-  const int st = launch_int8_decode(a, sp, head_dim, stream);
-  if (st != TKV_OK || !has_chunks(a.grp, a.max_q)) return st;
   Int8ChunkSplits cs;
   chunk_splits(cs, a.num_seqs, a.n_kv_heads, a.grp, a.max_q, a.max_len);
+  const bool chunks = has_chunks(a.grp, a.max_q);
+  // more CTAs than a grid has (the items beyond `whole` add fewer than 148)
+  if (chunks && static_cast<long long>(pairs) > (INT_MAX - kInt8ChunkSMs) / cs.row_tiles)
+    return TKV_INVALID_ARGUMENT;
+  const int st = launch_int8_decode(a, sp, head_dim, stream);
+  if (st != TKV_OK || !chunks) return st;
   cs.part_ml = reinterpret_cast<float*>(chunk_ws);
   cs.part_o = reinterpret_cast<float*>(
       chunk_ws + round256((pairs * cs.row_tiles - cs.whole) * cs.n * kInt8ChunkRows * 8));

@@ -836,7 +836,6 @@ int launch_t(const Int8AttendArgs& a, const Int8ChunkSplits& sp, cudaStream_t st
   }
   const long long items = static_cast<long long>(a.num_seqs) * a.n_kv_heads * sp.row_tiles;
   const long long ctas = sp.whole + (items - sp.whole) * sp.n, joins = (items - sp.whole) * (kSoftmax / 8);
-  if (items > INT_MAX || ctas > INT_MAX || joins > INT_MAX) return TKV_INVALID_ARGUMENT;
   int8_chunk_kernel<D><<<static_cast<unsigned int>(ctas), kCtaThreads, Sm<D>::BYTES, stream>>>(a, sp);
   if (cudaGetLastError() != cudaSuccess) return TKV_BACKEND_ERROR;
   if (sp.n > 1) {
