@@ -494,9 +494,9 @@ TKV_API int tkv_int8_read(const tkv_int8_cache_t* cache, void* k_out, void* v_ou
  * workspace: tkv_int8_attend_workspace_bytes(...) bytes for the same sizes,
  * 16-byte aligned, zeroed once when it is allocated (every call leaves its
  * counters zero); calls that share one must not overlap on the GPU, but may
- * differ in their sizes if it is large enough for each.  max_q_tokens times the q
- * heads of a kv head must be below 2^30, num_seqs 65535 or less, and num_seqs times n_kv_heads times
- * that in tiles of 256 rows must fit one grid. */
+ * differ in their sizes if it is large enough for each.  num_seqs is 65535 or
+ * less; max_q_tokens times the q heads of a kv head are below 2^30 rows, whose tiles
+ * of 256, times num_seqs times n_kv_heads, must fit one grid. */
 TKV_API size_t tkv_int8_attend_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads,
                                                int head_dim, int max_q_tokens,
                                                int max_context_len);

@@ -27,9 +27,12 @@ size_t round256(size_t x) { return (x + 255) / 256 * 256; }
 
 // one CTA for every place on the GPU, or for every step where there are fewer
 void decode_splits(Int8Splits& sp, int num_seqs, int num_kv_heads, int grp, int max_q, int max_len) {
-  const long long steps = (static_cast<long long>(max_len) + kInt8StepPages * kPage - 1) / (kInt8StepPages * kPage);
+  constexpr int kStep = kInt8StepPages * kPage;  // tokens
+  const long long steps = (static_cast<long long>(max_len) + kStep - 1) / kStep;
   const long long pairs = static_cast<long long>(num_seqs) * num_kv_heads;
-  sp.ctas = static_cast<int>(std::max<long long>(1, pairs >= kSlots ? kSlots : std::min<long long>(kSlots, pairs * steps)));
+  sp.ctas = pairs >= kSlots
+                ? kSlots
+                : static_cast<int>(std::max<long long>(1, std::min<long long>(kSlots, pairs * steps)));
   // contexts of 4 steps or less are not cut: 8 heads of 64 channels, 512 tokens: 7.5
   // us whole, 9.0 us in 4 parts; 8 heads of 128, 2048 tokens in parts of one
   // step 9.2 us, of four 11.8 us
