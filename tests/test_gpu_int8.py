@@ -817,3 +817,23 @@ def test_graphs_that_share_a_workspace_and_change_lengths(ops, cuda, D, dt):
         b.new = np.diff(b.cu)
         b.old = b.lens - b.new
         b.check(q2, graphs[1][1], rows=5)
+
+
+def test_append_at_the_smallest_scales(ops, cuda):
+    """bf16 rows whose scale is the smallest normal float and a little more (or
+    below it, which counts as none), every mantissa of the largest value."""
+    D, n = 64, 4 * 128
+    rng = np.random.default_rng(6)
+    x = rng.integers(-255, 256, (n, D)) * 2.0 ** rng.integers(-7, 1, (n, D))
+    x[:, 0] = np.repeat(np.arange(128, 256), 4)
+    x *= 2.0 ** np.tile([-126, -127, -125, -128], 128)[:, None]
+    t = torch.tensor(x, dtype=torch.float64, device=cuda).to(BF16)[:, None]
+    cache = ops.Int8PagedCache(1, D, n // PAGE)
+    ops.int8_append(cache, t, t.flip(0), t32([0, n], cuda), t32([0], cuda),
+                    t32([list(range(n // PAGE))], cuda))
+    kc, vc, s = unpack(cache.pool.cpu().numpy(), D)
+    want, d = quantise(f64(t))
+    assert (d == 0).any() and (d > 0).any()
+    flat = lambda c: c.transpose(0, 2, 1, 3).reshape(n, -1)  # noqa: E731
+    assert np.array_equal(flat(kc), want[:, 0]) and np.array_equal(flat(vc)[::-1], want[:, 0])
+    assert np.array_equal(flat(s)[:, :1], d[:, 0])

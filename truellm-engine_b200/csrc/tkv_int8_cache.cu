@@ -123,12 +123,12 @@ __device__ __forceinline__ void quantise16(const uint32_t (&x2)[8], float d, flo
   const uint32_t near_half = __reduce_or_sync(
       0xffffffffu, static_cast<uint32_t>(differ.x) | static_cast<uint32_t>(differ.y));
   if (near_half) {
-    const uint32_t h = __float_as_uint(0.5f * d);
     auto fix = [&](float x, float& v) {
       const float r = __fmaf_rn(__fsub_rn(kMagic, v), d, x);
-      // at a remainder of exactly d/2 an odd code gives way
-      const float most = __uint_as_float(h - (__float_as_uint(v) & 1u));
-      if (fabsf(r) > most) v += copysignf(1.f, r);
+      // at a remainder of exactly d/2 an odd code gives way (d/2 itself may lack the
+      // last bit, twice the remainder has it)
+      const float most = __uint_as_float(__float_as_uint(d) - (__float_as_uint(v) & 1u));
+      if (fabsf(r + r) > most) v += copysignf(1.f, r);
     };
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
