@@ -491,10 +491,12 @@ TKV_API int tkv_int8_read(const tkv_int8_cache_t* cache, void* k_out, void* v_ou
  * TKV_ERR_BAD_LENGTH.  A block-table entry outside the pool is flagged
  * TKV_ERR_BAD_PAGE and read as page 0 (that sequence's output is not
  * meaningful).
- * workspace: tkv_int8_attend_workspace_bytes(...) bytes for the same sizes,
- * 16-byte aligned, zeroed once when it is allocated (every call leaves its
- * counters zero); calls that share one must not overlap on the GPU, but may
- * differ in their sizes if it is large enough for each.  num_seqs is 65535 or
+ * workspace: tkv_int8_attend_workspace_bytes(...) bytes for these sizes or
+ * larger ones, 16-byte aligned, zeroed once when it is allocated (every call
+ * leaves its counters zero).  The size never falls when num_seqs, num_q_heads,
+ * max_q_tokens or max_context_len grow (kv heads and head_dim the same), so one
+ * workspace made for the largest serves every smaller call; calls that share one
+ * must not overlap on the GPU.  num_seqs is 65535 or
  * less; max_q_tokens times the q heads of a kv head are below 2^30 rows, whose tiles
  * of 256, times num_seqs times n_kv_heads, must fit one grid. */
 TKV_API size_t tkv_int8_attend_workspace_bytes(int num_seqs, int num_q_heads, int num_kv_heads,

@@ -67,11 +67,18 @@ void chunk_splits(Int8ChunkSplits& sp, int num_seqs, int num_kv_heads, int grp, 
   sp.whole = static_cast<int>(sp.n > 1 ? items - rest : items);
 }
 
-// bytes of the chunk kernel's share of the workspace
-size_t chunk_bytes(const Int8ChunkSplits& sp, int num_seqs, int num_kv_heads, int head_dim) {
-  if (sp.n <= 1) return 0;
-  const size_t items = static_cast<size_t>(num_seqs) * num_kv_heads * sp.row_tiles - sp.whole;
-  const size_t slots = items * sp.n * kInt8ChunkRows;
+// Bytes of the chunk kernel's share of the workspace, for every call of at most these
+// sizes.  A call's own need rises and falls with them (`rest` does), but it never has
+// more parts than the SMs, nor than its items' contexts have runs: rest * n <=
+// min(148, items * tiles / kMinTiles).  That bound only grows.
+size_t chunk_bytes(int num_seqs, int num_kv_heads, int grp, int max_q, int max_len, int head_dim) {
+  const long long runs = (static_cast<long long>(max_len) + 63) / 64 / kMinTiles;
+  if (runs <= 1) return 0;  // no context is cut
+  const long long row_tiles =
+      (static_cast<long long>(max_q) * grp + kInt8ChunkRows - 1) / kInt8ChunkRows;
+  const long long items =
+      std::min<long long>(kInt8ChunkSMs, static_cast<long long>(num_seqs) * num_kv_heads) * row_tiles;
+  const size_t slots = static_cast<size_t>(std::min<long long>(kInt8ChunkSMs, items * runs)) * kInt8ChunkRows;
   return round256(slots * 8) + slots * head_dim * 4;
 }
 
@@ -81,16 +88,14 @@ bool has_chunks(int grp, int max_q) {
 
 }  // namespace
 
+// Never falls when num_seqs, num_q_heads, max_q or max_len grow.
 size_t int8_attend_workspace(int num_seqs, int num_q_heads, int num_kv_heads, int head_dim,
                              int max_q, int max_len) {
   Int8Splits sp;
   decode_splits(sp, num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_q, max_len);
   size_t n = kCounterBytes + decode_bytes(sp, head_dim);
-  if (has_chunks(num_q_heads / num_kv_heads, max_q)) {
-    Int8ChunkSplits cs;
-    chunk_splits(cs, num_seqs, num_kv_heads, num_q_heads / num_kv_heads, max_q, max_len);
-    n += chunk_bytes(cs, num_seqs, num_kv_heads, head_dim);
-  }
+  const int grp = num_q_heads / num_kv_heads;
+  if (has_chunks(grp, max_q)) n += chunk_bytes(num_seqs, num_kv_heads, grp, max_q, max_len, head_dim);
   return n;
 }
 

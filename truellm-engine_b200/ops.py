@@ -797,8 +797,8 @@ def int8_workspace_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int, hea
 
 def int8_workspace(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
                    max_q_tokens: int, max_context_len: int, device="cuda") -> torch.Tensor:
-    """Zeroed workspace of int8_attend calls of up to these sizes (calls that
-    may overlap on the GPU need one each)."""
+    """Zeroed workspace of int8_attend calls of up to these sizes, on a cache of as
+    many kv heads and channels (calls that may overlap on the GPU need one each)."""
     n = int8_workspace_bytes(num_seqs, num_q_heads, num_kv_heads, head_dim, max_q_tokens,
                              max_context_len)
     if n <= 0:
