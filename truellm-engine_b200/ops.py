@@ -630,13 +630,18 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
     "blocks" gives axis a the next sections[a] pairs, "round_robin" deals the
     pairs to the axes in turn; pairing "halves" couples channels (i, i +
     rotary_dim / 2), "adjacent" (2 i, 2 i + 1).  inverse turns back (and is the
-    gradient; calls on tensors that require one are differentiable).  q_out /
-    k_out may be q / k (in place).  Returns (q_out, k_out)."""
+    gradient; calls on tensors that require one are differentiable, and the
+    gradient is computed on the call's stream, in order with what comes before and
+    after it).  q_out / k_out may be q / k (in place).  Returns (q_out, k_out)."""
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         if q_out is not None or k_out is not None:
             raise ValueError("q_out / k_out cannot be given where a gradient is needed")
-        got = _RopeAxes.apply(q, k, positions, tuple(sections), theta, order, pairing,
-                              inverse, stream)
+        dev = q.get_device()
+        _one_device(max(dev, 0), q, k, positions)
+        # autograd runs the backward pass on the stream that is current here, and orders
+        # the gradients that come and go with it
+        with _on(dev, stream):
+            got = _RopeAxes.apply(q, k, positions, tuple(sections), theta, order, pairing, inverse)
         return got if k is not None else (got[0], None)
     dev = q.get_device()
     _one_device(max(dev, 0), q, k, positions, q_out, k_out)
@@ -678,13 +683,12 @@ class _RopeAxes(torch.autograd.Function):
     """A rotation's gradient is the rotation back."""
 
     @staticmethod
-    def forward(ctx, q, k, positions, sections, theta, order, pairing, inverse, stream):
+    def forward(ctx, q, k, positions, sections, theta, order, pairing, inverse):
         ctx.save_for_backward(positions)
         ctx.how = (sections, theta, order, pairing)
-        ctx.inverse, ctx.stream, ctx.has_k = inverse, stream, k is not None
+        ctx.inverse, ctx.has_k = inverse, k is not None
         with torch.no_grad():
-            qo, ko = rope_axes(q, k, positions, sections, theta, order, pairing, inverse,
-                               stream=stream)
+            qo, ko = rope_axes(q, k, positions, sections, theta, order, pairing, inverse)
         return (qo, ko) if k is not None else (qo,)
 
     @staticmethod
@@ -692,8 +696,8 @@ class _RopeAxes(torch.autograd.Function):
         (positions,) = ctx.saved_tensors
         # (differentiable itself where a second derivative is asked for)
         gq, gk = rope_axes(grads[0], grads[1] if ctx.has_k else None, positions,
-                           *ctx.how, not ctx.inverse, stream=ctx.stream)
-        return gq, gk, None, None, None, None, None, None, None
+                           *ctx.how, not ctx.inverse)
+        return gq, gk, None, None, None, None, None, None
 
 
 class Int8PagedCache:
