@@ -1,4 +1,4 @@
-"""rope_axes and autograd: streams."""
+"""rope_axes and autograd: streams and tangents."""
 import pytest
 import torch
 
@@ -57,3 +57,56 @@ def test_a_backward_pass_of_a_given_stream_is_captured(ops, cuda):
     g.replay()
     assert torch.equal(gq, ops.rope_axes(wq, None, pos, SECTIONS, inverse=True)[0])
     assert torch.equal(gk, ops.rope_axes(wk, None, pos, SECTIONS, inverse=True)[0])
+
+
+def test_a_tangent_turns_as_its_input_does(ops, cuda):
+    """Forward mode: of both inputs, of one, and of a call that turns back."""
+    fwd = torch.autograd.forward_ad
+    q, k, pos, tq, tk = inputs(cuda, T=33)
+    how = dict(order="round_robin", pairing="adjacent")
+    turned = lambda t, **kw: ops.rope_axes(t, None, pos, SECTIONS, **how, **kw)[0]  # noqa: E731
+    with fwd.dual_level():
+        dq, dk = fwd.make_dual(q, tq), fwd.make_dual(k, tk)
+        for a, b in ((dq, dk), (dq, k), (q, dk), (dq, None)):
+            got = ops.rope_axes(a, b, pos, SECTIONS, **how)
+            for x, y, t, dual in ((got[0], q, tq, a is dq), (got[1], k, tk, b is dk)):
+                if x is None:
+                    continue
+                p, tangent = fwd.unpack_dual(x)
+                assert torch.equal(p, turned(y))
+                if dual:
+                    assert torch.equal(tangent, turned(t))
+                else:
+                    assert tangent is None or not tangent.any()
+        back = ops.rope_axes(dq, None, pos, SECTIONS, inverse=True, **how)[0]
+        assert torch.equal(fwd.unpack_dual(back).tangent, turned(tq, inverse=True))
+        with torch.no_grad():  # stops gradients, not tangents
+            out = ops.rope_axes(dq, None, pos, SECTIONS, **how)[0]
+        assert torch.equal(fwd.unpack_dual(out).tangent, turned(tq))
+        with pytest.raises(ValueError, match="gradient"):
+            ops.rope_axes(dq, None, pos, SECTIONS, q_out=torch.empty_like(q))
+
+
+def test_functional_transforms_are_refused(ops, cuda):
+    """torch.func hides tensors' memory: an error, and no lost derivative."""
+    q, k, pos, wq, wk = inputs(cuda, T=17)
+    f = lambda a, b: ops.rope_axes(a, b, pos, SECTIONS)  # noqa: E731
+    for call in (lambda: torch.func.vjp(f, q, k), lambda: torch.func.jvp(f, (q, k), (wq, wk)),
+                 lambda: torch.func.grad(lambda a: f(a, k)[0].sum())(q)):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+def test_what_has_no_derivative_refuses_a_tangent(ops, cuda):
+    fwd = torch.autograd.forward_ad
+    cache = ops.Int8PagedCache(2, 128, 2)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=cuda)  # noqa: E731
+    k, q = (torch.randn(5, h, 128, device=cuda, dtype=torch.float16) for h in (2, 8))
+    cu, old, bt = i32([0, 5]), i32([0]), i32([[0, 1]])
+    with fwd.dual_level(), torch.no_grad():
+        with pytest.raises(ValueError, match="tangent"):
+            ops.int8_append(cache, fwd.make_dual(k, k), k, cu, old, bt)
+        with pytest.raises(ValueError, match="tangent"):
+            ops.int8_attend(cache, fwd.make_dual(q, q), cu, bt, i32([5]))
+        ops.int8_append(cache, k, k, cu, old, bt)
+        ops.int8_attend(cache, q, cu, bt, i32([5]))

@@ -18,6 +18,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib as L
 
@@ -596,9 +597,19 @@ def _like(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
 _I64x2, _I64x4, _I64x8 = C.c_int64 * 2, C.c_int64 * 4, C.c_int64 * 8
 
 
+def _differentiated(*ts) -> bool:
+    """A gradient or a tangent of some tensor is wanted."""
+    grad = torch.is_grad_enabled()
+    for t in ts:
+        if t is not None and (grad and t.requires_grad or unpack_dual(t)[1] is not None):
+            return True
+    return False
+
+
 def _no_grad_path(name: str, *ts) -> None:
-    if torch.is_grad_enabled() and any([t.requires_grad for t in ts]):
-        raise ValueError(f"{name} has no gradient: call it under torch.no_grad()")
+    if _differentiated(*ts):
+        raise ValueError(f"{name} has no gradient: call it under torch.no_grad(), on tensors "
+                         "without tangents")
 
 
 @functools.lru_cache(maxsize=64)
@@ -630,10 +641,11 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
     "blocks" gives axis a the next sections[a] pairs, "round_robin" deals the
     pairs to the axes in turn; pairing "halves" couples channels (i, i +
     rotary_dim / 2), "adjacent" (2 i, 2 i + 1).  inverse turns back (and is the
-    gradient; calls on tensors that require one are differentiable, and the
+    gradient).  Calls on tensors that require a gradient, or carry a tangent of
+    torch.autograd.forward_ad, are differentiable (not through torch.func); the
     gradient is computed on the call's stream, in order with what comes before and
-    after it).  q_out / k_out may be q / k (in place).  Returns (q_out, k_out)."""
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    after it.  q_out / k_out may be q / k (in place).  Returns (q_out, k_out)."""
+    if _differentiated(q, k):
         if q_out is not None or k_out is not None:
             raise ValueError("q_out / k_out cannot be given where a gradient is needed")
         dev = q.get_device()
@@ -643,6 +655,12 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
         with _on(dev, stream):
             got = _RopeAxes.apply(q, k, positions, tuple(sections), theta, order, pairing, inverse)
         return got if k is not None else (got[0], None)
+    return _rope(q, k, positions, sections, theta, order, pairing, inverse, q_out, k_out, stream)
+
+
+def _rope(q, k, positions, sections, theta, order, pairing, inverse, q_out=None, k_out=None,
+          stream=None):
+    """rope_axes without derivatives."""
     dev = q.get_device()
     _one_device(max(dev, 0), q, k, positions, q_out, k_out)
     sections = tuple(sections)
@@ -680,24 +698,31 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
 
 
 class _RopeAxes(torch.autograd.Function):
-    """A rotation's gradient is the rotation back."""
+    """A rotation is linear: its gradient is the rotation back, a tangent turns as
+    the input does.  (rope_axes in both, so they have derivatives of their own.)"""
 
     @staticmethod
-    def forward(ctx, q, k, positions, sections, theta, order, pairing, inverse):
+    def forward(ctx, q, k, positions, *how):
         ctx.save_for_backward(positions)
-        ctx.how = (sections, theta, order, pairing)
-        ctx.inverse, ctx.has_k = inverse, k is not None
-        with torch.no_grad():
-            qo, ko = rope_axes(q, k, positions, sections, theta, order, pairing, inverse)
-        return (qo, ko) if k is not None else (qo,)
+        ctx.save_for_forward(positions)
+        *ctx.how, ctx.inverse = how
+        ctx.has_k = k is not None
+        got = _rope(q, k, positions, *how)
+        return got if ctx.has_k else got[:1]
 
     @staticmethod
     def backward(ctx, *grads):
         (positions,) = ctx.saved_tensors
-        # (differentiable itself where a second derivative is asked for)
-        gq, gk = rope_axes(grads[0], grads[1] if ctx.has_k else None, positions,
-                           *ctx.how, not ctx.inverse)
+        gq, gk = rope_axes(grads[0], grads[1] if ctx.has_k else None, positions, *ctx.how,
+                           not ctx.inverse)
         return gq, gk, None, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        (positions,) = ctx.saved_tensors
+        turn = lambda t: None if t is None else rope_axes(  # noqa: E731
+            t, None, positions, *ctx.how, ctx.inverse)[0]
+        return (turn(tq), turn(tk)) if ctx.has_k else (turn(tq),)
 
 
 class Int8PagedCache:
