@@ -6,14 +6,24 @@
 
 namespace tkv {
 
-// Range of the f16 weights.  A row's softmax reference m is moved only when its
-// weights outgrow 2^kInt8Lazy; the value scales are divided by a power of two 2^E
-// that is raised when one exceeds it; weights are held times 2^5.  So they stay
-// at 2^15 or below, and lose bits (fp16 has steps of 2^-24 at the bottom) only
-// below 2^-19 of the largest value row.
+// Range of the f16 weights.  The weight of a token is p s 2^(5 - e): p = 2^(score - m),
+// s its value scale.  A row's softmax reference m is moved only when p outgrows
+// 2^kInt8Lazy, so weights stay at 2^15 or below where s <= 2^e, and they lose bits (fp16
+// has steps of 2^-24 at the bottom) only below 2^-19 2^e.  e is the E of all rows that a
+// warp (decode) or CTA (chunk) works on together, the power of two at the largest scale
+// that any of them sees, so that s 2^(5 - E) is formed once a token.  But a row may not
+// see that token, or hardly weigh it.  Rows whose largest p s is below 2^(E -
+// kInt8Quiet) take an e of their own, from that product: their p is multiplied by 2^c, c =
+// E - e, whose inverse multiplies their sum of p.  That product is known from steps
+// that computed it and is a lower bound after them, which is the safe side: e only gets
+// too small, which a weight past 2^15 shows.  So every weight is within 2^-11 of itself
+// or 2^-25 of the row's largest p s.  Where c is more than kInt8Far (p 2^c nears the ends of
+// 32 bits), weights are 2^(score - m + log2 s + 5 - e) instead.
 constexpr float kInt8Lazy = 10.f;
 constexpr float kInt8LazyWeight = 1024.f;  // 2^kInt8Lazy
-constexpr float kInt8WeightUp = 32.f;
+constexpr float kInt8WeightUp = 32.f;     // 2^kInt8WeightExp
+constexpr float kInt8WeightExp = 5.f;
+constexpr float kInt8Quiet = 4.f, kInt8Far = 60.f;
 constexpr int kInt8DecodeRows = 16;     // most rows of the decode kernel
 
 // Decode kernel: the steps (8 pages of a (sequence, kv head)) of all its sequences
@@ -105,6 +115,28 @@ __device__ __forceinline__ void int8_row_power(float m, float& up, float& down) 
 __device__ __forceinline__ float int8_scale_inverse(float s) {
   const int e = static_cast<int>(__float_as_uint(s) >> 23);  // 2^(e - 127) <= s
   return __uint_as_float(static_cast<uint32_t>(min(253, max(1, 253 - e))) << 23);
+}
+
+// E of 2^-E
+__device__ __forceinline__ float int8_scale_exponent(float inverse) {
+  return static_cast<float>(127 - static_cast<int>(__float_as_uint(inverse) >> 23));
+}
+// 2^e, e a whole number from -126 to 126
+__device__ __forceinline__ float int8_pow2(float e) {
+  return __uint_as_float(static_cast<uint32_t>(127 + static_cast<int>(e)) << 23);
+}
+// log2 of a value scale: -inf for none
+__device__ __forceinline__ float int8_log2(float s) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;\n" : "=f"(y) : "f"(s));
+  return y;
+}
+// The e of a row with reference m whose largest score + log2 s is top (a row that has
+// seen nothing has no weights: E).  NaN, from scores that are no numbers, gives -126.
+__device__ __forceinline__ float int8_row_exponent(float top, float m, float E) {
+  if (m == -INFINITY) return E;
+  const float e = fminf(fmaxf(ceilf(top - m), -126.f), 126.f);
+  return E - e > kInt8Quiet ? e : E;
 }
 
 // four consecutive channels of an output row, rounded once

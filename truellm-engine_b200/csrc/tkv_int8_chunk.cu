@@ -240,10 +240,13 @@ struct Sm {
   static constexpr int V_OFF = K_OFF + kStages * K_BYTES;
   static constexpr int KS_OFF = V_OFF + kStages * V_BYTES;   // [stage][64] f32 key scales
   static constexpr int VS_OFF = KS_OFF + kStages * kTN * 4;  // [stage][64] value scales 2^-E 2^5
-  static constexpr int VI_OFF = VS_OFF + kStages * kTN * 4;  // [stage] 2^-E of the tile
+  static constexpr int VL_OFF = VS_OFF + kStages * kTN * 4;  // [stage][64] log2 of value scales
+  // [stage] 2^-E of the tile, [stage] log2 of its smallest value scale
+  static constexpr int VI_OFF = VL_OFF + kStages * kTN * 4;
   static constexpr int ROW_OFF = VI_OFF + 32;                // [256] f32 of the rows
   static constexpr int BAR_OFF = ROW_OFF + kSoftmax * 4;
   static constexpr int BYTES = BAR_OFF + 256;
+  static_assert(2 * kStages * 4 <= ROW_OFF - VI_OFF, "");
   static_assert(BYTES <= 227 * 1024, "one CTA's shared memory");
   static_assert(BYTES <= (1 << 18), "descriptor address fields never carry");
   static constexpr uint32_t TWG = 256, TO = 128, TCOLS = 512;
@@ -300,6 +303,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
   static_assert((4 * kStages + 13) * 8 + 4 <= 256, "the barriers fit their area");
   float* const ks_s = reinterpret_cast<float*>(smem + SM::KS_OFF);
   float* const vs_s = reinterpret_cast<float*>(smem + SM::VS_OFF);
+  float* const vl_s = reinterpret_cast<float*>(smem + SM::VL_OFF);
   float* const vi_s = reinterpret_cast<float*>(smem + SM::VI_OFF);
   float* const row_s = reinterpret_cast<float*>(smem + SM::ROW_OFF);
 
@@ -491,17 +495,25 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         prefetch_tile(i + 1, i + kPrefetch);
         // tokens that no row of the CTA sees count for nothing
         const int t0 = (j_lo + i) * kTN + 2 * lane;
-        const float v0 = t0 < kv_end && t0 >= kv_lo ? sr.y : 0.f;
-        const float v1 = t0 + 1 < kv_end && t0 + 1 >= kv_lo ? sr.w : 0.f;
+        const bool in0 = t0 < kv_end && t0 >= kv_lo, in1 = t0 + 1 < kv_end && t0 + 1 >= kv_lo;
+        const float v0 = in0 ? sr.y : 0.f, v1 = in1 ? sr.w : 0.f;
         float top = fmaxf(fmaxf(v0, v1), 0.f);
+        float low = fminf(in0 ? v0 : INFINITY, in1 ? v1 : INFINITY);
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+        for (int d = 1; d < 32; d <<= 1) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+          low = fminf(low, __shfl_xor_sync(0xffffffffu, low, d));
+        }
         if (top * vinv > 1.f) vinv = int8_scale_inverse(top);
         if (i >= kStages && !mbar_wait_near(&vfree[st], ((i / kStages) & 1) ^ 1, a.err)) break;
         *reinterpret_cast<float2*>(ks_s + st * kTN + 2 * lane) = make_float2(sr.x, sr.z);
         *reinterpret_cast<float2*>(vs_s + st * kTN + 2 * lane) =
             make_float2(v0 * vinv * kInt8WeightUp, v1 * vinv * kInt8WeightUp);
-        if (lane == 0) vi_s[st] = vinv;
+        *reinterpret_cast<float2*>(vl_s + st * kTN + 2 * lane) = make_float2(int8_log2(v0), int8_log2(v1));
+        if (lane == 0) {
+          vi_s[st] = vinv;
+          vi_s[kStages + st] = int8_log2(low);
+        }
         mbar_arrive(&vready[st]);
       }
     }
@@ -614,6 +626,12 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     const int pmin = a.window > 0 ? max(0, plim - a.window + 1) : 0;
     // a row that does not exist sees nothing and has no reference to move
     float m = valid ? -INFINITY : 0.f, l = 0.f, vinv = 0x1p126f;
+    // c = E - e of the row; shift: 0 when c is 0 in all rows of the warp, 2 when it is more
+    // than kInt8Far in one.  row_s keeps log2 of the row's largest product of weight and
+    // scale, m included (a lower bound).
+    row_s[ctid] = -INFINITY;
+    float c = 0.f;
+    int shift = 0;
     bool ok = true;
     const float2 ra2 = make_float2(ra, ra);
     bool fresh = true;  // a row of the warp has no reference yet
@@ -626,35 +644,41 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       umma::fence_after_sync();
       const bool masked = __any_sync(0xffffffffu, valid && (t0 + kTN - 1 > plim || t0 < pmin));
       const float vnew = vi_s[st];
-      float fv = 1.f;
-      if (vnew != vinv) {
-        fv = vnew / vinv;
-        vinv = vnew;
-      }
       const uint32_t tSi = tS + (i & 1) * kTN;
       const float4* ks4 = reinterpret_cast<const float4*>(ks_s + st * kTN);
       const float4* vs4 = reinterpret_cast<const float4*>(vs_s + st * kTN);
-      bool plain = !fresh && fv == 1.f;
+      bool plain = !fresh && vnew == vinv && shift < 2;
       if (plain) {
-        // A pass with the reference as it is: no maximum is taken.  A sum of
-        // 2^kInt8Lazy or less shows that no weight has outgrown it.
+        // A pass with the reference and the power of two as they are: no maximum is
+        // taken.  A sum of 2^kInt8Lazy or less shows that no p has outgrown the one; where
+        // the other is a row's own, the weights themselves show that none has outgrown it.
         float2 sum = make_float2(0.f, 0.f);
         uint32_t pk[32];
         if (masked)
-          tile_weights<true>(tSi, ks4, vs4, ra2, -m, t0, pmin, plim, sum, pk);
+          tile_weights<true>(tSi, ks4, vs4, ra2, c - m, t0, pmin, plim, sum, pk);
         else
-          tile_weights<false>(tSi, ks4, vs4, ra2, -m, 0, 0, 0, sum, pk);
-        plain = !__any_sync(0xffffffffu, sum.x + sum.y > kInt8LazyWeight);
+          tile_weights<false>(tSi, ks4, vs4, ra2, c - m, 0, 0, 0, sum, pk);
+        float all = sum.x + sum.y;
+        bool grown = all > kInt8LazyWeight;
+        if (__builtin_expect(shift, 0)) {
+          all *= fast_exp2(-c);
+          uint32_t w = pk[0];  // f16s that are not negative, as whole numbers: infinity is 0x7c00
+#pragma unroll
+          for (int k = 1; k < 32; ++k) w = __vmaxu2(w, pk[k]);
+          grown = all > kInt8LazyWeight || (w & 0xffffu) >= 0x7c00u || w >= 0x7c000000u;
+        }
+        plain = !__any_sync(0xffffffffu, grown);
         if (plain) {
-          l += sum.x + sum.y;
+          l += all;
           st32u(tSi, pk);
         }
       }
       if (!plain) {
-        // A first reference, one that has to move, or the value scales' power of two
-        // has: the tile's maximum, O and l brought to the new
+        // A first reference, one that has to move, or a power of two of the value scales
+        // that has: the tile's largest score (and product), O and l brought to the new
         // reference, then the weights.  (Compact code: it is rare, and instruction
         // fetches cost the CTA's start and end more than its loops.)
+        const float4* vl4 = reinterpret_cast<const float4*>(vl_s + st * kTN);
         float mx = -INFINITY;
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
@@ -662,15 +686,41 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
           ld16_wait(tSi + 16 * q, x);
           scale_scores<true>(x, ks4 + 4 * q, t0 + 16 * q, pmin, plim);
 #pragma unroll
-          for (int c = 0; c < 16; c += 2) mx = fmaxf(mx, fmaxf(x[c], x[c + 1]));
+          for (int k = 0; k < 16; k += 2) mx = fmaxf(mx, fmaxf(x[k], x[k + 1]));
         }
         mx *= ra;  // ra > 0 keeps the order
+        const float m0 = m;
         const bool up = mx > m;
-        const float f = up ? (m == -INFINITY ? 0.f : fast_exp2(m - mx)) : 1.f;
         m = up ? mx : m;
-        l *= f;
+        l *= up ? (m0 == -INFINITY ? 0.f : fast_exp2(m0 - mx)) : 1.f;
         fresh = __any_sync(0xffffffffu, m == -INFINITY);
-        if (i > 0 && __any_sync(0xffffffffu, f * fv != 1.f)) {
+        const float E = int8_scale_exponent(vnew), e0 = int8_scale_exponent(vinv) - c;
+        // The largest product is that of the largest score with the tile's smallest scale
+        // or more.  Where that does not show a row to be loud enough, it is taken exactly.
+        float top = fmaxf(row_s[ctid], mx + vi_s[kStages + st]);
+        float er = valid ? int8_row_exponent(top, m, E) : E;
+        if (__builtin_expect(__any_sync(0xffffffffu, er != E), 0)) {
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+            float x[16];
+            ld16_wait(tSi + 16 * q, x);
+            scale_scores<true>(x, ks4 + 4 * q, t0 + 16 * q, pmin, plim);
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              const float4 v4 = vl4[4 * q + e / 4];
+              top = fmaxf(top, fmaxf(fmaxf(fmaf(x[e], ra, v4.x), fmaf(x[e + 1], ra, v4.y)),
+                                     fmaxf(fmaf(x[e + 2], ra, v4.z), fmaf(x[e + 3], ra, v4.w))));
+            }
+          }
+          er = valid ? int8_row_exponent(top, m, E) : E;
+        }
+        row_s[ctid] = top;
+        c = E - er;
+        vinv = vnew;
+        shift = __any_sync(0xffffffffu, c > kInt8Far) ? 2 : __any_sync(0xffffffffu, c != 0.f) ? 1 : 0;
+        // O's factor (O is 0 in a row without a reference)
+        const float f = m0 == -INFINITY ? (m == -INFINITY ? 1.f : 0.f) : fast_exp2((m0 - m) + (e0 - er));
+        if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) {
           // O holds the tiles before, once the last one's products are in
           ok = __all_sync(0xffffffffu,
                           mbar_wait_near(&odone[2 * wg + ((i - 1) & 1)], ((i - 1) >> 1) & 1, a.err));
@@ -681,33 +731,59 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
             float o[16];
             ld16_wait(tO + c0, o);
 #pragma unroll
-            for (int c = 0; c < 16; ++c) o[c] *= f * fv;
+            for (int k = 0; k < 16; ++k) o[k] *= f;
             umma::st16(tO + c0, o);
           }
         }
         const float nm = m == -INFINITY ? 0.f : -m;
         // P of tokens 16 q .. goes over columns 8 q .., whose scores have been read
+        if (!__builtin_expect(shift, 0)) {
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          float x[16];
-          uint32_t pw[8];
-          ld16_wait(tSi + 16 * q, x);
-          scale_scores<true>(x, ks4 + 4 * q, t0 + 16 * q, pmin, plim);
+          for (int q = 0; q < 4; ++q) {
+            float x[16];
+            uint32_t pw[8];
+            ld16_wait(tSi + 16 * q, x);
+            scale_scores<true>(x, ks4 + 4 * q, t0 + 16 * q, pmin, plim);
 #pragma unroll
-          for (int c = 0; c < 16; c += 4) {
-            const float4 v4 = vs4[4 * q + c / 4];
-            const float v[4] = {v4.x, v4.y, v4.z, v4.w};
-            float w[4];
+            for (int e = 0; e < 16; e += 4) {
+              const float4 v4 = vs4[4 * q + e / 4];
+              const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+              float w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float p = fast_exp2(fmaf(x[c + e], ra, nm));
-              l += p;
-              w[e] = x[c + e] == -INFINITY ? 0.f : p * v[e];  // masked: whatever the scale holds
+              for (int k = 0; k < 4; ++k) {
+                const float p = fast_exp2(fmaf(x[e + k], ra, nm));
+                l += p;
+                w[k] = x[e + k] == -INFINITY ? 0.f : p * v[k];  // masked: whatever the scale holds
+              }
+              pw[e / 2] = pack_h2(w[0], w[1]);
+              pw[e / 2 + 1] = pack_h2(w[2], w[3]);
             }
-            pw[c / 2] = pack_h2(w[0], w[1]);
-            pw[c / 2 + 1] = pack_h2(w[2], w[3]);
+            umma::st8(tSi + 8 * q, pw);
           }
-          umma::st8(tSi + 8 * q, pw);
+        } else {
+          const float ve = kInt8WeightExp - er;
+#pragma unroll 1
+          for (int q = 0; q < 4; ++q) {
+            float x[16];
+            uint32_t pw[8];
+            ld16_wait(tSi + 16 * q, x);
+            scale_scores<true>(x, ks4 + 4 * q, t0 + 16 * q, pmin, plim);
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              const float4 v4 = vl4[4 * q + e / 4];
+              const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+              float w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float y = fmaf(x[e + k], ra, nm);
+                l += fast_exp2(y);
+                w[k] = x[e + k] == -INFINITY ? 0.f : fast_exp2(y + (v[k] + ve));
+              }
+              pw[e / 2] = pack_h2(w[0], w[1]);
+              pw[e / 2 + 1] = pack_h2(w[2], w[3]);
+            }
+            umma::st8(tSi + 8 * q, pw);
+          }
         }
       }
       umma::wait_st();
@@ -720,9 +796,10 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     umma::fence_after_sync();
     // ---- normalise and write the rows (a run's partial when the context is split),
     // eight channels a thread, 64 contiguous bytes a quad ----
-    row_s[ctid] = l == 0.f ? 0.f : 1.f / l;
+    // 2^(e - 5) / l, where the power may be subnormal
+    row_s[ctid] = (l == 0.f ? 0.f : 1.f / l) *
+                  (int8_pow2(int8_scale_exponent(vinv) - c) / kInt8WeightUp);
     __syncwarp();
-    const float vs = (1.f / vinv) / kInt8WeightUp;
     const int64_t slot0 = static_cast<int64_t>(blockIdx.x - sp.whole) * kSoftmax;  // of a split item
     if (ok) {
 #pragma unroll 1
@@ -733,7 +810,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const uint32_t rho = r0 + row0 + 8 * k, tok = rho / grp;
-          inv[k] = row_s[row0 + 8 * k] * vs;
+          inv[k] = row_s[row0 + 8 * k];
           at[k] = (static_cast<int64_t>(q0 + tok) * a.num_q_heads + h * grp + rho - tok * grp) * D;
         }
 #pragma unroll 1

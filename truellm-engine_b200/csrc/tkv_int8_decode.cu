@@ -92,6 +92,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
   constexpr int NU = D / 32;         // 32-channel units of V
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float s_ml[kWPC][RB][2];
+  // of a warp's rows: log2 of the largest product of weight and scale, m included (a lower
+  // bound), and c = E - e.  Looked at rarely, so not in registers (16 rows of 128
+  // channels have none left).
+  __shared__ float2 s_row[kWPC][RB];
   __shared__ int s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   // ---- this CTA's range of the steps: each thread counts its share of the
@@ -268,6 +272,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
 
     float o[2 * NU][NT][4], m[NT][2], l[NT][2];
     float vinv = 0x1p126f;  // 2^-E of the value scales
+    bool shifted = false;   // c is not 0 in some row of the warp
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -275,6 +280,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
     }
+    if (lane < RB) s_row[warp][lane] = make_float2(-INFINITY, 0.f);
+    __syncwarp();
     const int tk = 4 * (g >> 1) + (g & 1);  // page token of S row g (row g + 8: tk + 2)
     const int unmasked_hi = len - n;        // positions up to here are seen by every row,
     const int unmasked_lo = a.window > 0 ? len - a.window : 0;  // from here on
@@ -353,31 +360,53 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
         }
       float svm = fmaxf(fmaxf(sv[0][0], sv[0][1]), fmaxf(sv[1][0], sv[1][1]));
       need |= svm * vinv > 1.f;
-      if (__any_sync(0xffffffffu, need)) {
+      // this lane's largest product of a row, from its tokens tk and tk + 2 of each page
+      auto largest = [&](int nt, int e) {
+        float y = -INFINITY;
+#pragma unroll
+        for (int p = 0; p < kSP; ++p)
+#pragma unroll
+          for (int r2 = 0; r2 < 2; ++r2) y = fmaxf(y, x[p][nt][2 * r2 + e] + int8_log2(sv[p][r2]));
+        return y;
+      };
+      if (__builtin_expect(shifted, 0)) {  // rows with an e of their own: no weight may outgrow it
+        const float E = int8_scale_exponent(vinv);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            need |= largest(nt, e) - m[nt][e] > E - s_row[warp][8 * nt + 2 * t + e].y + kInt8Lazy;
+      }
+      if (__builtin_expect(__any_sync(0xffffffffu, need), 0)) {
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) svm = fmaxf(svm, __shfl_xor_sync(0xffffffffu, svm, d));
-        float fv = 1.f;
-        if (svm * vinv > 1.f) {
-          const float v2 = int8_scale_inverse(svm);
-          fv = v2 / vinv;
-          vinv = v2;
-        }
+        const float E0 = int8_scale_exponent(vinv);
+        if (svm * vinv > 1.f) vinv = int8_scale_inverse(svm);
+        const float E = int8_scale_exponent(vinv);
+        bool some = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float f[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float y = mx[nt][e];
-            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
-            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
-            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
-            f[e] = 1.f;
-            if (y > m[nt][e] + kInt8Lazy) {
-              f[e] = m[nt][e] == -INFINITY ? 0.f : fast_exp2(m[nt][e] - y);
-              m[nt][e] = y;
+            float y = mx[nt][e], z = largest(nt, e);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) {
+              y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
+              z = fmaxf(z, __shfl_xor_sync(0xffffffffu, z, d));
             }
-            l[nt][e] *= f[e];
-            f[e] *= fv;
+            float2& row = s_row[warp][8 * nt + 2 * t + e];
+            const float top = fmaxf(row.x, z), m0 = m[nt][e], e0 = E0 - row.y;
+            if (y > m0 + kInt8Lazy) m[nt][e] = y;
+            const float er = int8_row_exponent(top, m[nt][e], E);
+            some |= er != E;
+            __syncwarp();
+            if (g == 0) row = make_float2(top, E - er);
+            f[e] = 0.f;  // of O; a row without a reference has neither O nor l
+            if (m0 != -INFINITY) {
+              f[e] = fast_exp2((m0 - m[nt][e]) + (e0 - er));
+              l[nt][e] *= fast_exp2(m0 - m[nt][e]);
+            }
           }
 #pragma unroll
           for (int i = 0; i < 2 * NU; ++i) {
@@ -387,26 +416,50 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
             o[i][nt][3] *= f[1];
           }
         }
+        shifted = __any_sync(0xffffffffu, some);
+        __syncwarp();
       }
-      // ---- weights and O ----
+      // ---- weights (where the scores were) and O ----
+      if (!__builtin_expect(shifted, 0)) {
+#pragma unroll
+        for (int p = 0; p < kSP; ++p) {
+          const float v1 = sv[p][0] * vinv * kInt8WeightUp, v2 = sv[p][1] * vinv * kInt8WeightUp;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float ref = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
+              const float pe = fast_exp2(x[p][nt][e] - ref);
+              l[nt][e & 1] += pe;
+              const bool none = masked && x[p][nt][e] == -INFINITY;
+              x[p][nt][e] = none ? 0.f : pe * (e < 2 ? v1 : v2);  // whatever the scale holds
+            }
+        }
+      } else {
+        const float ve = kInt8WeightExp - int8_scale_exponent(vinv);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float ref = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
+            const float up = ve + s_row[warp][8 * nt + 2 * t + (e & 1)].y;
+#pragma unroll
+            for (int p = 0; p < kSP; ++p) {
+              const float y = x[p][nt][e] - ref;
+              l[nt][e & 1] += fast_exp2(y);
+              const bool none = masked && x[p][nt][e] == -INFINITY;
+              x[p][nt][e] = none ? 0.f : fast_exp2(y + (int8_log2(sv[p][e >> 1]) + up));
+            }
+          }
+      }
 #pragma unroll
       for (int p = 0; p < kSP; ++p) {
         const uint8_t* blk = st + (p == 0 || two ? p * F::BYTES : 0) + F::V_OFF;
         uint32_t b0[NT], b1[NT];
-        const float v1 = sv[p][0] * vinv * kInt8WeightUp, v2 = sv[p][1] * vinv * kInt8WeightUp;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float w[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float ref = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
-            const float pe = fast_exp2(x[p][nt][e] - ref);
-            l[nt][e & 1] += pe;
-            w[e] = pe * (e < 2 ? v1 : v2);
-            if (masked && x[p][nt][e] == -INFINITY) w[e] = 0.f;  // whatever the scale holds
-          }
-          b0[nt] = movmatrix_trans(pack_h2(w[0], w[1]));
-          b1[nt] = movmatrix_trans(pack_h2(w[2], w[3]));
+          b0[nt] = movmatrix_trans(pack_h2(x[p][nt][0], x[p][nt][1]));
+          b1[nt] = movmatrix_trans(pack_h2(x[p][nt][2], x[p][nt][3]));
         }
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
@@ -431,7 +484,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
     turns += issued;
 
     // ---- join the warps: rows normalised by their own sums, weighted by l 2^m ----
-    const float vs = (1.f / vinv) / kInt8WeightUp;  // 2^E / 2^5, subnormal at the least
     float* const so = reinterpret_cast<float*>(smem);  // [warp][row][D]
     __syncthreads();                                   // every ring is idle
 #pragma unroll
@@ -444,6 +496,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         const int r = 8 * nt + 2 * t + e;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        // 2^(e - 5), subnormal at the least
+        const float vs = int8_pow2(int8_scale_exponent(vinv) - s_row[warp][r].y) / kInt8WeightUp;
         if (g == 0) {
           s_ml[warp][r][0] = m[nt][e];
           s_ml[warp][r][1] = sum;
