@@ -152,3 +152,21 @@ def test_rows_that_see_only_zeros_at_first(ops, cuda, new):
     q = b.query(4, mult=0.5)
     for window in (0, 40, 95):
         check(b, q, b.attend(q, window), window)
+
+
+@pytest.mark.parametrize("new", [1, 3, 40, 150])
+@pytest.mark.parametrize("size,scale", [(2.0 ** -120, 2.0 ** -60), (2.0 ** -30, 2.0 ** -100),
+                                        (2.0 ** -120, 1.0), (2.0 ** -60, 2.0 ** -120)])
+def test_scores_too_small_for_32_bits(ops, cuda, new, size, scale):
+    """Queries and scales whose product is below the smallest float: all weights are
+    equal, and masked tokens stay masked."""
+    b = Batch(ops, cuda, [130], [new], 1, 128, BF16, seed=2)
+    b.fill()
+    q = b.query(4, mult=size)
+    for window in (0, 50):
+        out = b.attend(q, window, scale=scale)
+        values = unpack(b.pool.cpu().numpy(), 128)
+        k, v = b.dense(0, values)
+        want = attend64(f64(q), k, v, 130 + np.arange(new), scale, window)
+        off, lim = np.abs(f64(out) - want[0]), bound(*want, 128, BF16)
+        assert (off <= lim).all()

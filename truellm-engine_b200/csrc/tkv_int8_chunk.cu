@@ -612,7 +612,9 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     // thread ctid owns row ctid
     const bool valid = ctid < rows;
     const int qi = valid ? static_cast<int>((r0 + ctid) / grp) : 0;
-    const float ra = row_s[ctid] * a.alpha;  // 2^e * scale * log2(e)
+    // 2^e * scale * log2(e), not 0: a masked token's -inf times it stays -inf (and a score
+    // is below 2^-21 with the smallest float)
+    const float ra = fmaxf(row_s[ctid] * a.alpha, 0x1p-149f);
     if (wg < wgs && kRows * wg + 32 * (warp & 3) >= rows) {
       // no row of this warp exists: it only keeps the hand-overs going
       for (int i = 0; i < nj; ++i) {
