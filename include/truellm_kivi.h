@@ -481,6 +481,7 @@ TKV_API int tkv_int8_read(const tkv_int8_cache_t* cache, void* k_out, void* v_ou
  * n_s tokens (already appended), at positions p = seq_lens[s] - n_s + i.  Each
  * attends to the tokens (p - window, p] (window 0: [0, p]):
  *   out = softmax(scale * q . k) v, kv head = q head / (num_q_heads / n_kv_heads).
+ * scale is positive and below 2^127.
  * Scores, sums and outputs are 32-bit; a weight (probability times value scale)
  * is held in fp16: within 2^-11 of itself, or 2^-25 of the largest such product of
  * the row's own tokens, whatever tokens it does not see or weigh hold.  bf16

@@ -191,7 +191,7 @@ int tkv_int8_attend(const tkv_int8_cache_t* cache, const void* q, int q_dtype,
   if (!attend_sizes_ok(num_seqs, num_q_heads, cache->n_kv_heads, cache->head_dim, max_q_tokens,
                        max_context_len) ||
       total_q_tokens < 0 || max_blocks_per_seq <= 0 || window < 0 || !(scale > 0.f) ||
-      !isfinite(scale))
+      !isfinite(scale * 1.4426950408889634f))
     return TKV_INVALID_ARGUMENT;
   if (num_seqs == 0 || total_q_tokens == 0 || max_q_tokens == 0) return TKV_OK;
   if (!q || !q_stride || !out || !cu_q || !block_tables || !seq_lens || !workspace)
