@@ -28,3 +28,22 @@ def test_a_workspace_of_the_largest_sizes_serves_smaller_batches(ops, cuda, D, d
         b.check(q, out, rows=2)
         assert torch.equal(out, b.attend(q))
     assert (raw[n:] == 0x5a).all()
+
+
+def test_numbers_past_32_bits_are_refused(ops, cuda):
+    """A window of 2^32 is not "no window", a bound of 2^32 not 0."""
+    b = Batch(ops, cuda, [100], [4], 2, 64, DT["f16"])
+    b.fill()
+    q, z, cu = b.query(4), t32([0], cuda), t32([0, 4], cuda)
+    lens = t32(b.lens, cuda)
+    want = b.attend(q)
+    assert torch.equal(b.attend(q, window=2 ** 31 - 1), want)
+    for call in (lambda n: b.attend(q, window=n),
+                 lambda n: ops.int8_attend(b.cache, q, cu, b.bt_t, lens, max_q_tokens=n),
+                 lambda n: ops.int8_attend(b.cache, q, cu, b.bt_t, lens, max_context_len=n),
+                 lambda n: ops.int8_append(b.cache, b.k[:4], b.v[:4], cu, z, b.bt_t, max_new_tokens=n),
+                 lambda n: ops.int8_read(b.cache, b.bt_t, z, cu, 4, max_tokens=n),
+                 lambda n: ops.int8_read(b.cache, b.bt_t, z, cu, n)):
+        for n in (2 ** 31, 2 ** 32, 2 ** 32 + 200, -2 ** 32):
+            with pytest.raises(ValueError, match="32 bits"):
+                call(n)

@@ -41,3 +41,20 @@ def test_every_smaller_batch_and_chunk_fits():
         assert size(8, hq, 8, 128, 512, 8192) <= most, hq
     # the partials of one round of the SMs, not of the batch
     assert most < 32 << 20 and size(4096, 32, 8, 128, 512, 8192) < 32 << 20
+
+
+@pytest.mark.parametrize("at", range(6))
+@pytest.mark.parametrize("over", [2 ** 32, 2 ** 31, -2 ** 32])
+def test_sizes_past_32_bits_are_refused(ops, at, over):
+    """(and not taken for what their low 32 bits say)"""
+    sizes = [2, 8, 2, 128, 1, 64]
+    assert ops.int8_workspace_bytes(*sizes) > 0
+    sizes[at] += over
+    with pytest.raises(ValueError, match="32 bits"):
+        ops.int8_workspace_bytes(*sizes)
+
+
+def test_sections_past_32_bits_are_refused(ops):
+    for sections in ((64 + 2 ** 32,), (2 ** 32, 64), (64 + 2 ** 32, -2 ** 32)):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops._rope_plan(2 * sum(sections), sections, 1e4, "blocks", "halves")

@@ -564,6 +564,14 @@ def _count(t: torch.Tensor) -> int:
     return t.shape[0] if t.dim() == 1 else -1
 
 
+def _i32(name: str, n) -> int:
+    """n, which the library takes in 32 bits (ctypes would drop the others)."""
+    n = int(n)
+    if not -2 ** 31 <= n < 2 ** 31:
+        raise ValueError(f"{name} is {n}: 32 bits are supported")
+    return n
+
+
 def _err_ptr(err: Optional[torch.Tensor]):
     if err is None:
         return None
@@ -622,9 +630,10 @@ def _rope_plan(rotary_dim: int, sections: tuple, theta: float, order: str,
     if not 1 <= len(sections) <= L.TKV_ROPE_MAX_AXES:
         raise ValueError(f"1 to {L.TKV_ROPE_MAX_AXES} axes are supported")
     p = L.TkvRopePlan()
+    pairs = [_i32("a section", n) for n in sections]
     L.check("tkv_rope_plan_init", L.lib().tkv_rope_plan_init(
-        C.byref(p), rotary_dim, theta, (C.c_int32 * len(sections))(*sections), len(sections),
-        orders[order], pairings[pairing]))
+        C.byref(p), _i32("rotary_dim", rotary_dim), theta, (C.c_int32 * len(pairs))(*pairs),
+        len(pairs), orders[order], pairings[pairing]))
     return p
 
 
@@ -781,7 +790,8 @@ def int8_append(cache: Int8PagedCache, k_new: torch.Tensor, v_new: torch.Tensor,
             cache._ref, k.data_ptr(), v.data_ptr(), _DT[k.dtype],
             _I64x4(ks[0], ks[1], vs[0], vs[1]), _index("cu_new", cu_new, (B + 1,)),
             _index("seq_lens_old", seq_lens_old, (B,)), bt, mb, B, T,
-            T if max_new_tokens is None else int(max_new_tokens), _err_ptr(err), s))
+            T if max_new_tokens is None else _i32("max_new_tokens", max_new_tokens), _err_ptr(err),
+            s))
 
 
 def int8_read(cache: Int8PagedCache, block_tables: torch.Tensor, starts: torch.Tensor,
@@ -795,7 +805,7 @@ def int8_read(cache: Int8PagedCache, block_tables: torch.Tensor, starts: torch.T
     dev = cache._device
     _one_device(max(dev, 0), cache.pool, block_tables, starts, cu, k_out, v_out, err)
     B = _count(starts)
-    shape = (int(total_tokens), cache.n_kv_heads, cache.head_dim)
+    shape = (_i32("total_tokens", total_tokens), cache.n_kv_heads, cache.head_dim)
     with _on(dev, stream) as s:
         if k_out is not None or v_out is not None:
             dtype = (v_out if k_out is None else k_out).dtype
@@ -814,14 +824,14 @@ def int8_read(cache: Int8PagedCache, block_tables: torch.Tensor, starts: torch.T
         L.check("tkv_int8_read", L.lib().tkv_int8_read(
             cache._ref, k_out.data_ptr(), v_out.data_ptr(), _DT[dtype], bt, mb,
             _index("starts", starts, (B,)), _index("cu", cu, (B + 1,)), B, shape[0],
-            shape[0] if max_tokens is None else int(max_tokens), _err_ptr(err), s))
+            shape[0] if max_tokens is None else _i32("max_tokens", max_tokens), _err_ptr(err), s))
     return k_out, v_out
 
 
 def int8_workspace_bytes(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
                          max_q_tokens: int, max_context_len: int) -> int:
-    return int(L.lib().tkv_int8_attend_workspace_bytes(num_seqs, num_q_heads, num_kv_heads,
-                                                       head_dim, max_q_tokens, max_context_len))
+    sizes = (num_seqs, num_q_heads, num_kv_heads, head_dim, max_q_tokens, max_context_len)
+    return int(L.lib().tkv_int8_attend_workspace_bytes(*[_i32("a size", n) for n in sizes]))
 
 
 def int8_workspace(num_seqs: int, num_q_heads: int, num_kv_heads: int, head_dim: int,
@@ -860,8 +870,9 @@ def int8_attend(cache: Int8PagedCache, q: torch.Tensor, cu_q: torch.Tensor,
         if Hq % cache.n_kv_heads:
             raise ValueError(f"{Hq} q heads do not share {cache.n_kv_heads} kv heads evenly")
         bt, mb = _table(block_tables, B)
-        mq = T if max_q_tokens is None else int(max_q_tokens)
-        ml = mb * L.TKV_PAGE_SIZE if max_context_len is None else int(max_context_len)
+        mq = T if max_q_tokens is None else _i32("max_q_tokens", max_q_tokens)
+        ml = _i32("max_context_len",
+                  mb * L.TKV_PAGE_SIZE if max_context_len is None else max_context_len)
         if out is None:
             out = _like(x, out_dtype or x.dtype)
         elif out.shape != (T, Hq, D) or not out.is_contiguous():
@@ -876,7 +887,7 @@ def int8_attend(cache: Int8PagedCache, q: torch.Tensor, cu_q: torch.Tensor,
         L.check("tkv_int8_attend", L.lib().tkv_int8_attend(
             cache._ref, x.data_ptr(), _DT[x.dtype], _I64x2(st[0], st[1]),
             out.data_ptr(), _DT[out.dtype], _index("cu_q", cu_q, (B + 1,)), bt, mb,
-            _index("seq_lens", seq_lens, (B,)), B, Hq, T, mq, ml, int(window),
+            _index("seq_lens", seq_lens, (B,)), B, Hq, T, mq, ml, _i32("window", window),
             1.0 / math.sqrt(D) if scale is None else float(scale), workspace.data_ptr(),
             workspace.nbytes, _err_ptr(err), s))
     return out
