@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
 #pragma unroll
         for (int ci = 0; ci < CI; ++ci) {
           const uint4* s4 = reinterpret_cast<const uint4*>(src + 16 * (t + 4 * ci));
-          const uint4 x = __ldg(s4), y = __ldg(s4 + 1);
+          const uint4 x = s4[0], y = s4[1];  // (the output may lie where they do)
           w[ci][0] = x.x, w[ci][1] = x.y, w[ci][2] = x.z, w[ci][3] = x.w;
           w[ci][4] = y.x, w[ci][5] = y.y, w[ci][6] = y.z, w[ci][7] = y.w;
         }

@@ -602,6 +602,47 @@ def _like(x: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return torch.empty(x.shape, dtype=dtype, device=x.device)
 
 
+def _rows(t: torch.Tensor) -> tuple:
+    """Of a [tokens, heads, channels] tensor, in bytes: where it starts and ends, its
+    outer stride, and what one step along the outer axis spans."""
+    (T, H, D), (st, sh, _) = t.shape, t.stride()
+    st, sh, size = st if T > 1 else 0, sh if H > 1 else 0, t.element_size()
+    row = D + (sh * (H - 1) if st >= sh else st * (T - 1))
+    whole = D + st * (T - 1) + sh * (H - 1)
+    return t.data_ptr(), t.data_ptr() + size * whole, size * max(st, sh), size * row
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Two tensors lie one after the other, or side by side in rows of one length
+    (slices of a fused projection)."""
+    a0, a1, a_step, a_row = _rows(a)
+    b0, b1, b_step, b_row = _rows(b)
+    if a1 <= b0 or b1 <= a0 or not a.numel() or not b.numel():
+        return True
+    return a_step == b_step > 0 and a_row <= (b0 - a0) % a_step <= a_step - b_row
+
+
+def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
+
+
+def _rope_outputs(q, k, q_out, k_out) -> None:
+    """Refuses outputs whose elements, or whose and an input's, share memory (they may
+    be their inputs)."""
+    for name, o, own, other in (("q_out", q_out, q, k), ("k_out", k_out, k, q)):
+        if o is None:
+            continue
+        (T, H, D), (st, sh, _) = o.shape, o.stride()
+        # (of two axes, one steps over all of the other)
+        if (T > 1 and st < D or H > 1 and sh < D or
+                T > 1 and H > 1 and st < D + sh * (H - 1) and sh < D + st * (T - 1)):
+            raise ValueError(f"elements of {name} share memory")
+        if not (_same(o, own) or _apart(o, own)) or other is not None and not _apart(o, other):
+            raise ValueError(f"{name} overlaps an input")
+    if q_out is not None and k_out is not None and not _apart(q_out, k_out):
+        raise ValueError("q_out overlaps k_out")
+
+
 _I64x2, _I64x4, _I64x8 = C.c_int64 * 2, C.c_int64 * 4, C.c_int64 * 8
 
 
@@ -653,7 +694,8 @@ def rope_axes(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tenso
     gradient).  Calls on tensors that require a gradient, or carry a tangent of
     torch.autograd.forward_ad, are differentiable (not through torch.func); the
     gradient is computed on the call's stream, in order with what comes before and
-    after it.  q_out / k_out may be q / k (in place).  Returns (q_out, k_out)."""
+    after it.  q_out / k_out may be q / k (in place), and share no other memory with
+    them or each other.  Returns (q_out, k_out)."""
     if _differentiated(q, k):
         if q_out is not None or k_out is not None:
             raise ValueError("q_out / k_out cannot be given where a gradient is needed")
@@ -685,11 +727,14 @@ def _rope(q, k, positions, sections, theta, order, pairing, inverse, q_out=None,
             raise ValueError(f"positions must be an int32 [{len(sections)}, {T}] tensor")
         if kx is None and k_out is not None:
             raise ValueError("k_out without k")
-        for o, x in ((q_out, qx), (k_out, kx)):
-            if o is not None and (o.shape != x.shape or o.dtype is not x.dtype or
-                                  _heads("output", o) is not o):
-                raise ValueError("an output must have its input's shape and type, contiguous "
-                                 "channels and strides that are multiples of 8")
+        if q_out is not None or k_out is not None:
+            for o, x in ((q_out, qx), (k_out, kx)):
+                if o is not None and (o.shape != x.shape or o.dtype is not x.dtype or
+                                      _heads("output", o) is not o):
+                    raise ValueError("an output must have its input's shape and type, contiguous "
+                                     "channels and strides that are multiples of 8")
+            if q_out is not q or k_out is not k or q is k:
+                _rope_outputs(qx, kx, q_out, k_out)
         if q_out is None:
             q_out = _like(qx, qx.dtype)
         if kx is not None and k_out is None:
@@ -814,6 +859,8 @@ def int8_read(cache: Int8PagedCache, block_tables: torch.Tensor, starts: torch.T
                                       not t.is_contiguous()):
                     raise ValueError(f"k_out / v_out must be contiguous {list(shape)} tensors "
                                      "of one type")
+            if k_out is not None and v_out is not None and not _apart(k_out, v_out):
+                raise ValueError("k_out overlaps v_out")
         if dtype not in _DT:
             raise ValueError("dtype must be fp16, bf16 or fp32")
         if k_out is None:
@@ -857,7 +904,8 @@ def int8_attend(cache: Int8PagedCache, q: torch.Tensor, cu_q: torch.Tensor,
     strides that are multiples of 8) are the last tokens of sequence s, already
     appended; each attends to itself and the tokens before it, or to the last
     `window` of them.  One row a sequence is a decode step.  Returns out [T, Hq,
-    D] (fp16 or bf16); its rows outside the sequences are not written."""
+    D] (fp16 or bf16; it may be q, contiguous, and shares no other memory with it); its
+    rows outside the sequences are not written."""
     _no_grad_path("int8_attend", q)
     dev = cache._device
     _one_device(max(dev, 0), cache.pool, q, cu_q, block_tables, seq_lens, out, workspace, err)
@@ -873,12 +921,16 @@ def int8_attend(cache: Int8PagedCache, q: torch.Tensor, cu_q: torch.Tensor,
         mq = T if max_q_tokens is None else _i32("max_q_tokens", max_q_tokens)
         ml = _i32("max_context_len",
                   mb * L.TKV_PAGE_SIZE if max_context_len is None else max_context_len)
+        given = out
         if out is None:
             out = _like(x, out_dtype or x.dtype)
         elif out.shape != (T, Hq, D) or not out.is_contiguous():
             raise ValueError(f"out must be a contiguous {[T, Hq, D]} tensor")
         if out.dtype not in _HALF:
             raise ValueError("out must be fp16 or bf16")
+        if given is not None:
+            if not (_apart(out, x) or _same(out, x)):
+                raise ValueError("out overlaps q")
         if workspace is None:
             workspace = int8_workspace(B, Hq, cache.n_kv_heads, D, mq, ml, x.device)
         elif not workspace.is_contiguous():
