@@ -1,5 +1,5 @@
 """Outputs that the caller gives to the rotary step and the int8 cache: in place, side by
-side with inputs, and refused where memory is shared."""
+side with inputs, refused where memory is shared, and known to autograd."""
 import pytest
 import torch
 
@@ -79,3 +79,29 @@ def test_read_outputs_that_share_memory_are_refused(ops, cuda):
     for v in (buf[:20], buf[19:39]):
         with pytest.raises(ValueError, match="overlap"):
             ops.int8_read(*args, k_out=buf[:20], v_out=v)
+
+
+def test_autograd_knows_of_written_outputs(ops, cuda):
+    """What a backward pass has kept and a call then writes is an error in that pass;
+    tensors that require a gradient are no outputs."""
+    q, k, pos = tokens(cuda)
+    b = Batch(ops, cuda, [50], [37], 2, 128, F16)
+    b.fill()
+    read = (b.cache, b.bt_t, t32([0], cuda), t32([0, 37], cuda), 37)
+    for write, shape in ((lambda t: rope(ops, t, None, pos, q_out=t), q.shape),
+                         (lambda t: rope(ops, k, q, pos, k_out=t), q.shape),
+                         (lambda t: b.attend(q, out=t), q.shape),
+                         (lambda t: ops.int8_read(*read, k_out=t), k.shape),
+                         (lambda t: ops.int8_read(*read, v_out=t), k.shape)):
+        w = torch.randn(shape, device=cuda, dtype=F16, requires_grad=True)
+        kept = torch.randn(shape, device=cuda, dtype=F16)
+        loss = (w * kept).sum()
+        write(kept)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            loss.backward()
+        with pytest.raises(ValueError, match="gradient"):
+            write(w)
+        with torch.no_grad():
+            write(w)
+        with torch.inference_mode():
+            write(torch.randn(shape, device=cuda, dtype=F16))

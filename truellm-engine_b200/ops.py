@@ -626,12 +626,18 @@ def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.data_ptr() == b.data_ptr() and a.stride() == b.stride()
 
 
+def _plain(name: str, t: Optional[torch.Tensor]) -> None:
+    if t is not None and _differentiated(t):
+        raise ValueError(f"{name} requires a gradient or carries a tangent: give a plain tensor")
+
+
 def _rope_outputs(q, k, q_out, k_out) -> None:
     """Refuses outputs whose elements, or whose and an input's, share memory (they may
     be their inputs)."""
     for name, o, own, other in (("q_out", q_out, q, k), ("k_out", k_out, k, q)):
         if o is None:
             continue
+        _plain(name, o)
         (T, H, D), (st, sh, _) = o.shape, o.stride()
         # (of two axes, one steps over all of the other)
         if (T > 1 and st < D or H > 1 and sh < D or
@@ -641,6 +647,14 @@ def _rope_outputs(q, k, q_out, k_out) -> None:
             raise ValueError(f"{name} overlaps an input")
     if q_out is not None and k_out is not None and not _apart(q_out, k_out):
         raise ValueError("q_out overlaps k_out")
+
+
+def _written(*outs) -> None:
+    """Tells autograd that these were written (a backward pass that needs what they held
+    before is then an error)."""
+    for t in outs:
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 _I64x2, _I64x4, _I64x8 = C.c_int64 * 2, C.c_int64 * 4, C.c_int64 * 8
@@ -727,6 +741,7 @@ def _rope(q, k, positions, sections, theta, order, pairing, inverse, q_out=None,
             raise ValueError(f"positions must be an int32 [{len(sections)}, {T}] tensor")
         if kx is None and k_out is not None:
             raise ValueError("k_out without k")
+        given = q_out, k_out
         if q_out is not None or k_out is not None:
             for o, x in ((q_out, qx), (k_out, kx)):
                 if o is not None and (o.shape != x.shape or o.dtype is not x.dtype or
@@ -748,6 +763,8 @@ def _rope(q, k, positions, sections, theta, order, pairing, inverse, q_out=None,
             C.byref(plan), qx.data_ptr(), None if kx is None else kx.data_ptr(),
             q_out.data_ptr(), None if kx is None else k_out.data_ptr(), _DT[qx.dtype], Hq, Hk, D,
             T, strides, positions.data_ptr(), positions.stride(0), 1 if inverse else 0, s))
+    if given != (None, None):
+        _written(*given)
     return q_out, k_out
 
 
@@ -859,10 +876,13 @@ def int8_read(cache: Int8PagedCache, block_tables: torch.Tensor, starts: torch.T
                                       not t.is_contiguous()):
                     raise ValueError(f"k_out / v_out must be contiguous {list(shape)} tensors "
                                      "of one type")
+            _plain("k_out", k_out)
+            _plain("v_out", v_out)
             if k_out is not None and v_out is not None and not _apart(k_out, v_out):
                 raise ValueError("k_out overlaps v_out")
         if dtype not in _DT:
             raise ValueError("dtype must be fp16, bf16 or fp32")
+        given = k_out, v_out
         if k_out is None:
             k_out = torch.empty(shape, dtype=dtype, device=cache.pool.device)
         if v_out is None:
@@ -872,6 +892,8 @@ def int8_read(cache: Int8PagedCache, block_tables: torch.Tensor, starts: torch.T
             cache._ref, k_out.data_ptr(), v_out.data_ptr(), _DT[dtype], bt, mb,
             _index("starts", starts, (B,)), _index("cu", cu, (B + 1,)), B, shape[0],
             shape[0] if max_tokens is None else _i32("max_tokens", max_tokens), _err_ptr(err), s))
+    if given != (None, None):
+        _written(*given)
     return k_out, v_out
 
 
@@ -929,6 +951,7 @@ def int8_attend(cache: Int8PagedCache, q: torch.Tensor, cu_q: torch.Tensor,
         if out.dtype not in _HALF:
             raise ValueError("out must be fp16 or bf16")
         if given is not None:
+            _plain("out", out)
             if not (_apart(out, x) or _same(out, x)):
                 raise ValueError("out overlaps q")
         if workspace is None:
@@ -942,4 +965,6 @@ def int8_attend(cache: Int8PagedCache, q: torch.Tensor, cu_q: torch.Tensor,
             _index("seq_lens", seq_lens, (B,)), B, Hq, T, mq, ml, _i32("window", window),
             1.0 / math.sqrt(D) if scale is None else float(scale), workspace.data_ptr(),
             workspace.nbytes, _err_ptr(err), s))
+    if given is not None:
+        _written(given)
     return out
