@@ -101,7 +101,7 @@ template <int TOK>
 void launch_t(const tkv_rope_plan_t& plan, const RopeArgs& a, bool bf16, cudaStream_t stream) {
   const int units = (a.head_dim + 15) / 16;
   const dim3 block(units, kRopeThreads / units);
-  const unsigned int grid = (a.n_tokens + TOK - 1) / TOK;
+  const unsigned int grid = (a.n_tokens - 1) / TOK + 1;
   if (bf16)
     rope_kernel<TOK, true><<<grid, block, 0, stream>>>(plan, a);
   else
