@@ -79,11 +79,6 @@ __device__ __forceinline__ bool int8_seq_ok(int pos, int n, int row, int total, 
          static_cast<long long>(pos) + n <= static_cast<long long>(max_blocks) * kPage;
 }
 
-// f16 or bf16 bits to float
-template <bool BF16>
-__device__ __forceinline__ float half_bits_to_float(uint32_t x) {
-  return BF16 ? __uint_as_float(x << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(x)));
-}
 // two packed 16-bit values to floats
 template <bool BF16>
 __device__ __forceinline__ float2 unpack2(uint32_t x) {
@@ -98,6 +93,12 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   } else {
     return pack_h2(a, b);
   }
+}
+
+// 16 bytes global -> shared, of which the first `bytes` are copied, the rest zeros
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst_smem, const void* src_gmem, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst_smem), "l"(src_gmem), "r"(bytes)
+               : "memory");
 }
 
 // 4 x 4 transpose of 32-bit words over the 4 lanes of a quad (lane bits 0-1 =

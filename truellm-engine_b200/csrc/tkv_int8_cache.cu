@@ -56,12 +56,10 @@ __device__ __forceinline__ int find_seq(const int32_t* cu, int num_seqs, long lo
 constexpr int kAhead = 3;  // heads of the append kernel's rows in shared memory
 
 // How a launch is cut up.  heads: kv heads a CTA takes one after another;
-// per_token: the numbering of page units; wide: the dense rows and their strides
-// are multiples of 32 bytes, so 16 channels are one access of a whole sector
-// (ragged prefixes of 16 sequences read: 98 -> 88 us).
+// per_token: the numbering of page units.
 struct Plan {
   int heads;
-  bool per_token, wide;
+  bool per_token;
 };
 
 // what a CTA works on: page `page` (index in the sequence) of sequence s, and
@@ -206,10 +204,8 @@ __global__ void __launch_bounds__(2 * D, 1024 / (2 * D))
     if (h0 + h < h1) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                         to[e] + (h % kAhead) * static_cast<uint32_t>(sizeof(stage[0]))),
-                     "l"(src[e] + h * step), "r"(bytes[e])
-                     : "memory");
+        cp_async16_or_zero(to[e] + (h % kAhead) * static_cast<uint32_t>(sizeof(stage[0])),
+                           src[e] + h * step, bytes[e]);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -315,7 +311,7 @@ __device__ __forceinline__ void store16(void* out, int64_t at, const uint32_t (&
 }
 
 template <int D, int OUT>
-__global__ void __launch_bounds__(2 * D) int8_read_kernel(Int8ReadArgs a, Plan plan) {
+__global__ void __launch_bounds__(2 * D) int8_read_kernel(Int8ReadArgs a, Plan plan, bool wide) {
   using F = Int8Fmt<D>;
   constexpr int CH = D / 16, HALF = kPage * CH;
   const int parts = (a.n_kv_heads + plan.heads - 1) / plan.heads;
@@ -362,7 +358,7 @@ __global__ void __launch_bounds__(2 * D) int8_read_kernel(Int8ReadArgs a, Plan p
       sh = 0.f;
       w[0] = w[1] = w[2] = w[3] = 0x80808080u;
     }
-    if (valid) store16<OUT>(out, at, w, sh, plan.wide);
+    if (valid) store16<OUT>(out, at, w, sh, wide);
   }
 }
 
@@ -387,7 +383,6 @@ unsigned int plan_grid(int total, int num_seqs, int n_heads, Plan& plan) {
 
 int launch_int8_append(const Int8AppendArgs& a, int head_dim, bool bf16, cudaStream_t stream) {
   Plan plan;
-  plan.wide = false;
   const unsigned int grid = plan_grid(a.total, a.num_seqs, a.n_kv_heads, plan);
   if (grid == 0) return TKV_INVALID_ARGUMENT;
   if (head_dim == 128) {
@@ -406,11 +401,13 @@ int launch_int8_append(const Int8AppendArgs& a, int head_dim, bool bf16, cudaStr
 
 int launch_int8_read(const Int8ReadArgs& a, int head_dim, int out_dtype, cudaStream_t stream) {
   Plan plan;
-  plan.wide =
+  // both outputs start at multiples of 32 bytes, as their rows then do: 16 channels are
+  // one store of a whole sector (ragged prefixes of 16 sequences: 98 -> 88 us)
+  const bool wide =
       ((reinterpret_cast<uintptr_t>(a.k_out) | reinterpret_cast<uintptr_t>(a.v_out)) & 31) == 0;
   const unsigned int grid = plan_grid(a.total, a.num_seqs, a.n_kv_heads, plan);
   if (grid == 0) return TKV_INVALID_ARGUMENT;
-#define TKV_READ(D, OUT) int8_read_kernel<D, OUT><<<grid, 2 * D, 0, stream>>>(a, plan)
+#define TKV_READ(D, OUT) int8_read_kernel<D, OUT><<<grid, 2 * D, 0, stream>>>(a, plan, wide)
   if (head_dim == 128) {
     if (out_dtype == TKV_F32) TKV_READ(128, TKV_F32);
     else if (out_dtype == TKV_F16) TKV_READ(128, TKV_F16);

@@ -141,12 +141,6 @@ __device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
   return *reinterpret_cast<const float2*>(&d);
 }
 
-// 16 bytes global -> shared, or zeros
-__device__ __forceinline__ void cp_async16_or_zero(void* dst_smem, const void* src_gmem, bool copy) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(smem_u32(dst_smem)),
-               "l"(src_gmem), "r"(copy ? 16 : 0)
-               : "memory");
-}
 __device__ __forceinline__ float absmax2(uint32_t bf16_pair) {
   const float2 f = unpack2<true>(bf16_pair);
   return fmaxf(fabsf(f.x), fabsf(f.y));
@@ -339,8 +333,8 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
       const uint16_t* src = a.q + static_cast<int64_t>(q0 + tok) * a.q_t + (h * grp + rho - tok * grp) * a.q_h;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c)
-        cp_async16_or_zero(qs + umma::umma_off(r & 127, 8 * (4 * c + (lane >> 3)), D),
-                           src + 8 * (4 * c + (lane >> 3)), r < rows);
+        cp_async16_or_zero(smem_u32(qs + umma::umma_off(r & 127, 8 * (4 * c + (lane >> 3)), D)),
+                           src + 8 * (4 * c + (lane >> 3)), r < rows ? 16 : 0);
     }
   }
   if (warp == 8) umma::alloc(tslot, SM::TCOLS);

@@ -211,7 +211,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
 
     // ---- the query rows as B operands: lane (g, t) holds row 8 nt + g, channels
     // 16 (t + 4 ci) + 4 wi .. of k-slice 4 ci + wi.  bf16 rows are brought to
-    // f16 by a power of two (exact down to 2^-25 of the row's largest value).
+    // f16 by a power of two: the row's largest value lands in [1, 2), where steps of
+    // 2^-24 keep bf16's 8 bits exact down to 2^-17 of it, and within 2^-25 of it below.
     uint32_t bq[NT][4 * CI][2];
     float ra[NT][2];     // 2^e * scale * log2(e) of rows 8 nt + 2 t, + 1
     int plim[NT][2];     // last position that those rows see

@@ -111,9 +111,9 @@ void launch_t(const tkv_rope_plan_t& plan, const RopeArgs& a, bool bf16, cudaStr
 }  // namespace
 
 int launch_rope(const tkv_rope_plan_t& plan, const RopeArgs& a, bool bf16, cudaStream_t stream) {
-  // One token a CTA up to one round of the GPU's 8 x 148 resident CTAs, four beyond
-  // (40 heads of 128: 256 tokens 3.6 against 5.0 us, 1024 tokens 7.9 against 6.9,
-  // 16384 tokens 85.7 against 66.4).
+  // One token a CTA where there are few, four from 1024 on.  Measured, 40 heads of 128,
+  // one and four tokens a CTA: 256 tokens 3.6 and 5.0 us, 1024 tokens 7.9 and 6.9, 16384
+  // tokens 85.7 and 66.4.
   if (a.n_tokens < 1024)
     launch_t<1>(plan, a, bf16, stream);
   else
