@@ -170,3 +170,19 @@ def test_scores_too_small_for_32_bits(ops, cuda, new, size, scale):
         want = attend64(f64(q), k, v, 130 + np.arange(new), scale, window)
         off, lim = np.abs(f64(out) - want[0]), bound(*want, 128, BF16)
         assert (off <= lim).all()
+
+
+@pytest.mark.parametrize("new", [1, 3, 40, 150])
+@pytest.mark.parametrize("size", [2.0 ** -133, 2.0 ** -130, 2.0 ** -127])
+def test_queries_below_the_normal_range(ops, cuda, new, size):
+    """bf16 queries of subnormal size are no zeros: keys and a scale that bring them back."""
+    b = Batch(ops, cuda, [130], [new], 1, 128, BF16, seed=4)
+    b.k = (b.k.double() * 2.0 ** 60).to(BF16)
+    b.fill()
+    q = (torch.randint(-3, 4, (new, 4, 128), device=cuda).double() * size).to(BF16)
+    scale = 2.0 ** -62 / size / 8
+    out = b.attend(q, scale=scale)
+    k, v = b.dense(0, unpack(b.pool.cpu().numpy(), 128))
+    want = attend64(f64(q), k, v, 130 + np.arange(new), scale, 0)
+    off, lim = np.abs(f64(out) - want[0]), bound(*want, 128, BF16)
+    assert (off <= lim).all()

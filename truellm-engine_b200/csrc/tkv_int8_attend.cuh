@@ -99,12 +99,13 @@ __device__ __forceinline__ bool mbar_wait_near(uint64_t* bar, uint32_t parity, i
 }
 
 // Powers of two that bring a row whose largest magnitude is m into fp16's
-// range: down = 2^-e, up = 2^e with m 2^-e in [1, 4); 1 for zeros, infinities.
+// range: down = 2^-e, up = 2^e with m 2^-e in [1, 4), or below 1 where m is below the
+// normal range (bf16 has 2^-133 at least, so 2^-7); 1 for infinities.
 __device__ __forceinline__ void int8_row_power(float m, float& up, float& down) {
   const uint32_t e = __float_as_uint(m) >> 23;
   up = down = 1.f;
-  if (e > 0 && e < 255) {
-    const uint32_t ec = min(e, 253u);  // 2^-127 is no normal float
+  if (e < 255) {
+    const uint32_t ec = max(1u, min(e, 253u));  // 2^-127 is no normal float
     up = __uint_as_float(ec << 23);
     down = __uint_as_float((254u - ec) << 23);
   }
