@@ -186,3 +186,22 @@ def test_queries_below_the_normal_range(ops, cuda, new, size):
     want = attend64(f64(q), k, v, 130 + np.arange(new), scale, 0)
     off, lim = np.abs(f64(out) - want[0]), bound(*want, 128, BF16)
     assert (off <= lim).all()
+
+
+@pytest.mark.parametrize("new", [1, 3, 40, 150])
+@pytest.mark.parametrize("e,small", [(100, 0), (115, 0), (126, 0), (126, 30), (-106, 0), (-116, 0),
+                                     (-100, -100), (-110, -120)])
+def test_keys_near_the_ends_of_the_type(ops, cuda, new, e, small):
+    """Keys near 2^e in one direction with the queries, whose product passes 32 bits
+    before the scale brings it back; queries of
+    2^-small."""
+    b = Batch(ops, cuda, [130], [new], 1, 128, BF16, seed=6)
+    b.k = ((1 + 0.25 * b.k.float().clamp(-3, 3)).double() * 2.0 ** e).to(BF16)
+    b.fill()
+    q = ((1 + 0.1 * b.query(4).float()).double() * 2.0 ** -small).to(BF16)
+    scale = 2.0 ** (small - e) / 64
+    out = b.attend(q, scale=scale)
+    k, v = b.dense(0, unpack(b.pool.cpu().numpy(), 128))
+    want = attend64(f64(q), k, v, 130 + np.arange(new), scale, 0)
+    off, lim = np.abs(f64(out) - want[0]), bound(*want, 128, BF16)
+    assert (off <= lim).all()

@@ -23,6 +23,10 @@ constexpr float kInt8Lazy = 10.f;
 constexpr float kInt8LazyWeight = 1024.f;  // 2^kInt8Lazy
 constexpr float kInt8WeightUp = 32.f;     // 2^kInt8WeightExp
 constexpr float kInt8WeightExp = 5.f;
+// The chunk kernel multiplies products of a query and codes (2^15 at most) by the key
+// scale (2^121) before the row's factor; 2^-9 of the one and 2^9 of the other keep that in
+// 32 bits.  (Key scales below 2^-117 lose up to 9 of their 24 bits.)
+constexpr float kInt8KeyDown = 0x1p-9f, kInt8KeyUp = 0x1p9f;
 constexpr float kInt8Quiet = 4.f, kInt8Far = 60.f;
 constexpr int kInt8DecodeRows = 16;     // most rows of the decode kernel
 
@@ -99,13 +103,14 @@ __device__ __forceinline__ bool mbar_wait_near(uint64_t* bar, uint32_t parity, i
 }
 
 // Powers of two that bring a row whose largest magnitude is m into fp16's
-// range: down = 2^-e, up = 2^e with m 2^-e in [1, 4), or below 1 where m is below the
-// normal range (bf16 has 2^-133 at least, so 2^-7); 1 for infinities.
+// range: down = 2^-e, up = 2^e with m 2^-e in [1, 2), or below 1 where m is below the
+// normal range (bf16 has 2^-133 at least, so 2^-7), or up to 2^15 where m is above 2^113
+// (which keeps up * kInt8KeyUp finite); 1 for infinities.
 __device__ __forceinline__ void int8_row_power(float m, float& up, float& down) {
   const uint32_t e = __float_as_uint(m) >> 23;
   up = down = 1.f;
   if (e < 255) {
-    const uint32_t ec = max(1u, min(e, 253u));  // 2^-127 is no normal float
+    const uint32_t ec = max(1u, min(e, 240u));
     up = __uint_as_float(ec << 23);
     down = __uint_as_float((254u - ec) << 23);
   }

@@ -150,7 +150,7 @@ __device__ __forceinline__ uint32_t bf16_to_h2(uint32_t bf16_pair, float factor)
   return pack_h2(f.x * factor, f.y * factor);
 }
 
-// 16 scores of a row (tokens t ..) times their key scales; MASKED: tokens that
+// 16 scores of a row (tokens t ..) times their key scales (kInt8KeyDown included); MASKED: tokens that
 // the row does not see (outside [pmin, plim]) become -inf.
 template <bool MASKED>
 __device__ __forceinline__ void scale_scores(float (&x)[16], const float4* ks4, int t, int pmin,
@@ -232,7 +232,7 @@ struct Sm {
   static constexpr int Q_OFF = 0;                      // one operand per warpgroup
   static constexpr int K_OFF = Q_OFF + 2 * Q_BYTES;
   static constexpr int V_OFF = K_OFF + kStages * K_BYTES;
-  static constexpr int KS_OFF = V_OFF + kStages * V_BYTES;   // [stage][64] f32 key scales
+  static constexpr int KS_OFF = V_OFF + kStages * V_BYTES;   // [stage][64] f32 key scales 2^-9
   static constexpr int VS_OFF = KS_OFF + kStages * kTN * 4;  // [stage][64] value scales 2^-E 2^5
   static constexpr int VL_OFF = VS_OFF + kStages * kTN * 4;  // [stage][64] log2 of value scales
   // [stage] 2^-E of the tile, [stage] log2 of its smallest value scale
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         }
         if (top * vinv > 1.f) vinv = int8_scale_inverse(top);
         if (i >= kStages && !mbar_wait_near(&vfree[st], ((i / kStages) & 1) ^ 1, a.err)) break;
-        *reinterpret_cast<float2*>(ks_s + st * kTN + 2 * lane) = make_float2(sr.x, sr.z);
+        *reinterpret_cast<float2*>(ks_s + st * kTN + 2 * lane) = make_float2(sr.x * kInt8KeyDown, sr.z * kInt8KeyDown);
         *reinterpret_cast<float2*>(vs_s + st * kTN + 2 * lane) =
             make_float2(v0 * vinv * kInt8WeightUp, v1 * vinv * kInt8WeightUp);
         *reinterpret_cast<float2*>(vl_s + st * kTN + 2 * lane) = make_float2(int8_log2(v0), int8_log2(v1));
@@ -606,9 +606,9 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
     // thread ctid owns row ctid
     const bool valid = ctid < rows;
     const int qi = valid ? static_cast<int>((r0 + ctid) / grp) : 0;
-    // 2^e * scale * log2(e), not 0: a masked token's -inf times it stays -inf (and a score
+    // 2^e * scale * log2(e) * 2^9, not 0: a masked token's -inf times it stays -inf (and a score
     // is below 2^-21 with the smallest float)
-    const float ra = fmaxf(row_s[ctid] * a.alpha, 0x1p-149f);
+    const float ra = fmaxf(row_s[ctid] * kInt8KeyUp * a.alpha, 0x1p-149f);
     if (wg < wgs && kRows * wg + 32 * (warp & 3) >= rows) {
       // no row of this warp exists: it only keeps the hand-overs going
       for (int i = 0; i < nj; ++i) {
