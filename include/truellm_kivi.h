@@ -436,7 +436,11 @@ TKV_API int tkv_rope_axes(const tkv_rope_plan_t* plan, const void* q, const void
  * Block tables are [num_seqs][max_blocks_per_seq] int32, token p of sequence s
  * in page block_tables[s][p / 16] (cuda_allocator.cpp:273).  A page is written
  * as long as its sequence grows into it, so sequences that share a partly
- * filled page must copy it before either appends. */
+ * filled page must copy it before either appends: a page is n_kv_heads *
+ * page_bytes bytes in a row, so that (or moving it to the host and back) is one
+ * cudaMemcpyAsync on the stream of the calls around it.  A sequence of n tokens
+ * has (n + 15) / 16 pages; the allocator below counts KIVI pages, which are fewer
+ * by the residual ring. */
 typedef struct tkv_int8_cache {
   void* pool;         /* [num_pages][n_kv_heads][page_bytes], 16-byte aligned */
   int32_t num_pages;  /* pages in the pool (bounds for block-table entries)   */
@@ -490,7 +494,8 @@ TKV_API int tkv_int8_read(const tkv_int8_cache_t* cache, void* k_out, void* v_ou
  * n_s = 1 is a decode step; 0 is allowed.  q: fp16 or bf16 [total_q_tokens]
  * [num_q_heads][D] with token and head strides q_stride[2] in elements
  * (multiples of 8, 16-byte aligned); out: contiguous, fp16 or bf16, 16-byte
- * aligned.  Rows outside [cu_q[0], cu_q[num_seqs]) are left as they are.
+ * aligned; it may be q, where q is contiguous, and shares no other memory with
+ * it.  Rows outside [cu_q[0], cu_q[num_seqs]) are left as they are.
  * max_q_tokens bounds n_s and max_context_len bounds seq_lens (they size the
  * grid and the splits); sequences out of these bounds, with n_s > seq_lens[s]
  * or longer than their block table are left as they are and flagged

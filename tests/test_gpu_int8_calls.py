@@ -1,4 +1,5 @@
-"""int8 attention as an engine calls it: one workspace for batches of all sizes."""
+"""The int8 cache as an engine calls it: one workspace for batches of all sizes, numbers
+out of range, a sequence that forks."""
 import numpy as np
 import pytest
 import torch
@@ -47,3 +48,28 @@ def test_numbers_past_32_bits_are_refused(ops, cuda):
         for n in (2 ** 31, 2 ** 32, 2 ** 32 + 200, -2 ** 32):
             with pytest.raises(ValueError, match="32 bits"):
                 call(n)
+
+
+@pytest.mark.parametrize("through_host", [False, True])
+def test_a_sequence_that_forks_inside_a_page(ops, cuda, through_host):
+    """Two sequences share 21 tokens; the partly filled page is copied (or brought back
+    from the host), then both append and attend."""
+    H, Hq, D, old, new = 2, 8, 128, 21, 5
+    b = Batch(ops, cuda, [old, old], [new, new], H, D, DT["bf16"], seed=1)
+    whole = t32([0, old], cuda)
+    ops.int8_append(b.cache, b.k[:old], b.v[:old], whole, t32([0], cuda), b.bt_t[:1])
+    first, last, fresh = int(b.bt[0, 0]), int(b.bt[0, 1]), int(b.bt[1, 1])
+    b.pool[fresh] = b.pool[last].cpu().to(cuda) if through_host else b.pool[last]
+    b.bt[1, 0] = first
+    b.bt_t = t32(b.bt, cuda)
+    rows = torch.cat([torch.arange(old, old + new), torch.arange(2 * old + new, 2 * (old + new))])
+    at = rows.to(cuda)
+    ops.int8_append(b.cache, b.k[at], b.v[at], t32(b.cu, cuda), t32(b.old, cuda), b.bt_t)
+    q = b.query(Hq)
+    b.check(q, b.attend(q))
+    alone = ops.Int8PagedCache(H, D, 2)  # the second sequence's tokens without sharing
+    k, v = (torch.cat([x[:old], x[at[new:]]]) for x in (b.k, b.v))
+    ops.int8_append(alone, k, v, t32([0, old + new], cuda), t32([0], cuda), t32([[0, 1]], cuda))
+    assert torch.equal(
+        ops.int8_attend(alone, q[new:], t32([0, new], cuda), t32([[0, 1]], cuda), t32([26], cuda)),
+        ops.int8_attend(b.cache, q[new:], t32([0, new], cuda), b.bt_t[1:].contiguous(), t32([26], cuda)))

@@ -33,9 +33,11 @@ void decode_splits(Int8Splits& sp, int num_seqs, int num_kv_heads, int grp, int 
   sp.ctas = pairs >= kSlots
                 ? kSlots
                 : static_cast<int>(std::max<long long>(1, std::min<long long>(kSlots, pairs * steps)));
-  // contexts of 4 steps or less are not cut: 8 heads of 64 channels, 512 tokens: 7.5
-  // us whole, 9.0 us in 4 parts; 8 heads of 128, 2048 tokens in parts of one
-  // step 9.2 us, of four 11.8 us
+  // Contexts of 4 steps (512 tokens) or less are not cut.  8 kv heads, whole and in parts
+  // of one step, us: 1 sequence, heads of 64, 256 tokens 5.6 and 7.3, 512 7.1 and 8.4, 640
+  // 7.8 and 8.7, 1024 10.0 and 9.2; heads of 128 6.4 and 8.3, 8.2 and 8.7, 9.2 and 9.1,
+  // 11.7 and 9.7; 16 sequences, heads of 128, 4 q heads each: 7.0 and 9.6, 10.1 and 11.6,
+  // 11.3 and 16.2, 14.7 and 17.3, 2048 tokens 24.2 and 21.8.
   sp.least = steps <= 4 ? static_cast<int>(std::max<long long>(1, steps)) : 1;
   sp.rows = static_cast<int>(std::min<long long>(kInt8DecodeRows, static_cast<long long>(max_q) * grp));
 }

@@ -798,7 +798,9 @@ class _RopeAxes(torch.autograd.Function):
 
 class Int8PagedCache:
     """Device buffer of one layer's paged int8 cache: pool [num_pages,
-    n_kv_heads, page_bytes] uint8, allocated zeroed, or the caller's (pool=)."""
+    n_kv_heads, page_bytes] uint8, allocated zeroed, or the caller's (pool=).  A
+    page is pool[i]: pool[dst] = pool[src] copies it (a sequence that forks inside
+    a page), pool[i].cpu() takes it to the host."""
 
     def __init__(self, n_kv_heads: int, head_dim: int, num_pages: Optional[int] = None,
                  device="cuda", pool: Optional[torch.Tensor] = None):
