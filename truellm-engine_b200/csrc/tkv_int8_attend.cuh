@@ -18,7 +18,10 @@ namespace tkv {
 // that computed it and is a lower bound after them, which is the safe side: e only gets
 // too small, which a weight past 2^15 shows.  So every weight is within 2^-11 of itself
 // or 2^-25 of the row's largest p s.  Where c is more than kInt8Far (p 2^c nears the ends of
-// 32 bits), weights are 2^(score - m + log2 s + 5 - e) instead.
+// 32 bits), weights are 2^(score - m + log2 s + 5 - e) instead.  Measured with no such
+// row, with a loud token that all rows see and hardly weigh, and with one past kInt8Far:
+// 8 chunks of 512 tokens behind 4096 339, 349 and 981 us; 8 rows behind 8192 95, 96 and
+// 96 us; 16 rows behind 60000 75, 81 and 81 us.
 constexpr float kInt8Lazy = 10.f;
 constexpr float kInt8LazyWeight = 1024.f;  // 2^kInt8Lazy
 constexpr float kInt8WeightUp = 32.f;     // 2^kInt8WeightExp

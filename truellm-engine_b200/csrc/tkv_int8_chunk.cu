@@ -20,7 +20,7 @@
 // there is room for one buffer only, and every warpgroup then waits for its
 // products' latency at each tile (measured: 4800 cycles per 128 tokens).
 // Measured, 32 q heads on 8 kv heads of 128 channels: 8 chunks of 512 tokens behind
-// 4096 in 336 us, 868 TFLOP/s.  A tile of 256 rows takes 1900 cycles, of which the
+// 4096 in 340 us, 858 TFLOP/s.  A tile of 256 rows takes 1900 cycles, of which the
 // products are 1280; the two softmax warps of a scheduler take 1550 for the weights
 // (exponentials alone 1024) and 300 to wait and signal.  A CTA's start (query rows,
 // the first tile, whose reference needs a pass for the maximum) and end take

@@ -22,12 +22,12 @@
 // the sum is that of the CTAs, so the result does not depend on who is last.
 //
 // Bound by memory: 33 bytes a token, head and 16 channels of keys and values.  64
-// sequences of 1024 to 8192 tokens, 8 kv heads of 128 channels, 4 q heads each: 99 us,
-// 5.8 TB/s.  Equal runs of every context instead of one row of steps: 174, 123, 107,
+// sequences of 1024 to 8192 tokens, 8 kv heads of 128 channels, 4 q heads each: 97 us,
+// 6.0 TB/s.  Equal runs of every context instead of one row of steps: 174, 123, 107,
 // 103, 100 and 119 us with runs of 16, 32, 64, 128, 256 and 384 pages, and another
 // best length for every call.  More than one range a resident CTA: 101 to 106 us.
 // Up to 8 query rows take one column tile of the products and 16 rows two (2 x
-// 60000 tokens: 58 and 74 us); the chunk kernel takes 106 us for 20 rows of them.
+// 60000 tokens: 58 and 75 us); the chunk kernel takes 106 us for 20 rows of them.
 #include <atomic>
 
 #include "tkv_int8.cuh"
