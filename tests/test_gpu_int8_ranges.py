@@ -205,3 +205,22 @@ def test_keys_near_the_ends_of_the_type(ops, cuda, new, e, small):
     want = attend64(f64(q), k, v, 130 + np.arange(new), scale, 0)
     off, lim = np.abs(f64(out) - want[0]), bound(*want, 128, BF16)
     assert (off <= lim).all()
+
+
+@pytest.mark.parametrize("new,old,block", [(1, 300, 32), (4, 300, 32), (1, 5000, 600), (3, 5000, 600),
+                                           (40, 5000, 700), (150, 1000, 256)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_parts_whose_scores_and_values_are_far_apart(ops, cuda, new, old, block, D):
+    """Blocks of tokens in turn 2^80 louder and quieter, with scores as far the other way,
+    so that every block counts for as much: within a warp's share, between the warps of
+    a CTA and between the parts of a context."""
+    b = Batch(ops, cuda, [old], [new], 1, D, BF16, seed=8)
+    n = int(b.lens[0])
+    e = torch.where(torch.arange(n, device=cuda) // block % 2 == 0, 80.0, -80.0).double()
+    b.v[:] = (b.v.double() * (2.0 ** e)[:, None, None]).to(BF16)
+    x = -e * math.log(2.0) / scale_of(D) / D
+    b.k[:] = (x[:, None, None] * torch.ones(D, device=cuda)).to(BF16)
+    b.fill()
+    q = (torch.ones(new, 4, D, device=cuda) + 0.001 * b.query(4).float()).to(BF16)
+    for window in (0, 2 * block + 50):
+        check(b, q, b.attend(q, window), window, rows=5)

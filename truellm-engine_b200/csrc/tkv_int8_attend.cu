@@ -5,7 +5,7 @@
 // the group) is the decode kernel's, any other the chunk kernel's; both read the
 // lengths on the device, so one call serves a batch that mixes them.  A call
 // whose largest sequence has 16 rows or less launches the decode kernel alone.  (2 x
-// 60000 tokens, 4 q heads a kv head: 16 rows 75 us by the decode kernel, 20 rows 106
+// 60000 tokens, 4 q heads a kv head: 16 rows 78 us by the decode kernel, 20 rows 106
 // us by the other, whose time does not fall with the rows.)
 #include <limits.h>
 

@@ -42,7 +42,7 @@ struct Int8Splits {
   int ctas, least;      // CTAs at most; steps of a CTA at least
   int rows;             // the largest row count the launch may meet
   unsigned int* count;  // [ctas], zero between launches: of the pair begun there
-  float* part_ml;       // [2 ctas][row block][2]  (m in log2 units, l)
+  float* part_ml;       // [2 ctas][row block][2]  (m in log2 units, sqrt(l))
   float* part_o;        // [2 ctas][row block][D]  normalised
 };
 
@@ -53,7 +53,7 @@ constexpr int kInt8ChunkRows = 256;
 constexpr int kInt8ChunkSMs = 148;  // CTAs at a time: one per SM
 struct Int8ChunkSplits {
   int whole, n, row_tiles;
-  float* part_ml;  // [item - whole][run][256][2]
+  float* part_ml;  // [item - whole][run][256][2]  (m, sqrt(l))
   float* part_o;   // [item - whole][run][256][D]  normalised
 };
 struct Int8ChunkItem {
@@ -146,6 +146,19 @@ __device__ __forceinline__ float int8_row_exponent(float top, float m, float E) 
   if (m == -INFINITY) return E;
   const float e = fminf(fmaxf(ceilf(top - m), -126.f), 126.f);
   return E - e > kInt8Quiet ? e : E;
+}
+
+__device__ __forceinline__ float int8_sqrt(float x) {
+  float y;
+  asm("sqrt.approx.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+// A part of a row in a join: its outputs count times u^2, u = sqrt(l) 2^((m - M) / 2), M the
+// largest m.  Outputs are multiplied by u twice: a part whose m lies 2^-126 and more below
+// may hold values that are louder by as much.  Parts are stored with sqrt(l); its last bit
+// does not matter, as the sum of the weights has the same.
+__device__ __forceinline__ float int8_part_root(float root_l, float m, float M) {
+  return root_l * fast_exp2(0.5f * (m - (M == -INFINITY ? 0.f : M)));
 }
 
 // four consecutive channels of an output row, rounded once

@@ -846,7 +846,7 @@ __global__ void __launch_bounds__(kCtaThreads, 1)
         }
       }
       if (runs > 1 && valid)
-        *reinterpret_cast<float2*>(sp.part_ml + (slot0 + ctid) * 2) = make_float2(m, l);
+        *reinterpret_cast<float2*>(sp.part_ml + (slot0 + ctid) * 2) = make_float2(m, int8_sqrt(l));
     }
     }
   }
@@ -872,16 +872,15 @@ __global__ void __launch_bounds__(256) int8_chunk_join_kernel(const Int8AttendAr
   const long long slot0 = static_cast<long long>(item) * sp.n * kSoftmax + r;
   float M = -INFINITY;
   for (int i = 0; i < sp.n; ++i) M = fmaxf(M, __ldcg(sp.part_ml + (slot0 + static_cast<long long>(i) * kSoftmax) * 2));
-  const float ref = M == -INFINITY ? 0.f : M;
   float W = 0.f, acc[D / 32] = {};
   for (int i = 0; i < sp.n; ++i) {
     const long long slot = slot0 + static_cast<long long>(i) * kSoftmax;
     const float2 ml = __ldcg(reinterpret_cast<const float2*>(sp.part_ml + slot * 2));
-    const float w = ml.y * fast_exp2(ml.x - ref);
-    W += w;
+    const float u = int8_part_root(ml.y, ml.x, M);
+    W = fmaf(u, u, W);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
-      acc[c] = fmaf(w, __ldcg(sp.part_o + slot * D + (D / 32) * lane + c), acc[c]);
+      acc[c] = fmaf(u, __ldcg(sp.part_o + slot * D + (D / 32) * lane + c) * u, acc[c]);
   }
   const float inv = W == 0.f ? 0.f : 1.f / W;
   const uint32_t tok = rho / grp;

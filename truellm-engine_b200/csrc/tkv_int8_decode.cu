@@ -27,7 +27,7 @@
 // 103, 100 and 119 us with runs of 16, 32, 64, 128, 256 and 384 pages, and another
 // best length for every call.  More than one range a resident CTA: 101 to 106 us.
 // Up to 8 query rows take one column tile of the products and 16 rows two (2 x
-// 60000 tokens: 58 and 75 us); the chunk kernel takes 106 us for 20 rows of them.
+// 60000 tokens: 58 and 78 us); the chunk kernel takes 106 us for 20 rows of them.
 #include <atomic>
 
 #include "tkv_int8.cuh"
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
         const float vs = int8_pow2(int8_scale_exponent(vinv) - s_row[warp][r].y) / kInt8WeightUp;
         if (g == 0) {
           s_ml[warp][r][0] = m[nt][e];
-          s_ml[warp][r][1] = sum;
+          s_ml[warp][r][1] = int8_sqrt(sum);
         }
         float* dst = so + (warp * RB + r) * D + 4 * g;
 #pragma unroll
@@ -518,28 +518,30 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
     const int ns = c1 - c0 + 1, slot = 2 * me + (me == c0 ? 1 : 0);
     for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
       const int r = i / (D / 4), c = i % (D / 4) * 4;
-      float M = -INFINITY, W = 0.f, wt[kWPC];
+      float M = -INFINITY, W = 0.f, u[kWPC];
 #pragma unroll
       for (int w = 0; w < kWPC; ++w) M = fmaxf(M, s_ml[w][r][0]);
-      const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll
-      for (int w = 0; w < kWPC; ++w) W += wt[w] = s_ml[w][r][1] * fast_exp2(s_ml[w][r][0] - ref);
+      for (int w = 0; w < kWPC; ++w) {
+        u[w] = int8_part_root(s_ml[w][r][1], s_ml[w][r][0], M);
+        W = fmaf(u[w], u[w], W);
+      }
       const float inv = W == 0.f ? 0.f : 1.f / W;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kWPC; ++w) {
         const float4 v = *reinterpret_cast<const float4*>(so + (w * RB + r) * D + c);
-        const float f = wt[w] * inv;
-        acc.x = fmaf(f, v.x, acc.x);
-        acc.y = fmaf(f, v.y, acc.y);
-        acc.z = fmaf(f, v.z, acc.z);
-        acc.w = fmaf(f, v.w, acc.w);
+        const float f = u[w] * inv;
+        acc.x = fmaf(f, v.x * u[w], acc.x);
+        acc.y = fmaf(f, v.y * u[w], acc.y);
+        acc.z = fmaf(f, v.z * u[w], acc.z);
+        acc.w = fmaf(f, v.w * u[w], acc.w);
       }
       if (ns == 1) {
         int8_store4(a, (static_cast<int64_t>(q0 + r / a.grp) * a.num_q_heads + h * a.grp + r % a.grp) * D + c, acc);
       } else {
         *reinterpret_cast<float4*>(sp.part_o + static_cast<int64_t>(slot * RB + r) * D + c) = acc;
-        if (c == 0) *reinterpret_cast<float2*>(sp.part_ml + (slot * RB + r) * 2) = make_float2(M, W);
+        if (c == 0) *reinterpret_cast<float2*>(sp.part_ml + (slot * RB + r) * 2) = make_float2(M, int8_sqrt(W));
       }
     }
     // ---- join the parts: the CTA that counts the last one ----
@@ -557,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
     }
     if (last) {
       __threadfence();
-      float* const sw = reinterpret_cast<float*>(smem);  // [part][row] weights
+      float* const su = reinterpret_cast<float*>(smem);  // [part][row] roots of weights
       auto part = [&](int i) { return i == 0 ? 2 * c0 + 1 : 2 * (c0 + i); };
       for (int r = warp; r < rows; r += kWPC) {
         auto load = [&](int i) {
@@ -568,13 +570,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
         for (int i = lane + 32; i < ns; i += 32) M = fmaxf(M, load(i).x);
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-        const float ref = M == -INFINITY ? 0.f : M;
         float W = 0.f;
         for (int i = lane; i < ns; i += 32) {
           const float2 ml = i == lane ? own : load(i);
-          const float w = ml.y * fast_exp2(ml.x - ref);
-          sw[i * RB + r] = w;
-          W += w;
+          const float u = int8_part_root(ml.y, ml.x, M);
+          su[i * RB + r] = u;
+          W = fmaf(u, u, W);
         }
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) W += __shfl_xor_sync(0xffffffffu, W, d);
@@ -588,11 +589,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSM)
         for (int k = 0; k < ns; ++k) {
           const float4 v = __ldcg(reinterpret_cast<const float4*>(
               sp.part_o + static_cast<int64_t>(part(k) * RB + r) * D + c));
-          const float f = sw[k * RB + r];
-          acc.x = fmaf(f, v.x, acc.x);
-          acc.y = fmaf(f, v.y, acc.y);
-          acc.z = fmaf(f, v.z, acc.z);
-          acc.w = fmaf(f, v.w, acc.w);
+          const float u = su[k * RB + r];
+          acc.x = fmaf(u, v.x * u, acc.x);
+          acc.y = fmaf(u, v.y * u, acc.y);
+          acc.z = fmaf(u, v.z * u, acc.z);
+          acc.w = fmaf(u, v.w * u, acc.w);
         }
         const float inv = s_ml[0][r][0];
         acc.x *= inv;
